@@ -38,7 +38,9 @@ typedef enum {
     PMOE_Q4_K = 12,
     PMOE_Q5_K = 13,
     PMOE_Q6_K = 14,
-    PMOE_BF16 = 30
+    PMOE_I8 = 24,       /* rows in 8 bits with f32 scales: pmoe_add_rms_norm_q8 only */
+    PMOE_BF16 = 30,
+    PMOE_F8_E4M3 = 256  /* the same in 8-bit floats; not a GGML id */
 } pmoe_dtype;
 
 typedef enum {
@@ -303,6 +305,66 @@ int pmoe_dequantize(int device, int dtype, const void *blocks, size_t n_elems, f
  * f32 throughout; weight NULL = all ones. */
 int pmoe_add_rms_norm(int device, const float *resid_in, const float *delta, const float *weight,
                       int n, int H, float eps, float *resid_out, float *y, void *stream);
+
+/*
+ * pmoe_add_rms_norm with the normalised row in 8 bits and a scale per group of values: what a host that moves rows
+ * between GPUs or multiplies them in 8 bits does next anyway (the reference quantises a mat-mul's rows inside the
+ * mat-mul, models/with_tracing.rs:324-335).
+ *   r = resid_in + delta, rounded to the residual's type (delta may be NULL),  resid_out = r (may be NULL or resid_in),
+ *   v = r / sqrt(mean(r^2) + eps) * weight  (weight f32 [H], NULL = all ones),
+ *   per group: scale = max |v| / 127 (q_dtype PMOE_I8) or / 448 (PMOE_F8_E4M3),  q = v / scale rounded to nearest even;
+ *   a group of zeros has scale 0 and zeros.  values (NULL = not wanted) = q * scale in F32 or BF16.
+ * resid_in, resid_out [n, H] F32 or BF16; delta [n, H] F32 or BF16; q [n, H] bytes; scales [n, ceil(H / group)] f32.
+ * group is 32, 64, 128, 256 or 0 for the whole row (the last group of a row may be short); H <= 16384.  A group that
+ * holds an infinity or a NaN has a scale that is not finite, and zeros.  Sums and the norm are f32.
+ */
+int pmoe_add_rms_norm_q8(int device, const void *resid_in, int resid_dtype, const void *delta, int delta_dtype, const float *weight,
+                         int n, int H, float eps, int group, void *resid_out, int q_dtype, void *q, float *scales, void *values,
+                         int values_dtype, void *stream);
+
+/*
+ * Rows to the experts and back, as operators of their own, for a host that runs something else than this library's
+ * experts on the sorted rows (group_tokens_by_expert and the expert loop, ops.rs:74-157, qwen3_next.rs:2037-2050) or that
+ * trains.  A pair is p = t * top_k + j; it is kept when 0 <= idx[p] - expert_base < E (expert_base, E: the slice of an
+ * expert-parallel rank; all other ids, negative ones as int32 among them, are skipped).
+ *
+ * pmoe_sort_pairs: offsets [E + 1] = number of kept pairs of the experts before e; place [n, top_k] = the pair's row in
+ * expert order, -1 when it is skipped; order [n * top_k] = the pair at a row, -1 from row offsets[E] on.  Stable: pairs
+ * of one expert stay in ascending order.  order or place may be NULL.  E <= 4096, n * top_k <= 2^30.
+ */
+int pmoe_sort_pairs(int device, const uint32_t *idx, int n, int top_k, int expert_base, int E, int *order, int *place, int *offsets,
+                    void *stream);
+
+/* out[place[p]] = x[p / top_k] for every kept pair, rows of row_bytes bytes of any type; the rows from offsets[E] on are
+ * zeroed.  x [n, row_bytes], out [n * top_k, row_bytes], which must not overlap. */
+int pmoe_dispatch_rows(int device, const void *x, size_t row_bytes, int n, int top_k, const int *place, const int *offsets, int E,
+                       void *out, void *stream);
+
+/* out[t] = sum_j w[t, j] * rows[place[t, j]] (+ extra[t]), f32 sums in slot order, rounded once; pairs whose place is
+ * outside [0, n_rows) contribute nothing and their rows are not read.  w NULL = all ones, which is the gradient of
+ * pmoe_dispatch_rows.  rows [n_rows, H], extra [n, H] (NULL = none), out [n, H], each F32 or BF16; extra may be out when
+ * their types are equal (MoeBlock::forward_with_stats adds the shared expert there, qwen3_next.rs:1932-1937). */
+int pmoe_combine_rows(int device, const void *rows, int rows_dtype, int n_rows, int n, int top_k, int H, const int *place,
+                      const float *w, const void *extra, int extra_dtype, void *out, int out_dtype, void *stream);
+
+/* Gradient of pmoe_combine_rows: grad_rows[place[p]] = w[p] * grad_out[t] (type of rows, the rows from offsets[E] on are
+ * zeroed), grad_w[p] = <grad_out[t], rows[place[p]]> (f32, 0 for a skipped pair); extra's gradient is grad_out itself.
+ * grad_rows or grad_w may be NULL; rows may be NULL without grad_w.  rows and grad_rows [n * top_k, H] must not overlap. */
+int pmoe_combine_rows_grad(int device, const void *grad_out, int grad_dtype, const void *rows, int rows_dtype, int n, int top_k, int H,
+                           const int *place, const int *offsets, int E, const float *w, void *grad_rows, float *grad_w, void *stream);
+
+/*
+ * Low-rank adapters of many requests beside one projection (the low-rank update of QMatMul, models/with_tracing.rs:103-337,
+ * which the reference holds once and merges): out[t] = base[t] + scales[i] * B_i (A_i x[t]), i = ids[t]; a row whose id is
+ * outside [0, n_adapters) gets base[t].  x [n, K] and base, out [n, N] F32 or BF16 (base and out alike; out may be base);
+ * a [n_adapters, rank, K] and b [n_adapters, N, rank] BF16; scales [n_adapters] f32 or NULL (all ones); ids [n] int32.
+ * order and offsets: pmoe_sort_pairs of ids (top_k 1, expert_base 0, E = n_adapters), which a host computes once for all
+ * projections of a batch, or both NULL for n <= 1024.  K and N multiples of 8, rank a multiple of 8 up to 128, all
+ * pointers 16-byte aligned.  Products are exact bf16 products summed in f32; f32 rows lose nothing.
+ */
+int pmoe_adapters_add(int device, const void *base, const void *x, int x_dtype, int n, int K, int N, int rank, int n_adapters,
+                      const void *a, const void *b, const float *scales, const int *ids, const int *order, const int *offsets, void *out,
+                      int out_dtype, void *stream);
 
 /*
  * Home-rank side of the expert-parallel combine: out[t] = sum_r parts[r][t] (+ extra[t]).

@@ -5,6 +5,7 @@ import ctypes as C
 import os
 
 F32, F16, Q8_0, Q2_K, Q3_K, Q4_K, Q5_K, Q6_K, BF16 = 0, 1, 8, 10, 11, 12, 13, 14, 30
+I8, F8_E4M3 = 24, 256
 TRACE_PHASES = 8
 
 STATUS_NAMES = {
@@ -73,6 +74,12 @@ SYMBOLS = [
     ("pmoe_dequantize", _I, [_I, _I, _V, _Z, _V, _V]),
     ("pmoe_reduce_rows", _I, [_I, _V, _I, _V, _I, _I, _I, _V, _I, _V]),
     ("pmoe_add_rms_norm", _I, [_I, _V, _V, _V, _I, _I, C.c_float, _V, _V, _V]),
+    ("pmoe_add_rms_norm_q8", _I, [_I, _V, _I, _V, _I, _V, _I, _I, C.c_float, _I, _V, _I, _V, _V, _V, _I, _V]),
+    ("pmoe_sort_pairs", _I, [_I, _V, _I, _I, _I, _I, _V, _V, _V, _V]),
+    ("pmoe_dispatch_rows", _I, [_I, _V, _Z, _I, _I, _V, _V, _I, _V, _V]),
+    ("pmoe_combine_rows", _I, [_I, _V, _I, _I, _I, _I, _I, _V, _V, _V, _I, _V, _I, _V]),
+    ("pmoe_combine_rows_grad", _I, [_I, _V, _I, _V, _I, _I, _I, _I, _V, _V, _I, _V, _V, _V, _V]),
+    ("pmoe_adapters_add", _I, [_I, _V, _V, _I, _I, _I, _I, _I, _I, _V, _V, _V, _V, _V, _V, _V, _I, _V]),
     ("pmoe_layer_status", _I, [_V, _V]),
     ("pmoe_layer_trace", _I, [_V, _I]),
     ("pmoe_layer_trace_read", _I, [_V, _V]),

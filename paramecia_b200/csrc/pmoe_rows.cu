@@ -1,0 +1,329 @@
+// Rows to the experts and back as operators of their own: the stable sort of the (token, slot) pairs by expert, the
+// dispatch of a token's row to its places in expert order, the weighted sum back, and the gradients of both.
+//
+// The block's own kernels do the same inside (launch_group, launch_combine) without ever writing the sorted rows; these
+// entry points are for hosts that run something else between the two: their own experts, per-expert adapters, a
+// training step.  With key_p = idx_p - base kept where 0 <= key_p < E:
+//   offsets[e] = #{p kept : key_p < e},  place_p = offsets[key_p] + #{q < p : key_q = key_p}  (-1: not kept),
+//   order[place_p] = p  (-1 from offsets[E] on).
+// The order is stable, so all of it is a function of idx alone (the block's grouping leaves the order inside an expert
+// to its atomics).
+#include "pmoe_internal.h"
+#include "pmoe_vec.cuh"
+
+namespace pmoe {
+
+// ---------------------------------------------------------------- sort
+// A counting sort in one CTA.  Warp w owns the w-th run of consecutive pairs, takes it 32 pairs at a time, and ranks the
+// pairs of a step among those of the same expert with __match_any_sync: ranks inside the step, steps, warps are three
+// levels of the same order, so the result is stable without atomics.
+//   1. cnt[w][e]  pairs of expert e in warp w's run
+//   2. exclusive scan over (e, w): cnt[w][e] becomes the place of that warp's first pair of e
+//   3. the runs once more: place = cnt[w][e] + rank inside the step
+constexpr int SORT_MAX_E = 4096;
+constexpr int SORT_THREADS = 1024;
+
+__global__ void __launch_bounds__(SORT_THREADS) k_sort_pairs(const uint32_t *__restrict__ idx, int P, uint32_t base, int E, int warps,
+                                                             int run, int *__restrict__ order, int *__restrict__ place,
+                                                             int *__restrict__ offsets)
+{
+    extern __shared__ int cnt[];   // [warps][E]
+    __shared__ int warp_tot[32];
+    const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+    for (int i = tid; i < warps * E; i += SORT_THREADS) cnt[i] = 0;
+    pdl_wait();
+    pdl_launch_dependents();
+    __syncthreads();
+
+    const int p0 = min((int64_t)P, (int64_t)w * run), p1 = w < warps ? min((int64_t)P, (int64_t)p0 + run) : p0;
+    for (int p = p0; p < p1; p += 32) {
+        const uint32_t key = p + lane < p1 ? idx[p + lane] - base : 0xffffffffu;
+        const unsigned same = __match_any_sync(0xffffffffu, key);
+        if (key < (uint32_t)E && lane == __ffs(same) - 1) cnt[w * E + key] += __popc(same);
+        __syncwarp();
+    }
+    __syncthreads();
+
+    // thread t scans experts [t*q, t*q + q)
+    const int q = (E + SORT_THREADS - 1) / SORT_THREADS;
+    int mine = 0;
+    for (int e = tid * q; e < min(E, tid * q + q); e++)
+        for (int v = 0; v < warps; v++) mine += cnt[v * E + e];
+    int incl = mine;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, incl, off);
+        if (lane >= off) incl += y;
+    }
+    if (lane == 31) warp_tot[w] = incl;
+    __syncthreads();
+    int before = incl - mine, total = 0;
+    for (int v = 0; v < 32; v++) {
+        if (v < w) before += warp_tot[v];
+        total += warp_tot[v];
+    }
+    for (int e = tid * q; e < min(E, tid * q + q); e++) {
+        offsets[e] = before;
+        for (int v = 0; v < warps; v++) {
+            const int c = cnt[v * E + e];
+            cnt[v * E + e] = before;
+            before += c;
+        }
+    }
+    if (tid == 0) offsets[E] = total;
+    __syncthreads();
+
+    for (int p = p0; p < p1; p += 32) {
+        const uint32_t key = p + lane < p1 ? idx[p + lane] - base : 0xffffffffu;
+        const unsigned same = __match_any_sync(0xffffffffu, key);
+        const int rank = __popc(same & ((1u << lane) - 1));
+        int at = -1;
+        if (key < (uint32_t)E) at = cnt[w * E + key] + rank;
+        __syncwarp();
+        if (key < (uint32_t)E && rank == 0) cnt[w * E + key] += __popc(same);
+        __syncwarp();
+        if (p + lane < p1) {
+            if (place) place[p + lane] = at;
+            if (order && at >= 0) order[at] = p + lane;
+        }
+    }
+    if (order)
+        for (int p = total + tid; p < P; p += SORT_THREADS) order[p] = -1;
+}
+
+cudaError_t launch_sort_pairs(const uint32_t *idx, int P, int base, int E, int *order, int *place, int *offsets, cudaStream_t s)
+{
+    // the counts of all warps stay below 128 KB; no more warps than there are steps of 32 pairs
+    int warps = E <= 1024 ? 32 : 8;
+    warps = min(warps, max(1, (P + 31) / 32));
+    const int run = (((P + warps - 1) / warps) + 31) / 32 * 32;
+    const size_t smem = (size_t)warps * E * sizeof(int);
+    cudaError_t e = cudaFuncSetAttribute(k_sort_pairs, cudaFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024);
+    if (e != cudaSuccess) return e;
+    e = launch_pdl(k_sort_pairs, dim3(1), dim3(SORT_THREADS), smem, s, idx, P, (uint32_t)base, E, warps, run, order, place, offsets);
+    count_launch();
+    return e;
+}
+
+// ---------------------------------------------------------------- dispatch
+// Rows are moved as bytes, so any element type goes: one CTA per token reads the row once and writes it to the token's
+// places.  The rows behind the last kept pair are zeroed by the same CTAs.
+template <typename V>
+__global__ void __launch_bounds__(256) k_dispatch_rows(const V *__restrict__ x, int units, int top_k, int P, const int *__restrict__ place,
+                                                       const int *__restrict__ offsets, int E, V *__restrict__ out)
+{
+    pdl_wait();
+    pdl_launch_dependents();
+    const int t = blockIdx.x;
+    const int *pl = place + (size_t)t * top_k;
+    for (int u = threadIdx.x; u < units; u += 256) {
+        const V v = x[(size_t)t * units + u];
+        for (int j = 0; j < top_k; j++) {
+            const int at = pl[j];
+            if ((unsigned)at < (unsigned)P) out[(size_t)at * units + u] = v;
+        }
+    }
+    for (int64_t r = (int64_t)max(0, offsets[E]) + t; r < P; r += gridDim.x)
+        for (int u = threadIdx.x; u < units; u += 256) out[(size_t)r * units + u] = V{};
+}
+
+cudaError_t launch_dispatch_rows(const void *x, size_t row_bytes, int n, int top_k, const int *place, const int *offsets, int E,
+                                 void *out, cudaStream_t s)
+{
+    const uintptr_t a = (uintptr_t)x | (uintptr_t)out | row_bytes;
+    auto go = [&](auto v) {
+        using V = decltype(v);
+        return launch_pdl(k_dispatch_rows<V>, dim3(n), dim3(256), 0, s, (const V *)x, (int)(row_bytes / sizeof(V)), top_k, n * top_k,
+                          place, offsets, E, (V *)out);
+    };
+    count_launch();
+    return a % 16 == 0 ? go(uint4{}) : a % 8 == 0 ? go(uint2{}) : a % 4 == 0 ? go(0u) : a % 2 == 0 ? go((uint16_t)0) : go((uint8_t)0);
+}
+
+// ---------------------------------------------------------------- combine
+// out_t = extra_t + sum_j w_tj rows[place_tj], f32 in slot order, one CTA per token.  Without weights it is the
+// gradient of the dispatch.  (extra may be out: a thread reads the elements it later writes.)
+template <int U, typename RT, typename ET, typename OT>
+__global__ void __launch_bounds__(256) k_combine_rows(const RT *__restrict__ rows, int H, int top_k, int n_rows,
+                                                      const int *__restrict__ place, const float *__restrict__ w, const ET *extra,
+                                                      OT *out)
+{
+    pdl_wait();
+    pdl_launch_dependents();
+    const int t = blockIdx.x;
+    for (int h = threadIdx.x * U; h < H; h += 256 * U) {
+        float acc[U] = {};
+        for (int j = 0; j < top_k; j++) {
+            const int at = place[(size_t)t * top_k + j];
+            if ((unsigned)at >= (unsigned)n_rows) continue;
+            const float wt = w ? w[(size_t)t * top_k + j] : 1.f;
+            float v[U];
+            load_units<U>(rows + (size_t)at * H + h, v);
+#pragma unroll
+            for (int i = 0; i < U; i++) acc[i] = fmaf(wt, v[i], acc[i]);
+        }
+        if (extra) {
+            float v[U];
+            load_units<U>(extra + (size_t)t * H + h, v);
+#pragma unroll
+            for (int i = 0; i < U; i++) acc[i] += v[i];
+        }
+        store_units<U>(out + (size_t)t * H + h, acc);
+    }
+}
+
+cudaError_t launch_combine_rows(const void *rows, int rows_dtype, int n_rows, int n, int top_k, int H, const int *place, const float *w,
+                                const void *extra, int extra_dtype, void *out, int out_dtype, cudaStream_t s)
+{
+    count_launch();
+    const bool wide = H % 8 == 0 && aligned16(rows) && aligned16(extra) && aligned16(out);
+    return with_type(rows_dtype, [&](auto *rp) {
+        return with_type(extra_dtype, [&](auto *ep) {
+            return with_type(out_dtype, [&](auto *op) {
+                using RT = std::remove_pointer_t<decltype(rp)>;
+                using ET = std::remove_pointer_t<decltype(ep)>;
+                using OT = std::remove_pointer_t<decltype(op)>;
+                return launch_pdl(wide ? k_combine_rows<8, RT, ET, OT> : k_combine_rows<1, RT, ET, OT>, dim3(n), dim3(256), 0, s,
+                                  (const RT *)rows, H, top_k, n_rows, place, w, (const ET *)extra, (OT *)out);
+            });
+        });
+    });
+}
+
+// ---------------------------------------------------------------- gradient of combine
+// grad_rows[place_p] = w_p grad_out[t],  grad_w_p = <grad_out[t], rows[place_p]> for pair p = (t, j): one warp per pair.
+template <int U, typename GT, typename RT>
+__global__ void __launch_bounds__(256) k_combine_grad(const GT *__restrict__ grad_out, const RT *__restrict__ rows, int H, int top_k, int P,
+                                                      const int *__restrict__ place, const int *__restrict__ offsets, int E,
+                                                      const float *__restrict__ w, RT *__restrict__ grad_rows, float *__restrict__ grad_w)
+{
+    pdl_wait();
+    pdl_launch_dependents();
+    const int lane = threadIdx.x & 31;
+    const int64_t p = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (p >= P) return;
+    const int at = place[p];
+    const bool kept = (unsigned)at < (unsigned)P;
+    float dot = 0.f;
+    if (kept) {
+        const float wt = w ? w[p] : 1.f;
+        const GT *g = grad_out + (size_t)(p / top_k) * H;
+        for (int h = lane * U; h < H; h += 32 * U) {
+            float a[U], b[U];
+            load_units<U>(g + h, a);
+            if (grad_w) {
+                load_units<U>(rows + (size_t)at * H + h, b);
+#pragma unroll
+                for (int i = 0; i < U; i++) dot = fmaf(a[i], b[i], dot);
+            }
+            if (grad_rows) {
+#pragma unroll
+                for (int i = 0; i < U; i++) a[i] *= wt;
+                store_units<U>(grad_rows + (size_t)at * H + h, a);
+            }
+        }
+    }
+    if (grad_w) {
+#pragma unroll
+        for (int s = 16; s >= 1; s >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, s);
+        if (lane == 0) grad_w[p] = dot;
+    }
+    const int64_t r = (int64_t)max(0, offsets[E]) + p;   // one row behind the last kept pair each
+    if (grad_rows && r < P) {
+        const float zero[U] = {};
+        for (int h = lane * U; h < H; h += 32 * U) store_units<U>(grad_rows + (size_t)r * H + h, zero);
+    }
+}
+
+cudaError_t launch_combine_grad(const void *grad_out, int grad_dtype, const void *rows, int rows_dtype, int n, int top_k, int H,
+                                const int *place, const int *offsets, int E, const float *w, void *grad_rows, float *grad_w,
+                                cudaStream_t s)
+{
+    count_launch();
+    const int P = n * top_k;
+    const bool wide = H % 8 == 0 && aligned16(rows) && aligned16(grad_out) && aligned16(grad_rows);
+    return with_type(grad_dtype, [&](auto *gp) {
+        return with_type(rows_dtype, [&](auto *rp) {
+            using GT = std::remove_pointer_t<decltype(gp)>;
+            using RT = std::remove_pointer_t<decltype(rp)>;
+            return launch_pdl(wide ? k_combine_grad<8, GT, RT> : k_combine_grad<1, GT, RT>, dim3((P + 7) / 8), dim3(256), 0, s,
+                              (const GT *)grad_out, (const RT *)rows, H, top_k, P, place, offsets, E, w, (RT *)grad_rows, grad_w);
+        });
+    });
+}
+
+static int check_pairs(int n, int top_k, int E)
+{
+    if (n < 0 || top_k <= 0 || (int64_t)n * top_k > (1 << 30)) return fail(PMOE_ERR_INVALID_ARG, "n >= 0, top_k >= 1 and n * top_k <= 2^30 are served");
+    if (E <= 0 || E > SORT_MAX_E) return fail(PMOE_ERR_UNSUPPORTED_SHAPE, "1 to %d experts are served (got %d)", SORT_MAX_E, E);
+    return PMOE_OK;
+}
+
+}  // namespace pmoe
+
+using namespace pmoe;
+
+extern "C" {
+
+int pmoe_sort_pairs(int device, const uint32_t *idx, int n, int top_k, int expert_base, int E, int *order, int *place, int *offsets,
+                    void *stream)
+{
+    int rc = check_pairs(n, top_k, E);
+    if (rc) return rc;
+    if (expert_base < 0) return fail(PMOE_ERR_INVALID_ARG, "expert_base must not be negative");
+    if (!offsets || (n && !idx)) return fail(PMOE_ERR_INVALID_ARG, "idx / offsets is NULL");
+    DeviceGuard guard(device);
+    if (!guard.ok) return fail(PMOE_ERR_NO_DEVICE, "cannot select device %d", device);
+    CU(launch_sort_pairs(idx, n * top_k, expert_base, E, order, place, offsets, (cudaStream_t)stream));
+    return PMOE_OK;
+}
+
+int pmoe_dispatch_rows(int device, const void *x, size_t row_bytes, int n, int top_k, const int *place, const int *offsets, int E,
+                       void *out, void *stream)
+{
+    int rc = check_pairs(n, top_k, E);
+    if (rc) return rc;
+    if (!row_bytes || row_bytes > (1u << 30)) return fail(PMOE_ERR_INVALID_ARG, "row_bytes must be 1 to 2^30");
+    if (!n) return PMOE_OK;
+    if (!x || !place || !offsets || !out) return fail(PMOE_ERR_INVALID_ARG, "x / place / offsets / out is NULL");
+    DeviceGuard guard(device);
+    if (!guard.ok) return fail(PMOE_ERR_NO_DEVICE, "cannot select device %d", device);
+    CU(launch_dispatch_rows(x, row_bytes, n, top_k, place, offsets, E, out, (cudaStream_t)stream));
+    return PMOE_OK;
+}
+
+int pmoe_combine_rows(int device, const void *rows, int rows_dtype, int n_rows, int n, int top_k, int H, const int *place,
+                      const float *w, const void *extra, int extra_dtype, void *out, int out_dtype, void *stream)
+{
+    int rc = check_pairs(n, top_k, 1);
+    if (rc) return rc;
+    if (H <= 0 || n_rows < 0) return fail(PMOE_ERR_INVALID_ARG, "bad H / n_rows");
+    if (!f32_or_bf16(rows_dtype) || !f32_or_bf16(out_dtype) || (extra && !f32_or_bf16(extra_dtype)))
+        return fail(PMOE_ERR_UNSUPPORTED_DTYPE, "rows / extra / out must be F32 or BF16");
+    if (!n) return PMOE_OK;
+    if ((n_rows && !rows) || !place || !out) return fail(PMOE_ERR_INVALID_ARG, "rows / place / out is NULL");
+    DeviceGuard guard(device);
+    if (!guard.ok) return fail(PMOE_ERR_NO_DEVICE, "cannot select device %d", device);
+    CU(launch_combine_rows(rows, rows_dtype, n_rows, n, top_k, H, place, w, extra, extra ? extra_dtype : out_dtype, out, out_dtype,
+                           (cudaStream_t)stream));
+    return PMOE_OK;
+}
+
+int pmoe_combine_rows_grad(int device, const void *grad_out, int grad_dtype, const void *rows, int rows_dtype, int n, int top_k, int H,
+                           const int *place, const int *offsets, int E, const float *w, void *grad_rows, float *grad_w, void *stream)
+{
+    int rc = check_pairs(n, top_k, E);
+    if (rc) return rc;
+    if (H <= 0) return fail(PMOE_ERR_INVALID_ARG, "bad H");
+    if (!f32_or_bf16(grad_dtype) || !f32_or_bf16(rows_dtype)) return fail(PMOE_ERR_UNSUPPORTED_DTYPE, "grad_out / rows must be F32 or BF16");
+    if (!n) return PMOE_OK;
+    if (!grad_rows && !grad_w) return fail(PMOE_ERR_INVALID_ARG, "neither grad_rows nor grad_w is asked for");
+    if (!grad_out || !place || !offsets || (grad_w && !rows)) return fail(PMOE_ERR_INVALID_ARG, "grad_out / rows / place / offsets is NULL");
+    DeviceGuard guard(device);
+    if (!guard.ok) return fail(PMOE_ERR_NO_DEVICE, "cannot select device %d", device);
+    CU(launch_combine_grad(grad_out, grad_dtype, rows, rows_dtype, n, top_k, H, place, offsets, E, w, grad_rows, grad_w,
+                           (cudaStream_t)stream));
+    return PMOE_OK;
+}
+
+}  // extern "C"
