@@ -2,61 +2,373 @@
 // batch whose rows belong to different adapters.  base is the shared projection's output (pmoe_qmatmul's, say); a row whose
 // id is outside [0, L) keeps it.  The reference's QMatMul holds one low-rank update and merges it
 // (paramecia-model/src/models/with_tracing.rs:103-337).
+//
+// What bounds it: 2 r (K + N) flops over K x + 2 N out elements a row, at most r flops a byte, below the ridge of the card
+// for every rank served (r <= 128), so the rows' stream from memory is the limit for prompts, and latency for single
+// tokens.  The warp-level matrix instructions are fast enough for that rate and take their operands from registers, where
+// the loads put them: no shared-memory staging of x, A or B at all.
+//
+// One kernel does both products.  A tile of up to T rows of one adapter belongs to a cluster of eight CTAs: each takes an
+// eighth of K for its share of h = A x, the shares are added through distributed shared memory, and each CTA
+// then takes an eighth of the N output columns.  h never goes to memory, and a single token still uses eight SMs.
+#include <cooperative_groups.h>
+
 #include "pmoe_internal.h"
 #include "pmoe_vec.cuh"
 
 namespace pmoe {
 
+namespace cg = cooperative_groups;
+
 constexpr int ADAPTER_MAX_RANK = 128;
 constexpr int ADAPTER_ROWS_UNSORTED = 1024;   // rows that are grouped by id without pmoe_sort_pairs
+constexpr int AD_CTAS = 8;                    // CTAs of a cluster
+constexpr int AD_WARPS = 4;
+constexpr int AD_THREADS = AD_WARPS * 32;
 
-// one CTA per row: h = A x by one warp per rank, then one output column per thread
-template <typename XT, typename OT>
-__global__ void __launch_bounds__(256) k_adapters(const OT *base, const XT *__restrict__ x, int K, int N, int r,
-                                                  const __nv_bfloat16 *__restrict__ a, const __nv_bfloat16 *__restrict__ b,
-                                                  const float *__restrict__ scales, int L, const int *__restrict__ ids, OT *out)
+// c += a b, 16 x 8 x 16, bf16 operands, f32 sums.  Lane l, g = l / 4, q = l % 4: a0 / a1 = rows g / g + 8 at the inner pair
+// (2q, 2q + 1), a2 / a3 the same at inner pair 2q + 8; b0, b1 the same inner pairs of column g; c0, c1 = row g, columns
+// 2q, 2q + 1; c2, c3 = row g + 8.  The inner index is summed over, so any renaming of it that a and b share is allowed:
+// a lane's pairs are taken from consecutive elements (one wide load) instead of the two places the layout names.
+__device__ inline void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
 {
-    __shared__ float h[ADAPTER_MAX_RANK];
-    pdl_wait();
-    pdl_launch_dependents();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const size_t t = blockIdx.x;
-    const int id = ids[t];
-    const bool has = (unsigned)id < (unsigned)L;
-    if (has) {
-        const float s = scales ? scales[id] : 1.f;
-        for (int c = warp; c < r; c += 8) {
-            const __nv_bfloat16 *ar = a + ((size_t)id * r + c) * K;
-            float acc = 0.f;
-            for (int k = lane; k < K; k += 32) acc = fmaf(load_as_float(x, t * K + k), __bfloat162float(ar[k]), acc);
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// A pair of f32 values as PIECES pairs of bf16 whose sum is the value: three hold all 24 bits of it (8 + 8 + 8, each
+// remainder is exact), two hold 16.
+template <int PIECES> __device__ inline void split_pair(float lo, float hi, uint32_t (&w)[PIECES])
+{
 #pragma unroll
-            for (int o = 16; o >= 1; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-            if (lane == 0) h[c] = acc * s;
-        }
-    }
-    __syncthreads();
-    for (int o = threadIdx.x; o < N; o += 256) {
-        float v = load_as_float(base, t * N + o);
-        if (has) {
-            const __nv_bfloat16 *br = b + ((size_t)id * N + o) * r;
-            float acc = 0.f;
-            for (int c = 0; c < r; c++) acc = fmaf(h[c], __bfloat162float(br[c]), acc);
-            v += acc;
-        }
-        store_from_float(out, t * N + o, v);
+    for (int p = 0; p < PIECES; p++) {
+        w[p] = pack_bf16(lo, hi);
+        lo -= __uint_as_float(w[p] << 16);
+        hi -= __uint_as_float(w[p] & 0xffff0000u);
     }
 }
 
-cudaError_t launch_adapters(const void *base, int out_dtype, const void *x, int x_dtype, int n, int K, int N, int r, const void *a,
-                            const void *b, const float *scales, int L, const int *ids, void *out, cudaStream_t s)
+// eight consecutive inner elements of a row as matrix operands: four pairs, in one piece for bf16 and in three for f32
+template <typename XT> struct XFrag;
+template <> struct XFrag<__nv_bfloat16> {
+    static constexpr int PIECES = 1;
+    uint4 v;
+    __device__ void load(const __nv_bfloat16 *p, bool there) { v = there ? *reinterpret_cast<const uint4 *>(p) : make_uint4(0, 0, 0, 0); }
+    __device__ void words(uint32_t (&w)[4][1]) const { w[0][0] = v.x; w[1][0] = v.y; w[2][0] = v.z; w[3][0] = v.w; }
+};
+template <> struct XFrag<float> {
+    static constexpr int PIECES = 3;
+    float4 v0, v1;
+    __device__ void load(const float *p, bool there)
+    {
+        v0 = there ? reinterpret_cast<const float4 *>(p)[0] : make_float4(0.f, 0.f, 0.f, 0.f);
+        v1 = there ? reinterpret_cast<const float4 *>(p)[1] : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    __device__ void words(uint32_t (&w)[4][3]) const
+    {
+        split_pair<3>(v0.x, v0.y, w[0]);
+        split_pair<3>(v0.z, v0.w, w[1]);
+        split_pair<3>(v1.x, v1.y, w[2]);
+        split_pair<3>(v1.z, v1.w, w[3]);
+    }
+};
+
+struct AdapterArgs {
+    int n, K, N, r, L;
+    const __nv_bfloat16 *a, *b;
+    const float *scales;
+    const int *ids, *order, *offsets;
+};
+
+// floats between two rows of h in shared memory: sixteen more where rows would start in the same bank
+__host__ __device__ inline int h_stride(int r16) { return r16 % 32 ? r16 : r16 + 16; }
+
+template <typename OT> __device__ inline void copy_row(const OT *from, OT *to, int units, int first)
 {
+    for (int u = first; u < units; u += AD_CTAS * AD_THREADS) {
+        float v[8];
+        load_units<8>(from + u * 8, v);
+        store_units<8>(to + u * 8, v);
+    }
+}
+
+// T = 16: the four warps of a CTA share the tile's rows and split K and N again.  T = 64: sixteen rows a warp.
+// RT: groups of eight ranks that the accumulators are sized for.
+template <typename XT, typename OT, int T, int RT>
+__global__ void __launch_bounds__(AD_THREADS) k_adapters(AdapterArgs P, const XT *__restrict__ x, const OT *base, OT *out)
+{
+    extern __shared__ __align__(16) float smem[];
+    __shared__ int rows[T];
+    __shared__ int tile_id, tile_rows;
+    __shared__ int all_ids[T == 16 ? ADAPTER_ROWS_UNSORTED : 1];   // without an order T is 16
+    constexpr int SPLIT = T == 16 ? AD_WARPS : 1;   // warps that share rows
+    constexpr int HP = std::is_same<OT, float>::value ? 3 : 2;   // pieces of h: an f32 result keeps all of it, a bf16 result 16 bits
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int c = (int)cluster.block_rank(), slot = blockIdx.x / AD_CTAS;
+    const int r16 = (P.r + 15) / 16 * 16, hs = h_stride(r16);
+    float *part = smem;                       // [AD_WARPS * 16][hs] this CTA's share of h
+    float *h = smem + AD_WARPS * 16 * hs;     // [T][hs]
+    pdl_wait();
+    pdl_launch_dependents();
+
+    // ---- the tile: its adapter and rows.  Every CTA of the cluster finds the same.
+    if (P.order) {
+        // Tile slots of adapter e begin at offsets[e] / T + e: with one slot more than whole multiples of T inside its
+        // range that is never fewer than it has tiles, and needs no scan over the adapters.
+        if (tid < T) rows[tid] = -1;
+        if (tid == 0) {
+            int lo = 0, hi = P.L;     // last e with start(e) <= slot
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) / 2;
+                if (P.offsets[mid] / T + mid <= slot) lo = mid;
+                else hi = mid;
+            }
+            const int first = P.offsets[lo] + (slot - (P.offsets[lo] / T + lo)) * T;
+            tile_id = lo;
+            tile_rows = first;        // for the moment: where the tile begins
+        }
+        __syncthreads();
+        const int first = tile_rows, end = min(P.n, P.offsets[tile_id + 1]);
+        __syncthreads();
+        if (tid < T && first >= 0 && first + tid < end) rows[tid] = P.order[first + tid];
+        if (tid == 0) tile_rows = first >= 0 ? max(0, min(T, end - first)) : 0;
+        __syncthreads();
+        // rows without an adapter are nowhere in the order: the slots pass over the batch once more for them
+        const int t = slot * T + tid;
+        if (__syncthreads_or(tid < T && t < P.n && (unsigned)P.ids[min(t, P.n - 1)] >= (unsigned)P.L) && out != base)
+            for (int t = slot * T; t < min(P.n, slot * T + T); t++)
+                if ((unsigned)P.ids[t] >= (unsigned)P.L) copy_row(base + (size_t)t * P.N, out + (size_t)t * P.N, P.N / 8, c * AD_THREADS + tid);
+        if (tile_rows == 0) return;
+    } else if constexpr (T == 16) {
+        // slot t leads a tile when the number of earlier rows with its id is a multiple of T
+        const int id = P.ids[slot];
+        if ((unsigned)id >= (unsigned)P.L) {
+            if (out != base) copy_row(base + (size_t)slot * P.N, out + (size_t)slot * P.N, P.N / 8, c * AD_THREADS + tid);
+            return;
+        }
+        if (tid < T) rows[tid] = -1;
+        for (int t = tid; t < P.n; t += AD_THREADS) all_ids[t] = P.ids[t];
+        __syncthreads();
+        if (warp == 0) {
+            int before = 0, found = 0;
+            for (int t = 0; t < P.n && found < T; t += 32) {
+                const bool same = t + lane < P.n && all_ids[t + lane] == id;
+                const unsigned m = __ballot_sync(0xffffffffu, same);
+                const unsigned early = t + 32 <= slot ? m : t > slot ? 0u : m & ((1u << (slot - t)) - 1);
+                before += __popc(early);
+                const int at = found + __popc(m & ~early & ((1u << lane) - 1));
+                if (same && !(early >> lane & 1) && at < T) rows[at] = t + lane;
+                found += __popc(m & ~early);
+            }
+            if (lane == 0) {
+                tile_id = id;
+                tile_rows = before % T ? 0 : min(found, T);
+            }
+        }
+        __syncthreads();
+        if (tile_rows == 0) return;
+    }
+    const int id = tile_id, nrows = tile_rows;
+    const int row_base = T == 16 ? 0 : warp * 16;
+    const int t0 = rows[row_base + g], t1 = rows[row_base + g + 8];
+    const bool has0 = (unsigned)t0 < (unsigned)P.n, has1 = (unsigned)t1 < (unsigned)P.n;
+    const bool busy = row_base < nrows;       // a warp of a T = 64 tile may have no rows
+
+    // ---- this warp's share of h = A x: its chunks of 32 inner elements, eight consecutive ones a lane
+    float acc[RT][4] = {};
+    if (busy) {
+        const int chunks = (P.K + 31) / 32, share = c * SPLIT + (SPLIT > 1 ? warp : 0);
+        const int c0 = (int)((int64_t)chunks * share / (AD_CTAS * SPLIT)), c1 = (int)((int64_t)chunks * (share + 1) / (AD_CTAS * SPLIT));
+        const XT *x0 = x + (has0 ? (size_t)t0 * P.K : 0), *x1 = x + (has1 ? (size_t)t1 * P.K : 0);
+        const __nv_bfloat16 *a = P.a + ((size_t)id * P.r + g) * P.K;
+        const int tiles = P.r / 8;
+#pragma unroll 2
+        for (int ch = c0; ch < c1; ch++) {
+            const int k = ch * 32 + q * 8;
+            const bool in = k < P.K;
+            XFrag<XT> f0, f1;
+            f0.load(x0 + k, in && has0);
+            f1.load(x1 + k, in && has1);
+            uint4 av[RT];
+#pragma unroll
+            for (int i = 0; i < RT; i++)
+                if (i < tiles) av[i] = in ? __ldg(reinterpret_cast<const uint4 *>(a + (size_t)i * 8 * P.K + k)) : make_uint4(0, 0, 0, 0);
+            uint32_t w0[4][XFrag<XT>::PIECES], w1[4][XFrag<XT>::PIECES];
+            f0.words(w0);
+            f1.words(w1);
+#pragma unroll
+            for (int i = 0; i < RT; i++)
+                if (i < tiles) {
+#pragma unroll
+                    for (int p = 0; p < XFrag<XT>::PIECES; p++) {
+                        mma_bf16(acc[i], w0[0][p], w1[0][p], w0[1][p], w1[1][p], av[i].x, av[i].y);
+                        mma_bf16(acc[i], w0[2][p], w1[2][p], w0[3][p], w1[3][p], av[i].z, av[i].w);
+                    }
+                }
+        }
+    }
+    {
+        float *mine = part + warp * 16 * hs;
+#pragma unroll
+        for (int i = 0; i < RT; i++)
+            if (i * 8 < r16) {
+                *reinterpret_cast<float2 *>(mine + g * hs + i * 8 + 2 * q) = make_float2(acc[i][0], acc[i][1]);
+                *reinterpret_cast<float2 *>(mine + (g + 8) * hs + i * 8 + 2 * q) = make_float2(acc[i][2], acc[i][3]);
+            }
+    }
+
+    // ---- the shares of the cluster added, in CTA order, times the adapter's scale
+    const float scale = P.scales ? P.scales[id] : 1.f;
+    const int per_row = r16 / 4;
+    if (T == 16) {
+        __syncthreads();
+        for (int i = tid; i < 16 * per_row; i += AD_THREADS) {   // the warps of this CTA first
+            float4 *p = reinterpret_cast<float4 *>(part + i / per_row * hs) + i % per_row;
+            float4 s = *p;
+#pragma unroll
+            for (int w = 1; w < AD_WARPS; w++) {
+                const float4 v = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(p) + w * 16 * hs);
+                s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+            }
+            *p = s;
+        }
+        cluster.sync();
+        for (int i = tid; i < 16 * per_row; i += AD_THREADS) {   // every CTA adds all of it: one barrier less on the way
+            float *p = part + i / per_row * hs + i % per_row * 4;
+            float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int o = 0; o < AD_CTAS; o++) {
+                const float4 v = *reinterpret_cast<const float4 *>(cluster.map_shared_rank(p, o));
+                s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+            }
+            *reinterpret_cast<float4 *>(h + i / per_row * hs + i % per_row * 4) = make_float4(s.x * scale, s.y * scale, s.z * scale, s.w * scale);
+        }
+        __syncthreads();
+    } else {
+        cluster.sync();
+        for (int i = c * AD_THREADS + tid; i < T * per_row; i += AD_CTAS * AD_THREADS) {   // each CTA an eighth, given to all
+            const int at = i / per_row * hs + i % per_row * 4;
+            float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int o = 0; o < AD_CTAS; o++) {
+                const float4 v = *reinterpret_cast<const float4 *>(cluster.map_shared_rank(part + at, o));
+                s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+            }
+            s = make_float4(s.x * scale, s.y * scale, s.z * scale, s.w * scale);
+#pragma unroll
+            for (int o = 0; o < AD_CTAS; o++) *reinterpret_cast<float4 *>(cluster.map_shared_rank(h + at, o)) = s;
+        }
+        cluster.sync();
+    }
+
+    // ---- out = base + B h over this CTA's chunks of 32 columns.  Column (i / 2) * 8 + j * 2 + i % 2 of a chunk is column i
+    // of its j-th product, so that a lane ends with eight consecutive columns of its two rows.
+    if (busy) {
+        constexpr int KS = RT / 2 > 0 ? RT / 2 : 1;   // steps of sixteen ranks; a lane takes four consecutive ones of each
+        uint32_t hf[KS][HP][4];
+#pragma unroll
+        for (int s = 0; s < KS; s++)
+            if (s * 16 < r16) {
+                const float4 v0 = *reinterpret_cast<const float4 *>(h + (row_base + g) * hs + s * 16 + q * 4);
+                const float4 v1 = *reinterpret_cast<const float4 *>(h + (row_base + g + 8) * hs + s * 16 + q * 4);
+                uint32_t w[4][HP];
+                split_pair<HP>(v0.x, v0.y, w[0]);
+                split_pair<HP>(v1.x, v1.y, w[1]);
+                split_pair<HP>(v0.z, v0.w, w[2]);
+                split_pair<HP>(v1.z, v1.w, w[3]);
+#pragma unroll
+                for (int p = 0; p < HP; p++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) hf[s][p][i] = w[i][p];
+            }
+        const int chunks = (P.N + 31) / 32, share = c * SPLIT + (SPLIT > 1 ? warp : 0);
+        const int c0 = (int)((int64_t)chunks * share / (AD_CTAS * SPLIT)), c1 = (int)((int64_t)chunks * (share + 1) / (AD_CTAS * SPLIT));
+        const __nv_bfloat16 *b = P.b + (size_t)id * P.N * P.r;
+        for (int ch = c0; ch < c1; ch++) {
+            float o[4][4] = {};
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int col = ch * 32 + (g >> 1) * 8 + j * 2 + (g & 1);
+                const __nv_bfloat16 *br = b + (size_t)col * P.r;
+#pragma unroll
+                for (int s = 0; s < KS; s++)
+                    if (s * 16 < r16) {
+                        const int k = s * 16 + q * 4;
+                        const uint2 bv = col < P.N && k < P.r ? __ldg(reinterpret_cast<const uint2 *>(br + k)) : make_uint2(0, 0);
+#pragma unroll
+                        for (int p = 0; p < HP; p++) mma_bf16(o[j], hf[s][p][0], hf[s][p][1], hf[s][p][2], hf[s][p][3], bv.x, bv.y);
+                    }
+            }
+            const int col = ch * 32 + q * 8;
+            if (col >= P.N) continue;
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+                if (!(half ? has1 : has0)) continue;
+                const size_t at = (size_t)(half ? t1 : t0) * P.N + col;
+                float v[8];
+                load_units<8>(base + at, v);
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    v[2 * j] += o[j][2 * half];
+                    v[2 * j + 1] += o[j][2 * half + 1];
+                }
+                store_units<8>(out + at, v);
+            }
+        }
+    }
+    if (T == 16) cluster.sync();   // no CTA leaves while another reads its shares
+}
+
+template <typename XT, typename OT, int T, int RT>
+static cudaError_t launch_adapters_as(const AdapterArgs &P, const XT *x, const OT *base, OT *out, cudaStream_t s)
+{
+    const int hs = h_stride((P.r + 15) / 16 * 16);
+    const size_t smem = (size_t)(AD_WARPS * 16 + T) * hs * sizeof(float);
+    auto *kern = k_adapters<XT, OT, T, RT>;
+    if (smem > 40 * 1024) {
+        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return e;
+    }
+    const int slots = P.order ? P.n / T + P.L : P.n;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)slots * AD_CTAS);
+    cfg.blockDim = dim3(AD_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = AD_CTAS;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+    cfg.attrs = at;
+    cfg.numAttrs = 2;
     count_launch();
+    return cudaLaunchKernelEx(&cfg, kern, P, x, base, out);
+}
+
+cudaError_t launch_adapters(const void *base, int out_dtype, const void *x, int x_dtype, const AdapterArgs &P, void *out, cudaStream_t s)
+{
+    // tiles of 64 rows where an adapter has that many on average; else of 16
+    const bool wide = P.order && P.n / P.L >= 48;
     return with_type(x_dtype, [&](auto *xp) {
         return with_type(out_dtype, [&](auto *op) {
             using XT = std::remove_pointer_t<decltype(xp)>;
             using OT = std::remove_pointer_t<decltype(op)>;
-            return launch_pdl(k_adapters<XT, OT>, dim3(n), dim3(256), 0, s, (const OT *)base, (const XT *)x, K, N, r,
-                              (const __nv_bfloat16 *)a, (const __nv_bfloat16 *)b, scales, L, ids, (OT *)out);
+            const XT *xx = (const XT *)x;
+            const OT *bb = (const OT *)base;
+            OT *oo = (OT *)out;
+            if (wide)
+                return P.r <= 16   ? launch_adapters_as<XT, OT, 64, 2>(P, xx, bb, oo, s)
+                       : P.r <= 32 ? launch_adapters_as<XT, OT, 64, 4>(P, xx, bb, oo, s)
+                       : P.r <= 64 ? launch_adapters_as<XT, OT, 64, 8>(P, xx, bb, oo, s)
+                                   : launch_adapters_as<XT, OT, 64, 16>(P, xx, bb, oo, s);
+            return P.r <= 16   ? launch_adapters_as<XT, OT, 16, 2>(P, xx, bb, oo, s)
+                   : P.r <= 32 ? launch_adapters_as<XT, OT, 16, 4>(P, xx, bb, oo, s)
+                   : P.r <= 64 ? launch_adapters_as<XT, OT, 16, 8>(P, xx, bb, oo, s)
+                               : launch_adapters_as<XT, OT, 16, 16>(P, xx, bb, oo, s);
         });
     });
 }
@@ -85,6 +397,7 @@ extern "C" int pmoe_adapters_add(int device, const void *base, const void *x, in
         return fail(PMOE_ERR_INVALID_ARG, "base, x, a, b and out must be 16-byte aligned");
     DeviceGuard guard(device);
     if (!guard.ok) return fail(PMOE_ERR_NO_DEVICE, "cannot select device %d", device);
-    CU(launch_adapters(base, out_dtype, x, x_dtype, n, K, N, rank, a, b, scales, n_adapters, ids, out, (cudaStream_t)stream));
+    const AdapterArgs args{n, K, N, rank, n_adapters, (const __nv_bfloat16 *)a, (const __nv_bfloat16 *)b, scales, ids, order, offsets};
+    CU(launch_adapters(base, out_dtype, x, x_dtype, args, out, (cudaStream_t)stream));
     return PMOE_OK;
 }
