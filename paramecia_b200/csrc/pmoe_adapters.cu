@@ -32,7 +32,7 @@ constexpr int AD_THREADS = AD_WARPS * 32;
 // a lane's pairs are taken from consecutive elements (one wide load) instead of the two places the layout names.
 __device__ inline void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
 {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -53,26 +53,35 @@ template <int PIECES> __device__ inline void split_pair(float lo, float hi, uint
 template <typename XT> struct XFrag;
 template <> struct XFrag<__nv_bfloat16> {
     static constexpr int PIECES = 1;
-    uint4 v;
-    __device__ void load(const __nv_bfloat16 *p, bool there) { v = there ? *reinterpret_cast<const uint4 *>(p) : make_uint4(0, 0, 0, 0); }
-    __device__ void words(uint32_t (&w)[4][1]) const { w[0][0] = v.x; w[1][0] = v.y; w[2][0] = v.z; w[3][0] = v.w; }
+    static __device__ void words(const uint4 *p, uint32_t (&w)[4][1])
+    {
+        const uint4 v = p[0];
+        w[0][0] = v.x; w[1][0] = v.y; w[2][0] = v.z; w[3][0] = v.w;
+    }
 };
 template <> struct XFrag<float> {
     static constexpr int PIECES = 3;
-    float4 v0, v1;
-    __device__ void load(const float *p, bool there)
+    static __device__ void words(const uint4 *p, uint32_t (&w)[4][3])
     {
-        v0 = there ? reinterpret_cast<const float4 *>(p)[0] : make_float4(0.f, 0.f, 0.f, 0.f);
-        v1 = there ? reinterpret_cast<const float4 *>(p)[1] : make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-    __device__ void words(uint32_t (&w)[4][3]) const
-    {
+        const float4 v0 = reinterpret_cast<const float4 *>(p)[0], v1 = reinterpret_cast<const float4 *>(p)[32];
         split_pair<3>(v0.x, v0.y, w[0]);
         split_pair<3>(v0.z, v0.w, w[1]);
         split_pair<3>(v1.x, v1.y, w[2]);
         split_pair<3>(v1.z, v1.w, w[3]);
     }
 };
+
+// Asynchronous copies of 16 (8) bytes to shared memory; `there` = false writes zeros and reads nothing.
+__device__ inline void copy16(void *dst, const void *src, bool there)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ inline void copy8(void *dst, const void *src, bool there)
+{
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(there ? 8 : 0) : "memory");
+}
+__device__ inline void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT> __device__ inline void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
 
 struct AdapterArgs {
     int n, K, N, r, L;
@@ -95,10 +104,26 @@ template <typename OT> __device__ inline void copy_row(const OT *from, OT *to, i
 
 // T = 16: the four warps of a CTA share the tile's rows and split K and N again.  T = 64: sixteen rows a warp.
 // RT: groups of eight ranks that the accumulators are sized for.
+//
+// A CTA walks its share of K and then its share of N in stages of four chunks of 32: a stage holds what the matrix
+// instructions of those chunks need, as the lanes need it (sixteen bytes per lane, lanes side by side, so no
+// access meets a bank twice).  The copies are asynchronous and up to STAGES stages are on their way, the first ones of N
+// while the shares of h are still being added: without them the loads of one chunk at a time left the memory
+// idle (8192 rows of 2048 bf16, rank 64: 162 us, now see launch_adapters).
+template <typename XT, typename OT, int T, int RT> struct AdapterStage {
+    static constexpr int STAGES = T == 16 ? 4 : 2;
+    static constexpr int WEIGHTS = 4 * RT * 32 * 16;                     // A: 4 chunks x RT rank groups; B: 4 chunks x 4 products x RT / 4 rank steps
+    static constexpr int SIZE = sizeof(XT) > sizeof(OT) ? sizeof(XT) : sizeof(OT);
+    static constexpr int ROW_CHUNK = 2 * 32 * 8 * SIZE;                 // two rows of eight elements a lane
+    static constexpr int ROWS = (T == 16 ? 1 : 4) * 4 * ROW_CHUNK;
+    static constexpr int BYTES = WEIGHTS + ROWS;
+};
+
 template <typename XT, typename OT, int T, int RT>
 __global__ void __launch_bounds__(AD_THREADS) k_adapters(AdapterArgs P, const XT *__restrict__ x, const OT *base, OT *out)
 {
-    extern __shared__ __align__(16) float smem[];
+    using S = AdapterStage<XT, OT, T, RT>;
+    extern __shared__ __align__(16) uint8_t smem[];
     __shared__ int rows[T];
     __shared__ int tile_id, tile_rows;
     __shared__ int all_ids[T == 16 ? ADAPTER_ROWS_UNSORTED : 1];   // without an order T is 16
@@ -108,8 +133,8 @@ __global__ void __launch_bounds__(AD_THREADS) k_adapters(AdapterArgs P, const XT
     cg::cluster_group cluster = cg::this_cluster();
     const int c = (int)cluster.block_rank(), slot = blockIdx.x / AD_CTAS;
     const int r16 = (P.r + 15) / 16 * 16, hs = h_stride(r16);
-    float *part = smem;                       // [AD_WARPS * 16][hs] this CTA's share of h
-    float *h = smem + AD_WARPS * 16 * hs;     // [T][hs]
+    float *part = reinterpret_cast<float *>(smem + S::STAGES * S::BYTES);   // [AD_WARPS * 16][hs] this CTA's share of h
+    float *h = part + AD_WARPS * 16 * hs;                                   // [T][hs]
     pdl_wait();
     pdl_launch_dependents();
 
@@ -176,38 +201,116 @@ __global__ void __launch_bounds__(AD_THREADS) k_adapters(AdapterArgs P, const XT
     const bool has0 = (unsigned)t0 < (unsigned)P.n, has1 = (unsigned)t1 < (unsigned)P.n;
     const bool busy = row_base < nrows;       // a warp of a T = 64 tile may have no rows
 
-    // ---- this warp's share of h = A x: its chunks of 32 inner elements, eight consecutive ones a lane
-    float acc[RT][4] = {};
-    if (busy) {
-        const int chunks = (P.K + 31) / 32, share = c * SPLIT + (SPLIT > 1 ? warp : 0);
-        const int c0 = (int)((int64_t)chunks * share / (AD_CTAS * SPLIT)), c1 = (int)((int64_t)chunks * (share + 1) / (AD_CTAS * SPLIT));
-        const XT *x0 = x + (has0 ? (size_t)t0 * P.K : 0), *x1 = x + (has1 ? (size_t)t1 * P.K : 0);
-        const __nv_bfloat16 *a = P.a + ((size_t)id * P.r + g) * P.K;
-        const int tiles = P.r / 8;
-#pragma unroll 2
-        for (int ch = c0; ch < c1; ch++) {
-            const int k = ch * 32 + q * 8;
-            const bool in = k < P.K;
-            XFrag<XT> f0, f1;
-            f0.load(x0 + k, in && has0);
-            f1.load(x1 + k, in && has1);
-            uint4 av[RT];
+    // ---- the stages of this CTA
+    const int kc = (P.K + 31) / 32, nc = (P.N + 31) / 32;
+    const int k0 = (int)((int64_t)kc * c / AD_CTAS), k1 = (int)((int64_t)kc * (c + 1) / AD_CTAS);
+    const int n0 = (int)((int64_t)nc * c / AD_CTAS), n1 = (int)((int64_t)nc * (c + 1) / AD_CTAS);
+    const int kstages = (k1 - k0 + 3) / 4, stages = kstages + (n1 - n0 + 3) / 4;
+    const int tiles = P.r / 8;
+    const XT *x0 = x + (has0 ? (size_t)t0 * P.K : 0), *x1 = x + (has1 ? (size_t)t1 * P.K : 0);
+    const OT *b0 = base + (has0 ? (size_t)t0 * P.N : 0), *b1 = base + (has1 ? (size_t)t1 * P.N : 0);
+    const __nv_bfloat16 *aw = P.a + ((size_t)id * P.r + g) * P.K;
+    const __nv_bfloat16 *bw = P.b + (size_t)id * P.N * P.r;
+    // chunk i of a stage: its weights are fetched by warp i; its rows by their warp (T = 16: by warp i too)
+    auto weights_of = [&](int st, int i) { return reinterpret_cast<uint4 *>(smem + (st % S::STAGES) * S::BYTES + i * (S::WEIGHTS / 4)) + lane; };
+    auto rows_of = [&](int st, int i) {
+        return reinterpret_cast<uint4 *>(smem + (st % S::STAGES) * S::BYTES + S::WEIGHTS + (T == 16 ? i : warp * 4 + i) * S::ROW_CHUNK) + lane;
+    };
+    auto copy_rows = [&](uint4 *dst, const auto *p0, const auto *p1, bool in) {
+        constexpr int V = sizeof(*p0) / 2;   // 16-byte units of eight elements
 #pragma unroll
-            for (int i = 0; i < RT; i++)
-                if (i < tiles) av[i] = in ? __ldg(reinterpret_cast<const uint4 *>(a + (size_t)i * 8 * P.K + k)) : make_uint4(0, 0, 0, 0);
-            uint32_t w0[4][XFrag<XT>::PIECES], w1[4][XFrag<XT>::PIECES];
-            f0.words(w0);
-            f1.words(w1);
+        for (int v = 0; v < V; v++) {
+            copy16(dst + v * 32, reinterpret_cast<const uint4 *>(p0) + v, in && has0);
+            copy16(dst + (V + v) * 32, reinterpret_cast<const uint4 *>(p1) + v, in && has1);
+        }
+    };
+    auto fetch = [&](int st) {
+        if (st < kstages) {
+            const int ch0 = k0 + st * 4;
+            {
+                const int k = (ch0 + warp) * 32 + q * 8;
+                const bool in = ch0 + warp < k1 && k < P.K;
+                uint4 *dst = weights_of(st, warp);
+                for (int i = 0; i < tiles; i++) copy16(dst + i * 32, in ? aw + (size_t)i * 8 * P.K + k : P.a, in);
+            }
 #pragma unroll
-            for (int i = 0; i < RT; i++)
-                if (i < tiles) {
+            for (int i = 0; i < 4; i++) {
+                if (T == 16 && i != warp) continue;
+                const int k = (ch0 + i) * 32 + q * 8;
+                const bool in = ch0 + i < k1 && k < P.K;
+                copy_rows(rows_of(st, i), in ? x0 + k : x, in ? x1 + k : x, in);
+            }
+        } else if (st < stages) {
+            const int ch0 = n0 + (st - kstages) * 4;
+            uint4 *dst = weights_of(st, warp);
 #pragma unroll
-                    for (int p = 0; p < XFrag<XT>::PIECES; p++) {
-                        mma_bf16(acc[i], w0[0][p], w1[0][p], w0[1][p], w1[1][p], av[i].x, av[i].y);
-                        mma_bf16(acc[i], w0[2][p], w1[2][p], w0[3][p], w1[3][p], av[i].z, av[i].w);
+            for (int j = 0; j < 4; j++) {
+                const int col = (ch0 + warp) * 32 + (g >> 1) * 8 + j * 2 + (g & 1);
+                const bool in = ch0 + warp < n1 && col < P.N;
+                const __nv_bfloat16 *br = in ? bw + (size_t)col * P.r : P.b;
+                if constexpr (RT == 2) {
+                    const bool there = in && q * 4 < P.r;
+                    copy8(reinterpret_cast<uint2 *>(dst - lane) + j * 32 + lane, there ? br + q * 4 : P.b, there);
+                } else {
+#pragma unroll
+                    for (int s = 0; s < RT / 4; s++) {
+                        const bool there = in && s * 32 + q * 8 < P.r;
+                        copy16(dst + (j * (RT / 4) + s) * 32, there ? br + s * 32 + q * 8 : P.b, there);
                     }
                 }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if (T == 16 && i != warp) continue;
+                const int col = (ch0 + i) * 32 + q * 8;
+                const bool in = ch0 + i < n1 && col < P.N;
+                copy_rows(rows_of(st, i), in ? b0 + col : base, in ? b1 + col : base, in);
+            }
         }
+        copies_commit();
+    };
+    // T = 16: a warp reads what its own lanes fetched; T = 64: the weights come from all four warps
+    auto landed = [&] {
+        copies_wait<S::STAGES - 1>();
+        if (T == 16) __syncwarp();
+        else __syncthreads();
+    };
+    auto done_with = [&](int st) {
+        if (T == 16) __syncwarp();
+        else __syncthreads();
+        fetch(st + S::STAGES);
+    };
+#pragma unroll
+    for (int st = 0; st < S::STAGES; st++) fetch(st);
+
+    // ---- this warp's share of h = A x
+    float acc[RT][4] = {};
+    for (int st = 0; st < kstages; st++) {
+        landed();
+        const int here = min(4, k1 - k0 - st * 4);
+        if (busy)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if ((T == 16 && i != warp) || i >= here) continue;
+                constexpr int V = sizeof(XT) / 2, PC = XFrag<XT>::PIECES;
+                uint32_t w0[4][PC], w1[4][PC];
+                XFrag<XT>::words(rows_of(st, i), w0);
+                XFrag<XT>::words(rows_of(st, i) + V * 32, w1);
+                const uint4 *av = weights_of(st, i);
+#pragma unroll
+                for (int t = 0; t < RT; t += 2) {
+                    if (t >= tiles) break;
+                    const uint4 u = av[t * 32], v = t + 1 < tiles ? av[(t + 1) * 32] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                    for (int p = 0; p < PC; p++) {
+                        mma_bf16(acc[t], w0[0][p], w1[0][p], w0[1][p], w1[1][p], u.x, u.y);
+                        mma_bf16(acc[t + 1], w0[0][p], w1[0][p], w0[1][p], w1[1][p], v.x, v.y);
+                        mma_bf16(acc[t], w0[2][p], w1[2][p], w0[3][p], w1[3][p], u.z, u.w);
+                        mma_bf16(acc[t + 1], w0[2][p], w1[2][p], w0[3][p], w1[3][p], v.z, v.w);
+                    }
+                }
+            }
+        done_with(st);
     }
     {
         float *mine = part + warp * 16 * hs;
@@ -264,59 +367,93 @@ __global__ void __launch_bounds__(AD_THREADS) k_adapters(AdapterArgs P, const XT
     }
 
     // ---- out = base + B h over this CTA's chunks of 32 columns.  Column (i / 2) * 8 + j * 2 + i % 2 of a chunk is column i
-    // of its j-th product, so that a lane ends with eight consecutive columns of its two rows.
-    if (busy) {
-        constexpr int KS = RT / 2 > 0 ? RT / 2 : 1;   // steps of sixteen ranks; a lane takes four consecutive ones of each
-        uint32_t hf[KS][HP][4];
+    // of its j-th product, so that a lane ends with eight consecutive columns of its two rows.  Ranks: a lane takes four
+    // (RT = 2) or eight consecutive ones, which are one or two steps of the matrix instruction.
+    constexpr int KS = RT / 2;
+    uint32_t hf[KS][HP][4];
 #pragma unroll
-        for (int s = 0; s < KS; s++)
-            if (s * 16 < r16) {
-                const float4 v0 = *reinterpret_cast<const float4 *>(h + (row_base + g) * hs + s * 16 + q * 4);
-                const float4 v1 = *reinterpret_cast<const float4 *>(h + (row_base + g + 8) * hs + s * 16 + q * 4);
-                uint32_t w[4][HP];
-                split_pair<HP>(v0.x, v0.y, w[0]);
-                split_pair<HP>(v1.x, v1.y, w[1]);
-                split_pair<HP>(v0.z, v0.w, w[2]);
-                split_pair<HP>(v1.z, v1.w, w[3]);
-#pragma unroll
-                for (int p = 0; p < HP; p++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) hf[s][p][i] = w[i][p];
-            }
-        const int chunks = (P.N + 31) / 32, share = c * SPLIT + (SPLIT > 1 ? warp : 0);
-        const int c0 = (int)((int64_t)chunks * share / (AD_CTAS * SPLIT)), c1 = (int)((int64_t)chunks * (share + 1) / (AD_CTAS * SPLIT));
-        const __nv_bfloat16 *b = P.b + (size_t)id * P.N * P.r;
-        for (int ch = c0; ch < c1; ch++) {
-            float o[4][4] = {};
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int col = ch * 32 + (g >> 1) * 8 + j * 2 + (g & 1);
-                const __nv_bfloat16 *br = b + (size_t)col * P.r;
-#pragma unroll
-                for (int s = 0; s < KS; s++)
-                    if (s * 16 < r16) {
-                        const int k = s * 16 + q * 4;
-                        const uint2 bv = col < P.N && k < P.r ? __ldg(reinterpret_cast<const uint2 *>(br + k)) : make_uint2(0, 0);
-#pragma unroll
-                        for (int p = 0; p < HP; p++) mma_bf16(o[j], hf[s][p][0], hf[s][p][1], hf[s][p][2], hf[s][p][3], bv.x, bv.y);
-                    }
-            }
-            const int col = ch * 32 + q * 8;
-            if (col >= P.N) continue;
-#pragma unroll
-            for (int half = 0; half < 2; half++) {
-                if (!(half ? has1 : has0)) continue;
-                const size_t at = (size_t)(half ? t1 : t0) * P.N + col;
-                float v[8];
-                load_units<8>(base + at, v);
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    v[2 * j] += o[j][2 * half];
-                    v[2 * j + 1] += o[j][2 * half + 1];
-                }
-                store_units<8>(out + at, v);
-            }
+    for (int s = 0; s < KS; s++) {
+        const int k = RT == 2 ? q * 4 : s / 2 * 32 + q * 8 + s % 2 * 4;
+        float4 v0 = make_float4(0.f, 0.f, 0.f, 0.f), v1 = v0;
+        if (k < r16) {
+            v0 = *reinterpret_cast<const float4 *>(h + (row_base + g) * hs + k);
+            v1 = *reinterpret_cast<const float4 *>(h + (row_base + g + 8) * hs + k);
         }
+        uint32_t w[4][HP];
+        split_pair<HP>(v0.x, v0.y, w[0]);
+        split_pair<HP>(v1.x, v1.y, w[1]);
+        split_pair<HP>(v0.z, v0.w, w[2]);
+        split_pair<HP>(v1.z, v1.w, w[3]);
+#pragma unroll
+        for (int p = 0; p < HP; p++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) hf[s][p][i] = w[i][p];
+    }
+    for (int st = kstages; st < stages; st++) {
+        landed();
+        const int ch0 = n0 + (st - kstages) * 4;
+        if (busy)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if ((T == 16 && i != warp) || ch0 + i >= n1) continue;
+                float o[4][4] = {};
+                const uint4 *bv = weights_of(st, i);
+                // the four products of a step are independent: in turn, so that none waits for its own sum
+                if constexpr (RT == 2) {
+#pragma unroll
+                    for (int p = 0; p < HP; p++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            const uint2 v = (reinterpret_cast<const uint2 *>(bv - lane) + j * 32)[lane];
+                            mma_bf16(o[j], hf[0][p][0], hf[0][p][1], hf[0][p][2], hf[0][p][3], v.x, v.y);
+                        }
+                } else {
+#pragma unroll
+                    for (int s = 0; s < RT / 4; s++) {
+                        if (s * 32 >= P.r) break;
+                        uint4 v[4];
+#pragma unroll
+                        for (int j = 0; j < 4; j++) v[j] = bv[(j * (RT / 4) + s) * 32];
+#pragma unroll
+                        for (int p = 0; p < HP; p++) {
+#pragma unroll
+                            for (int j = 0; j < 4; j++)
+                                mma_bf16(o[j], hf[2 * s][p][0], hf[2 * s][p][1], hf[2 * s][p][2], hf[2 * s][p][3], v[j].x, v[j].y);
+#pragma unroll
+                            for (int j = 0; j < 4; j++)
+                                mma_bf16(o[j], hf[2 * s + 1][p][0], hf[2 * s + 1][p][1], hf[2 * s + 1][p][2], hf[2 * s + 1][p][3], v[j].z, v[j].w);
+                        }
+                    }
+                }
+                const int col = (ch0 + i) * 32 + q * 8;
+                if (col < P.N) {
+                    constexpr int V = sizeof(OT) / 2;
+#pragma unroll
+                    for (int half = 0; half < 2; half++) {
+                        if (!(half ? has1 : has0)) continue;
+                        float v[8];
+                        const uint4 *bp = rows_of(st, i) + half * V * 32;
+                        if constexpr (V == 1) {
+                            load_units<8>(reinterpret_cast<const OT *>(bp), v);
+                        } else {
+                            float u[4];
+                            load_units<4>(reinterpret_cast<const OT *>(bp), u);
+#pragma unroll
+                            for (int e = 0; e < 4; e++) v[e] = u[e];
+                            load_units<4>(reinterpret_cast<const OT *>(bp + 32), u);
+#pragma unroll
+                            for (int e = 0; e < 4; e++) v[4 + e] = u[e];
+                        }
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            v[2 * j] += o[j][2 * half];
+                            v[2 * j + 1] += o[j][2 * half + 1];
+                        }
+                        store_units<8>(out + (size_t)(half ? t1 : t0) * P.N + col, v);
+                    }
+                }
+            }
+        done_with(st);
     }
     if (T == 16) cluster.sync();   // no CTA leaves while another reads its shares
 }
@@ -325,9 +462,9 @@ template <typename XT, typename OT, int T, int RT>
 static cudaError_t launch_adapters_as(const AdapterArgs &P, const XT *x, const OT *base, OT *out, cudaStream_t s)
 {
     const int hs = h_stride((P.r + 15) / 16 * 16);
-    const size_t smem = (size_t)(AD_WARPS * 16 + T) * hs * sizeof(float);
+    const size_t smem = (size_t)(AD_WARPS * 16 + T) * hs * sizeof(float) + AdapterStage<XT, OT, T, RT>::STAGES * AdapterStage<XT, OT, T, RT>::BYTES;
     auto *kern = k_adapters<XT, OT, T, RT>;
-    if (smem > 40 * 1024) {
+    if (smem > 40 * 1024) {   // with the static arrays, more than a launch may have without asking
         cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return e;
     }

@@ -8,48 +8,92 @@
 //   order[place_p] = p  (-1 from offsets[E] on).
 // The order is stable, so all of it is a function of idx alone (the block's grouping leaves the order inside an expert
 // to its atomics).
+#include <cooperative_groups.h>
+
 #include "pmoe_internal.h"
 #include "pmoe_vec.cuh"
 
 namespace pmoe {
 
+namespace cg = cooperative_groups;
+
 // ---------------------------------------------------------------- sort
-// A counting sort in one CTA.  Warp w owns the w-th run of consecutive pairs, takes it 32 pairs at a time, and ranks the
-// pairs of a step among those of the same expert with __match_any_sync: ranks inside the step, steps, warps are three
-// levels of the same order, so the result is stable without atomics.
+// A counting sort in one launch, by one CTA or by a cluster of eight.  Every warp owns a run of consecutive pairs, takes it
+// 32 pairs at a time, and ranks the pairs of such a step among those of the same expert with __match_any_sync: ranks
+// inside the step, steps, warps and CTAs are four levels of the same order, so the result is stable without atomics.
 //   1. cnt[w][e]  pairs of expert e in warp w's run
-//   2. exclusive scan over (e, w): cnt[w][e] becomes the place of that warp's first pair of e
+//   2. the CTAs' totals are exchanged through distributed shared memory; exclusive scan over (e, CTA, w): cnt[w][e]
+//      becomes the place of that warp's first pair of e
 //   3. the runs once more: place = cnt[w][e] + rank inside the step
+// The pairs are few bytes (4 to read, 8 to write): what counts is latency, so a lane loads its keys of eight steps at once
+// and keeps them from 1. to 3. where the run is no longer than that.
 constexpr int SORT_MAX_E = 4096;
 constexpr int SORT_THREADS = 1024;
+constexpr int SORT_CTAS = 8;
+constexpr int SORT_BATCH = 8;
+constexpr int SORT_ONE_CTA = 4096;   // pairs up to which one CTA sorts
 
+struct SortKeys {
+    uint32_t v[SORT_BATCH];
+    // the keys of the steps from pair p on; pairs behind p1 get one that no expert has
+    __device__ void load(const uint32_t *idx, int64_t p, int64_t p1, uint32_t base, int lane)
+    {
+#pragma unroll
+        for (int i = 0; i < SORT_BATCH; i++) v[i] = p + i * 32 + lane < p1 ? __ldg(idx + p + i * 32 + lane) - base : 0xffffffffu;
+    }
+};
+
+template <int CTAS>
 __global__ void __launch_bounds__(SORT_THREADS) k_sort_pairs(const uint32_t *__restrict__ idx, int P, uint32_t base, int E, int warps,
                                                              int run, int *__restrict__ order, int *__restrict__ place,
                                                              int *__restrict__ offsets)
 {
-    extern __shared__ int cnt[];   // [warps][E]
+    extern __shared__ int cnt[];   // [warps][E], then this CTA's totals [E]
     __shared__ int warp_tot[32];
+    int *mine = cnt + warps * E;
     const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int rank = CTAS > 1 ? (int)cluster.block_rank() : 0;
     for (int i = tid; i < warps * E; i += SORT_THREADS) cnt[i] = 0;
     pdl_wait();
     pdl_launch_dependents();
-    __syncthreads();
 
-    const int p0 = min((int64_t)P, (int64_t)w * run), p1 = w < warps ? min((int64_t)P, (int64_t)p0 + run) : p0;
-    for (int p = p0; p < p1; p += 32) {
-        const uint32_t key = p + lane < p1 ? idx[p + lane] - base : 0xffffffffu;
-        const unsigned same = __match_any_sync(0xffffffffu, key);
-        if (key < (uint32_t)E && lane == __ffs(same) - 1) cnt[w * E + key] += __popc(same);
-        __syncwarp();
+    const int64_t p0 = min((int64_t)P, (int64_t)(rank * warps + w) * run), p1 = w < warps ? min((int64_t)P, p0 + run) : p0;
+    const bool once = run <= SORT_BATCH * 32;
+    SortKeys keys;
+    keys.load(idx, p0, p1, base, lane);
+    __syncthreads();
+    for (int64_t p = p0; p < p1; p += SORT_BATCH * 32) {
+        if (p != p0) keys.load(idx, p, p1, base, lane);
+#pragma unroll
+        for (int i = 0; i < SORT_BATCH; i++) {
+            if (p + i * 32 >= p1) break;
+            const uint32_t key = keys.v[i];
+            const unsigned same = __match_any_sync(0xffffffffu, key);
+            if (key < (uint32_t)E && lane == __ffs(same) - 1) cnt[w * E + key] += __popc(same);
+            __syncwarp();
+        }
     }
     __syncthreads();
 
     // thread t scans experts [t*q, t*q + q)
-    const int q = (E + SORT_THREADS - 1) / SORT_THREADS;
-    int mine = 0;
-    for (int e = tid * q; e < min(E, tid * q + q); e++)
-        for (int v = 0; v < warps; v++) mine += cnt[v * E + e];
-    int incl = mine;
+    const int q = (E + SORT_THREADS - 1) / SORT_THREADS, e0 = min(E, tid * q), e1 = min(E, e0 + q);
+    int sum = 0;      // of all CTAs, over this thread's experts
+    for (int e = e0; e < e1; e++) {
+        int t = 0;
+#pragma unroll 8
+        for (int v = 0; v < warps; v++) t += cnt[v * E + e];
+        mine[e] = t;
+        sum += t;
+    }
+    if (CTAS > 1) {
+        cluster.sync();
+        sum = 0;
+        for (int e = e0; e < e1; e++)
+#pragma unroll
+            for (int o = 0; o < CTAS; o++) sum += *cluster.map_shared_rank(mine + e, o);
+    }
+    int incl = sum;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
         const int y = __shfl_up_sync(0xffffffffu, incl, off);
@@ -57,52 +101,92 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_pairs(const uint32_t *__r
     }
     if (lane == 31) warp_tot[w] = incl;
     __syncthreads();
-    int before = incl - mine, total = 0;
-    for (int v = 0; v < 32; v++) {
-        if (v < w) before += warp_tot[v];
-        total += warp_tot[v];
+    int total = warp_tot[lane], upto = total;      // every warp scans the 32 warp totals for itself
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, upto, off);
+        if (lane >= off) upto += y;
     }
-    for (int e = tid * q; e < min(E, tid * q + q); e++) {
-        offsets[e] = before;
+    total = __shfl_sync(0xffffffffu, upto, 31);
+    const int earlier = __shfl_sync(0xffffffffu, upto, max(0, w - 1));
+    int before = incl - sum + (w > 0 ? earlier : 0);
+    for (int e = e0; e < e1; e++) {
+        if (rank == 0) offsets[e] = before;
+        int at = before;
+        if (CTAS > 1) {
+#pragma unroll
+            for (int o = 0; o < CTAS; o++) {
+                const int t = *cluster.map_shared_rank(mine + e, o);
+                if (o < rank) at += t;
+                before += t;
+            }
+        } else {
+            before += mine[e];
+        }
+#pragma unroll 8
         for (int v = 0; v < warps; v++) {
-            const int c = cnt[v * E + e];
-            cnt[v * E + e] = before;
-            before += c;
+            const int t = cnt[v * E + e];
+            cnt[v * E + e] = at;
+            at += t;
         }
     }
-    if (tid == 0) offsets[E] = total;
+    if (rank == 0 && tid == 0) offsets[E] = total;
     __syncthreads();
 
-    for (int p = p0; p < p1; p += 32) {
-        const uint32_t key = p + lane < p1 ? idx[p + lane] - base : 0xffffffffu;
-        const unsigned same = __match_any_sync(0xffffffffu, key);
-        const int rank = __popc(same & ((1u << lane) - 1));
-        int at = -1;
-        if (key < (uint32_t)E) at = cnt[w * E + key] + rank;
-        __syncwarp();
-        if (key < (uint32_t)E && rank == 0) cnt[w * E + key] += __popc(same);
-        __syncwarp();
-        if (p + lane < p1) {
-            if (place) place[p + lane] = at;
-            if (order && at >= 0) order[at] = p + lane;
+    for (int64_t p = p0; p < p1; p += SORT_BATCH * 32) {
+        if (!once) keys.load(idx, p, p1, base, lane);
+#pragma unroll
+        for (int i = 0; i < SORT_BATCH; i++) {
+            const int64_t pair = p + i * 32 + lane;
+            if (p + i * 32 >= p1) break;
+            const uint32_t key = keys.v[i];
+            const unsigned same = __match_any_sync(0xffffffffu, key);
+            const int nth = __popc(same & ((1u << lane) - 1));
+            int at = -1;
+            if (key < (uint32_t)E) at = cnt[w * E + key] + nth;
+            __syncwarp();
+            if (key < (uint32_t)E && nth == 0) cnt[w * E + key] = at + __popc(same);
+            __syncwarp();
+            if (pair < p1) {
+                if (place) place[pair] = at;
+                if (order && at >= 0) order[at] = (int)pair;
+            }
         }
     }
     if (order)
-        for (int p = total + tid; p < P; p += SORT_THREADS) order[p] = -1;
+        for (int64_t p = total + rank * SORT_THREADS + tid; p < P; p += CTAS * SORT_THREADS) order[p] = -1;
+    if (CTAS > 1) cluster.sync();   // no CTA leaves while another reads its totals
 }
 
 cudaError_t launch_sort_pairs(const uint32_t *idx, int P, int base, int E, int *order, int *place, int *offsets, cudaStream_t s)
 {
-    // the counts of all warps stay below 128 KB; no more warps than there are steps of 32 pairs
-    int warps = E <= 1024 ? 32 : 8;
-    warps = min(warps, max(1, (P + 31) / 32));
-    const int run = (((P + warps - 1) / warps) + 31) / 32 * 32;
-    const size_t smem = (size_t)warps * E * sizeof(int);
-    cudaError_t e = cudaFuncSetAttribute(k_sort_pairs, cudaFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024);
-    if (e != cudaSuccess) return e;
-    e = launch_pdl(k_sort_pairs, dim3(1), dim3(SORT_THREADS), smem, s, idx, P, (uint32_t)base, E, warps, run, order, place, offsets);
+    // the counts of all warps stay below 144 KB; no more warps than there are steps of 32 pairs
+    const int most = E <= 1024 ? 32 : 8;
+    const bool one = P <= SORT_ONE_CTA;
+    const int ctas = one ? 1 : SORT_CTAS;
+    const int warps = min(most, max(1, (P + 31) / 32 / ctas));
+    const int run = (int)((((int64_t)P + ctas * warps - 1) / (ctas * warps) + 31) / 32 * 32);
+    const size_t smem = (size_t)(warps + 1) * E * sizeof(int);
+    auto *kern = one ? k_sort_pairs<1> : k_sort_pairs<SORT_CTAS>;
+    if (smem > 40 * 1024) {
+        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return e;
+    }
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(ctas);
+    cfg.blockDim = dim3(SORT_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = ctas;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = one ? 1 : 2;
     count_launch();
-    return e;
+    return cudaLaunchKernelEx(&cfg, kern, idx, P, (uint32_t)base, E, warps, run, order, place, offsets);
 }
 
 // ---------------------------------------------------------------- dispatch
