@@ -22,9 +22,7 @@ namespace cg = cooperative_groups;
 
 constexpr int ADAPTER_MAX_RANK = 128;
 constexpr int ADAPTER_ROWS_UNSORTED = 1024;   // rows that are grouped by id without pmoe_sort_pairs
-constexpr int AD_CTAS = 8;                    // CTAs of a cluster
-constexpr int AD_WARPS = 4;
-constexpr int AD_THREADS = AD_WARPS * 32;
+constexpr int AD_MAX_CTAS = 8;                // CTAs of a cluster
 
 // c += a b, 16 x 8 x 16, bf16 operands, f32 sums.  Lane l, g = l / 4, q = l % 4: a0 / a1 = rows g / g + 8 at the inner pair
 // (2q, 2q + 1), a2 / a3 the same at inner pair 2q + 8; b0, b1 the same inner pairs of column g; c0, c1 = row g, columns
@@ -71,14 +69,14 @@ template <> struct XFrag<float> {
     }
 };
 
-// Asynchronous copies of 16 (8) bytes to shared memory; `there` = false writes zeros and reads nothing.
-__device__ inline void copy16(void *dst, const void *src, bool there)
+// Asynchronous copies of 16 (8) bytes to shared memory; size 0 writes zeros and reads nothing.
+__device__ inline void copy16(void *dst, const void *src, int size)
 {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(there ? 16 : 0) : "memory");
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(size) : "memory");
 }
-__device__ inline void copy8(void *dst, const void *src, bool there)
+__device__ inline void copy8(void *dst, const void *src, int size)
 {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(there ? 8 : 0) : "memory");
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(size) : "memory");
 }
 __device__ inline void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int LEFT> __device__ inline void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
@@ -93,48 +91,66 @@ struct AdapterArgs {
 // floats between two rows of h in shared memory: sixteen more where rows would start in the same bank
 __host__ __device__ inline int h_stride(int r16) { return r16 % 32 ? r16 : r16 + 16; }
 
-template <typename OT> __device__ inline void copy_row(const OT *from, OT *to, int units, int first)
+// out = base in the listed rows, eight elements at a time; four loads are on their way before the first is stored
+template <typename OT>
+__device__ inline void copy_rows_of(const OT *base, OT *out, int N, const int *list, int count, int first, int step)
 {
-    for (int u = first; u < units; u += AD_CTAS * AD_THREADS) {
-        float v[8];
-        load_units<8>(from + u * 8, v);
-        store_units<8>(to + u * 8, v);
+    const int units = N / 8, total = count * units;
+    for (int u = first; u < total; u += 4 * step) {
+        float v[4][8];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int k = u + i * step;
+            if (k < total) load_units<8>(base + (size_t)list[k / units] * N + k % units * 8, v[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int k = u + i * step;
+            if (k < total) store_units<8>(out + (size_t)list[k / units] * N + k % units * 8, v[i]);
+        }
     }
 }
 
-// T = 16: the four warps of a CTA share the tile's rows and split K and N again.  T = 64: sixteen rows a warp.
-// RT: groups of eight ranks that the accumulators are sized for.
-//
 // A CTA walks its share of K and then its share of N in stages of four chunks of 32: a stage holds what the matrix
 // instructions of those chunks need, as the lanes need it (sixteen bytes per lane, lanes side by side, so no
-// access meets a bank twice).  The copies are asynchronous and up to STAGES stages are on their way, the first ones of N
-// while the shares of h are still being added: without them the loads of one chunk at a time left the memory
-// idle (8192 rows of 2048 bf16, rank 64: 162 us, now see launch_adapters).
+// access meets a bank twice).  The copies are asynchronous and STAGES stages are on their way, the first ones of N
+// while the shares of h are still being added.
+//
+// A warp has sixteen rows and KH of them share a stage's four chunks: what a warp does per chunk is a chain of dependent
+// steps (read, multiply, add the base, write), so it takes about sixteen warps an SM to fill each other's gaps.  With one warp
+// per sixteen rows (four to eight an SM) 8192 rows of 2048 bf16, rank 64, took 82 us.
+// RT: groups of eight ranks that the accumulators are sized for.
 template <typename XT, typename OT, int T, int RT> struct AdapterStage {
+    static constexpr int SIZE = sizeof(XT) > sizeof(OT) ? sizeof(XT) : sizeof(OT);
+    static constexpr int KH = T == 16 ? 4 : SIZE == 4 && RT < 16 ? 4 : 2;
+    static constexpr int WARPS = T / 16 * KH, THREADS = WARPS * 32, CPW = 4 / KH;
+    static constexpr int MIN_CTAS = T == 16 ? 4 : WARPS == 8 && RT < 16 ? 2 : 1;
     static constexpr int STAGES = T == 16 ? 4 : 2;
     static constexpr int WEIGHTS = 4 * RT * 32 * 16;                     // A: 4 chunks x RT rank groups; B: 4 chunks x 4 products x RT / 4 rank steps
-    static constexpr int SIZE = sizeof(XT) > sizeof(OT) ? sizeof(XT) : sizeof(OT);
     static constexpr int ROW_CHUNK = 2 * 32 * 8 * SIZE;                 // two rows of eight elements a lane
-    static constexpr int ROWS = (T == 16 ? 1 : 4) * 4 * ROW_CHUNK;
+    static constexpr int ROWS = T / 16 * 4 * ROW_CHUNK;
     static constexpr int BYTES = WEIGHTS + ROWS;
+    static size_t smem(int r16) { return STAGES * BYTES + (size_t)(KH / 2 + 1) * T * h_stride(r16) * sizeof(float); }
 };
 
 template <typename XT, typename OT, int T, int RT>
-__global__ void __launch_bounds__(AD_THREADS) k_adapters(AdapterArgs P, const XT *__restrict__ x, const OT *base, OT *out)
+__global__ void __launch_bounds__(AdapterStage<XT, OT, T, RT>::THREADS, AdapterStage<XT, OT, T, RT>::MIN_CTAS) k_adapters(AdapterArgs P, const XT *__restrict__ x, const OT *base, OT *out)
 {
     using S = AdapterStage<XT, OT, T, RT>;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ int rows[T];
-    __shared__ int tile_id, tile_rows;
+    __shared__ int tile_id, tile_rows, tile_first, bare_list[T];
+    __shared__ unsigned bare_mask[2];
     __shared__ int all_ids[T == 16 ? ADAPTER_ROWS_UNSORTED : 1];   // without an order T is 16
-    constexpr int SPLIT = T == 16 ? AD_WARPS : 1;   // warps that share rows
+    constexpr int THREADS = S::THREADS, CPW = S::CPW;
     constexpr int HP = std::is_same<OT, float>::value ? 3 : 2;   // pieces of h: an f32 result keeps all of it, a bf16 result 16 bits
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3;
+    const int rg = warp % (T / 16), kh = warp / (T / 16);   // this warp's sixteen rows and its chunks of a stage
     cg::cluster_group cluster = cg::this_cluster();
-    const int c = (int)cluster.block_rank(), slot = blockIdx.x / AD_CTAS;
+    const int ctas = (int)cluster.num_blocks(), c = (int)cluster.block_rank(), slot = blockIdx.x / ctas;
     const int r16 = (P.r + 15) / 16 * 16, hs = h_stride(r16);
-    float *part = reinterpret_cast<float *>(smem + S::STAGES * S::BYTES);   // [AD_WARPS * 16][hs] this CTA's share of h
-    float *h = part + AD_WARPS * 16 * hs;                                   // [T][hs]
+    float *part = reinterpret_cast<float *>(smem + S::STAGES * S::BYTES);   // [KH / 2][T][hs] this CTA's share of h
+    float *h = part + S::KH / 2 * T * hs;                                   // [T][hs]
     pdl_wait();
     pdl_launch_dependents();
 
@@ -142,39 +158,44 @@ __global__ void __launch_bounds__(AD_THREADS) k_adapters(AdapterArgs P, const XT
     if (P.order) {
         // Tile slots of adapter e begin at offsets[e] / T + e: with one slot more than whole multiples of T inside its
         // range that is never fewer than it has tiles, and needs no scan over the adapters.
-        if (tid < T) rows[tid] = -1;
-        if (tid == 0) {
-            int lo = 0, hi = P.L;     // last e with start(e) <= slot
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) / 2;
-                if (P.offsets[mid] / T + mid <= slot) lo = mid;
-                else hi = mid;
+        if (tid == 0) tile_rows = 0;
+        __syncthreads();
+        for (int e = tid; e < P.L; e += THREADS) {
+            const int from = P.offsets[e], to = min(P.offsets[e + 1], P.n), nth = slot - (from / T + e);
+            if (from >= 0 && nth >= 0 && nth < (to - from + T - 1) / T) {   // one adapter at most
+                tile_id = e;
+                tile_first = from + nth * T;
+                tile_rows = min(T, to - from - nth * T);
             }
-            const int first = P.offsets[lo] + (slot - (P.offsets[lo] / T + lo)) * T;
-            tile_id = lo;
-            tile_rows = first;        // for the moment: where the tile begins
         }
-        __syncthreads();
-        const int first = tile_rows, end = min(P.n, P.offsets[tile_id + 1]);
-        __syncthreads();
-        if (tid < T && first >= 0 && first + tid < end) rows[tid] = P.order[first + tid];
-        if (tid == 0) tile_rows = first >= 0 ? max(0, min(T, end - first)) : 0;
-        __syncthreads();
         // rows without an adapter are nowhere in the order: the slots pass over the batch once more for them
         const int t = slot * T + tid;
-        if (__syncthreads_or(tid < T && t < P.n && (unsigned)P.ids[min(t, P.n - 1)] >= (unsigned)P.L) && out != base)
-            for (int t = slot * T; t < min(P.n, slot * T + T); t++)
-                if ((unsigned)P.ids[t] >= (unsigned)P.L) copy_row(base + (size_t)t * P.N, out + (size_t)t * P.N, P.N / 8, c * AD_THREADS + tid);
+        const bool bare = tid < T && t < P.n && (unsigned)P.ids[min(t, P.n - 1)] >= (unsigned)P.L;
+        const unsigned bare_here = __ballot_sync(0xffffffffu, bare);
+        if (lane == 0 && warp < (T + 31) / 32) bare_mask[warp] = bare_here;
+        const int any = __syncthreads_count(bare);
+        if (tid < T) rows[tid] = tid < tile_rows ? P.order[tile_first + tid] : -1;
+        if (any && out != base) {
+            // listed in ascending order: the CTAs of the cluster share the list out among them
+            if (bare) bare_list[__popc(bare_here & ((1u << lane) - 1)) + (warp > 0 ? __popc(bare_mask[0]) : 0)] = t;
+            __syncthreads();
+            copy_rows_of(base, out, P.N, bare_list, any, c * THREADS + tid, ctas * THREADS);
+        }
+        __syncthreads();
         if (tile_rows == 0) return;
     } else if constexpr (T == 16) {
         // slot t leads a tile when the number of earlier rows with its id is a multiple of T
         const int id = P.ids[slot];
         if ((unsigned)id >= (unsigned)P.L) {
-            if (out != base) copy_row(base + (size_t)slot * P.N, out + (size_t)slot * P.N, P.N / 8, c * AD_THREADS + tid);
+            if (out != base) {
+                if (tid == 0) bare_list[0] = slot;
+                __syncthreads();
+                copy_rows_of(base, out, P.N, bare_list, 1, c * THREADS + tid, ctas * THREADS);
+            }
             return;
         }
         if (tid < T) rows[tid] = -1;
-        for (int t = tid; t < P.n; t += AD_THREADS) all_ids[t] = P.ids[t];
+        for (int t = tid; t < P.n; t += THREADS) all_ids[t] = P.ids[t];
         __syncthreads();
         if (warp == 0) {
             int before = 0, found = 0;
@@ -196,80 +217,105 @@ __global__ void __launch_bounds__(AD_THREADS) k_adapters(AdapterArgs P, const XT
         if (tile_rows == 0) return;
     }
     const int id = tile_id, nrows = tile_rows;
-    const int row_base = T == 16 ? 0 : warp * 16;
+    const int row_base = rg * 16;
     const int t0 = rows[row_base + g], t1 = rows[row_base + g + 8];
     const bool has0 = (unsigned)t0 < (unsigned)P.n, has1 = (unsigned)t1 < (unsigned)P.n;
     const bool busy = row_base < nrows;       // a warp of a T = 64 tile may have no rows
 
     // ---- the stages of this CTA
     const int kc = (P.K + 31) / 32, nc = (P.N + 31) / 32;
-    const int k0 = (int)((int64_t)kc * c / AD_CTAS), k1 = (int)((int64_t)kc * (c + 1) / AD_CTAS);
-    const int n0 = (int)((int64_t)nc * c / AD_CTAS), n1 = (int)((int64_t)nc * (c + 1) / AD_CTAS);
+    const int k0 = (int)((int64_t)kc * c / ctas), k1 = (int)((int64_t)kc * (c + 1) / ctas);
+    const int n0 = (int)((int64_t)nc * c / ctas), n1 = (int)((int64_t)nc * (c + 1) / ctas);
     const int kstages = (k1 - k0 + 3) / 4, stages = kstages + (n1 - n0 + 3) / 4;
     const int tiles = P.r / 8;
     const XT *x0 = x + (has0 ? (size_t)t0 * P.K : 0), *x1 = x + (has1 ? (size_t)t1 * P.K : 0);
     const OT *b0 = base + (has0 ? (size_t)t0 * P.N : 0), *b1 = base + (has1 ? (size_t)t1 * P.N : 0);
     const __nv_bfloat16 *aw = P.a + ((size_t)id * P.r + g) * P.K;
     const __nv_bfloat16 *bw = P.b + (size_t)id * P.N * P.r;
-    // chunk i of a stage: its weights are fetched by warp i; its rows by their warp (T = 16: by warp i too)
+    // chunk i of a stage: its weights are fetched by the warps i, i + 4, ...; its rows by the warp that uses them
     auto weights_of = [&](int st, int i) { return reinterpret_cast<uint4 *>(smem + (st % S::STAGES) * S::BYTES + i * (S::WEIGHTS / 4)) + lane; };
     auto rows_of = [&](int st, int i) {
-        return reinterpret_cast<uint4 *>(smem + (st % S::STAGES) * S::BYTES + S::WEIGHTS + (T == 16 ? i : warp * 4 + i) * S::ROW_CHUNK) + lane;
+        return reinterpret_cast<uint4 *>(smem + (st % S::STAGES) * S::BYTES + S::WEIGHTS + (rg * 4 + i) * S::ROW_CHUNK) + lane;
     };
-    auto copy_rows = [&](uint4 *dst, const auto *p0, const auto *p1, bool in) {
+    const int size0 = has0 ? 16 : 0, size1 = has1 ? 16 : 0;
+    auto copy_rows = [&](uint4 *dst, const auto *p0, const auto *p1, int n0, int n1) {
         constexpr int V = sizeof(*p0) / 2;   // 16-byte units of eight elements
 #pragma unroll
         for (int v = 0; v < V; v++) {
-            copy16(dst + v * 32, reinterpret_cast<const uint4 *>(p0) + v, in && has0);
-            copy16(dst + (V + v) * 32, reinterpret_cast<const uint4 *>(p1) + v, in && has1);
+            copy16(dst + v * 32, reinterpret_cast<const uint4 *>(p0) + v, n0);
+            copy16(dst + (V + v) * 32, reinterpret_cast<const uint4 *>(p1) + v, n1);
+        }
+    };
+    // WHOLE: every chunk of the stage lies inside the share and inside K or N
+    auto fetch_k = [&](int st, auto whole) {
+        constexpr bool WHOLE = decltype(whole)::value;
+        const int ch0 = k0 + st * 4;
+        {
+            const int wc = warp % 4, k = (ch0 + wc) * 32 + q * 8;
+            const bool in = WHOLE || (ch0 + wc < k1 && k < P.K);
+            uint4 *dst = weights_of(st, wc) + warp / 4 * 32;
+            const __nv_bfloat16 *src = in ? aw + (size_t)(warp / 4) * 8 * P.K + k : P.a;
+            const size_t step = in ? (size_t)(S::WARPS / 4) * 8 * P.K : 0;
+#pragma unroll
+            for (int i = 0; i < RT; i += S::WARPS / 4) {
+                if (i + warp / 4 >= tiles) break;
+                copy16(dst + i * 32, src, in ? 16 : 0);
+                src += step;
+            }
+        }
+        const XT *p0 = x0 + ch0 * 32 + q * 8, *p1 = x1 + ch0 * 32 + q * 8;
+#pragma unroll
+        for (int u = 0; u < CPW; u++) {
+            const int i = kh * CPW + u;
+            const bool in = WHOLE || (ch0 + i < k1 && (ch0 + i) * 32 + q * 8 < P.K);
+            copy_rows(rows_of(st, i), in ? p0 + i * 32 : x, in ? p1 + i * 32 : x, in ? size0 : 0, in ? size1 : 0);
+        }
+    };
+    auto fetch_n = [&](int st, auto whole) {
+        constexpr bool WHOLE = decltype(whole)::value;
+        const int ch0 = n0 + (st - kstages) * 4;
+        constexpr int JW = 16 / S::WARPS;    // of the four products of a chunk, those that this warp fetches the weights of
+        const int wc = warp % 4, j0 = warp / 4 * JW;
+        uint4 *dst = weights_of(st, wc);
+        const int col0 = (ch0 + wc) * 32 + (g >> 1) * 8 + j0 * 2 + (g & 1);
+        const __nv_bfloat16 *br = bw + (size_t)col0 * P.r + q * (RT == 2 ? 4 : 8);
+#pragma unroll
+        for (int jj = 0; jj < JW; jj++) {
+            const int j = j0 + jj;
+            const bool in = WHOLE || (ch0 + wc < n1 && col0 + jj * 2 < P.N);
+            if constexpr (RT == 2) {
+                const bool there = in && q * 4 < P.r;
+                copy8(reinterpret_cast<uint2 *>(dst - lane) + j * 32 + lane, there ? br : P.b, there ? 8 : 0);
+            } else {
+#pragma unroll
+                for (int s = 0; s < RT / 4; s++) {
+                    const bool there = in && s * 32 + q * 8 < P.r;
+                    copy16(dst + (j * (RT / 4) + s) * 32, there ? br + s * 32 : P.b, there ? 16 : 0);
+                }
+            }
+            br += 2 * P.r;
+        }
+        const OT *p0 = b0 + ch0 * 32 + q * 8, *p1 = b1 + ch0 * 32 + q * 8;
+#pragma unroll
+        for (int u = 0; u < CPW; u++) {
+            const int i = kh * CPW + u;
+            const bool in = WHOLE || (ch0 + i < n1 && (ch0 + i) * 32 + q * 8 < P.N);
+            copy_rows(rows_of(st, i), in ? p0 + i * 32 : base, in ? p1 + i * 32 : base, in ? size0 : 0, in ? size1 : 0);
         }
     };
     auto fetch = [&](int st) {
         if (st < kstages) {
-            const int ch0 = k0 + st * 4;
-            {
-                const int k = (ch0 + warp) * 32 + q * 8;
-                const bool in = ch0 + warp < k1 && k < P.K;
-                uint4 *dst = weights_of(st, warp);
-                for (int i = 0; i < tiles; i++) copy16(dst + i * 32, in ? aw + (size_t)i * 8 * P.K + k : P.a, in);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                if (T == 16 && i != warp) continue;
-                const int k = (ch0 + i) * 32 + q * 8;
-                const bool in = ch0 + i < k1 && k < P.K;
-                copy_rows(rows_of(st, i), in ? x0 + k : x, in ? x1 + k : x, in);
-            }
+            const int last = k0 + st * 4 + 4;
+            if (last <= k1 && last * 32 <= P.K) fetch_k(st, std::true_type{});
+            else fetch_k(st, std::false_type{});
         } else if (st < stages) {
-            const int ch0 = n0 + (st - kstages) * 4;
-            uint4 *dst = weights_of(st, warp);
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int col = (ch0 + warp) * 32 + (g >> 1) * 8 + j * 2 + (g & 1);
-                const bool in = ch0 + warp < n1 && col < P.N;
-                const __nv_bfloat16 *br = in ? bw + (size_t)col * P.r : P.b;
-                if constexpr (RT == 2) {
-                    const bool there = in && q * 4 < P.r;
-                    copy8(reinterpret_cast<uint2 *>(dst - lane) + j * 32 + lane, there ? br + q * 4 : P.b, there);
-                } else {
-#pragma unroll
-                    for (int s = 0; s < RT / 4; s++) {
-                        const bool there = in && s * 32 + q * 8 < P.r;
-                        copy16(dst + (j * (RT / 4) + s) * 32, there ? br + s * 32 + q * 8 : P.b, there);
-                    }
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                if (T == 16 && i != warp) continue;
-                const int col = (ch0 + i) * 32 + q * 8;
-                const bool in = ch0 + i < n1 && col < P.N;
-                copy_rows(rows_of(st, i), in ? b0 + col : base, in ? b1 + col : base, in);
-            }
+            const int last = n0 + (st - kstages) * 4 + 4;
+            if (last <= n1 && last * 32 <= P.N) fetch_n(st, std::true_type{});
+            else fetch_n(st, std::false_type{});
         }
         copies_commit();
     };
-    // T = 16: a warp reads what its own lanes fetched; T = 64: the weights come from all four warps
+    // T = 16: a warp reads what its own lanes fetched; T = 64: the weights come from all warps
     auto landed = [&] {
         copies_wait<S::STAGES - 1>();
         if (T == 16) __syncwarp();
@@ -290,8 +336,9 @@ __global__ void __launch_bounds__(AD_THREADS) k_adapters(AdapterArgs P, const XT
         const int here = min(4, k1 - k0 - st * 4);
         if (busy)
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                if ((T == 16 && i != warp) || i >= here) continue;
+            for (int u = 0; u < CPW; u++) {
+                const int i = kh * CPW + u;
+                if (i >= here) continue;
                 constexpr int V = sizeof(XT) / 2, PC = XFrag<XT>::PIECES;
                 uint32_t w0[4][PC], w1[4][PC];
                 XFrag<XT>::words(rows_of(st, i), w0);
@@ -312,37 +359,51 @@ __global__ void __launch_bounds__(AD_THREADS) k_adapters(AdapterArgs P, const XT
             }
         done_with(st);
     }
-    {
-        float *mine = part + warp * 16 * hs;
+    // the warps of the same rows: the upper half hands its sums to the lower half, lane to lane, until one has them all
+    auto at_part = [&](int buffer, int i, int half) {
+        return reinterpret_cast<float2 *>(part + (buffer * T + row_base + g + half * 8) * hs + i * 8 + 2 * q);
+    };
+    auto put = [&](int buffer) {
 #pragma unroll
         for (int i = 0; i < RT; i++)
             if (i * 8 < r16) {
-                *reinterpret_cast<float2 *>(mine + g * hs + i * 8 + 2 * q) = make_float2(acc[i][0], acc[i][1]);
-                *reinterpret_cast<float2 *>(mine + (g + 8) * hs + i * 8 + 2 * q) = make_float2(acc[i][2], acc[i][3]);
+                *at_part(buffer, i, 0) = make_float2(acc[i][0], acc[i][1]);
+                *at_part(buffer, i, 1) = make_float2(acc[i][2], acc[i][3]);
             }
+    };
+    auto add = [&](int buffer) {
+#pragma unroll
+        for (int i = 0; i < RT; i++)
+            if (i * 8 < r16) {
+                const float2 u = *at_part(buffer, i, 0), v = *at_part(buffer, i, 1);
+                acc[i][0] += u.x; acc[i][1] += u.y; acc[i][2] += v.x; acc[i][3] += v.y;
+            }
+    };
+    if constexpr (S::KH == 4) {
+        if (kh >= 2) put(kh - 2);
+        __syncthreads();
+        if (kh < 2) add(kh);
+        if (kh == 1) put(1);
+        __syncthreads();
+        if (kh == 0) add(1);
+    } else {
+        if (kh == 1) put(0);
+        __syncthreads();
+        if (kh == 0) add(0);
     }
+    if (kh == 0) put(0);
 
     // ---- the shares of the cluster added, in CTA order, times the adapter's scale
     const float scale = P.scales ? P.scales[id] : 1.f;
     const int per_row = r16 / 4;
     if (T == 16) {
-        __syncthreads();
-        for (int i = tid; i < 16 * per_row; i += AD_THREADS) {   // the warps of this CTA first
-            float4 *p = reinterpret_cast<float4 *>(part + i / per_row * hs) + i % per_row;
-            float4 s = *p;
-#pragma unroll
-            for (int w = 1; w < AD_WARPS; w++) {
-                const float4 v = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(p) + w * 16 * hs);
-                s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
-            }
-            *p = s;
-        }
         cluster.sync();
-        for (int i = tid; i < 16 * per_row; i += AD_THREADS) {   // every CTA adds all of it: one barrier less on the way
+        for (int i = tid; i < 16 * per_row; i += THREADS) {   // every CTA adds all of it: one barrier less on the way
             float *p = part + i / per_row * hs + i % per_row * 4;
             float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (int o = 0; o < AD_CTAS; o++) {
+            for (int o = 0; o < AD_MAX_CTAS; o++) {
+                if (o >= ctas) break;
                 const float4 v = *reinterpret_cast<const float4 *>(cluster.map_shared_rank(p, o));
                 s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
             }
@@ -351,17 +412,19 @@ __global__ void __launch_bounds__(AD_THREADS) k_adapters(AdapterArgs P, const XT
         __syncthreads();
     } else {
         cluster.sync();
-        for (int i = c * AD_THREADS + tid; i < T * per_row; i += AD_CTAS * AD_THREADS) {   // each CTA an eighth, given to all
+        for (int i = c * THREADS + tid; i < T * per_row; i += ctas * THREADS) {   // each CTA its part, given to all
             const int at = i / per_row * hs + i % per_row * 4;
             float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (int o = 0; o < AD_CTAS; o++) {
+            for (int o = 0; o < AD_MAX_CTAS; o++) {
+                if (o >= ctas) break;
                 const float4 v = *reinterpret_cast<const float4 *>(cluster.map_shared_rank(part + at, o));
                 s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
             }
             s = make_float4(s.x * scale, s.y * scale, s.z * scale, s.w * scale);
 #pragma unroll
-            for (int o = 0; o < AD_CTAS; o++) *reinterpret_cast<float4 *>(cluster.map_shared_rank(h + at, o)) = s;
+            for (int o = 0; o < AD_MAX_CTAS; o++)
+                if (o < ctas) *reinterpret_cast<float4 *>(cluster.map_shared_rank(h + at, o)) = s;
         }
         cluster.sync();
     }
@@ -394,8 +457,9 @@ __global__ void __launch_bounds__(AD_THREADS) k_adapters(AdapterArgs P, const XT
         const int ch0 = n0 + (st - kstages) * 4;
         if (busy)
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                if ((T == 16 && i != warp) || ch0 + i >= n1) continue;
+            for (int u = 0; u < CPW; u++) {
+                const int i = kh * CPW + u;
+                if (ch0 + i >= n1) continue;
                 float o[4][4] = {};
                 const uint4 *bv = weights_of(st, i);
                 // the four products of a step are independent: in turn, so that none waits for its own sum
@@ -461,22 +525,33 @@ __global__ void __launch_bounds__(AD_THREADS) k_adapters(AdapterArgs P, const XT
 template <typename XT, typename OT, int T, int RT>
 static cudaError_t launch_adapters_as(const AdapterArgs &P, const XT *x, const OT *base, OT *out, cudaStream_t s)
 {
-    const int hs = h_stride((P.r + 15) / 16 * 16);
-    const size_t smem = (size_t)(AD_WARPS * 16 + T) * hs * sizeof(float) + AdapterStage<XT, OT, T, RT>::STAGES * AdapterStage<XT, OT, T, RT>::BYTES;
+    using S = AdapterStage<XT, OT, T, RT>;
+    const size_t smem = S::smem((P.r + 15) / 16 * 16);
     auto *kern = k_adapters<XT, OT, T, RT>;
     if (smem > 40 * 1024) {   // with the static arrays, more than a launch may have without asking
         cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return e;
     }
+    // The cluster's size: more CTAs share a tile's K and N, each with the same work around it (finding the tile, the
+    // exchange of h: about as long as eight stages).  Taken is the size with the shortest sum over the waves
+    // that the grid makes: eight where the rows are few, one or two where the tiles alone fill the card.
     const int slots = P.order ? P.n / T + P.L : P.n;
+    const int64_t room = 148 * (int64_t)max(1, min(2 * S::MIN_CTAS, (int)(227 * 1024 / (smem + 6144))));
+    int ctas = AD_MAX_CTAS;
+    double best = 1e30;
+    for (int c = AD_MAX_CTAS; c >= 1; c /= 2) {
+        const int64_t tiles = P.order ? (P.n + T - 1) / T + min(P.L, (P.n + T - 1) / T) / 2 : min(P.n, P.L);
+        const double cost = (double)((tiles * c + room - 1) / room) * (8.0 + (P.K + P.N) / 128.0 / c);
+        if (cost < best) { best = cost; ctas = c; }
+    }
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)slots * AD_CTAS);
-    cfg.blockDim = dim3(AD_THREADS);
+    cfg.gridDim = dim3((unsigned)slots * ctas);
+    cfg.blockDim = dim3(S::THREADS);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = AD_CTAS;
+    at[0].val.clusterDim.x = ctas;
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[1].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
