@@ -47,7 +47,8 @@ template <int PIECES> __device__ inline void split_pair(float lo, float hi, uint
     }
 }
 
-// eight consecutive inner elements of a row as matrix operands: four pairs, in one piece for bf16 and in three for f32
+// Eight consecutive inner elements of a row as matrix operands, four pairs: in one piece for bf16, in three for f32 (whose
+// second sixteen bytes lie one unit of the warp further).
 template <typename XT> struct XFrag;
 template <> struct XFrag<__nv_bfloat16> {
     static constexpr int PIECES = 1;
@@ -69,17 +70,30 @@ template <> struct XFrag<float> {
     }
 };
 
-// Asynchronous copies of 16 (8) bytes to shared memory; size 0 writes zeros and reads nothing.
-__device__ inline void copy16(void *dst, const void *src, int size)
+// Asynchronous copies of 16 (8) bytes to shared memory at byte offsets that the instruction carries; size 0 writes zeros
+// and reads nothing.
+template <int D, int S> __device__ inline void copy16(uint32_t dst, const void *src, int size)
 {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(size) : "memory");
+    asm volatile("cp.async.cg.shared.global [%0 + %3], [%1 + %4], 16, %2;" ::"r"(dst), "l"(src), "r"(size), "n"(D), "n"(S) : "memory");
 }
-__device__ inline void copy8(void *dst, const void *src, int size)
+__device__ inline void copy8(uint32_t dst, const void *src, int size)
 {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(size) : "memory");
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(size) : "memory");
 }
 __device__ inline void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int LEFT> __device__ inline void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
+
+// f(Const<0>), ..., f(Const<N - 1>): offsets that depend on the index stay constants
+template <int I> struct Const {
+    __host__ __device__ constexpr operator int() const { return I; }
+};
+template <int N, typename F> __device__ __forceinline__ void each(F &&f)
+{
+    if constexpr (N > 0) {
+        each<N - 1>(f);
+        f(Const<N - 1>{});
+    }
+}
 
 struct AdapterArgs {
     int n, K, N, r, L;
@@ -88,26 +102,45 @@ struct AdapterArgs {
     const int *ids, *order, *offsets;
 };
 
-// floats between two rows of h in shared memory: sixteen more where rows would start in the same bank
-__host__ __device__ inline int h_stride(int r16) { return r16 % 32 ? r16 : r16 + 16; }
-
-// out = base in the listed rows, eight elements at a time; four loads are on their way before the first is stored
-template <typename OT>
-__device__ inline void copy_rows_of(const OT *base, OT *out, int N, const int *list, int count, int first, int step)
+// out = base in the rows that have no adapter.  They are in no tile, and may be any number of them side by side, so every CTA
+// of the grid takes the rows blockIdx.x, blockIdx.x + gridDim.x, ... when its tile is done (copied by the tiles' slots,
+// 64 rows each before their tile, they doubled the time of 8192 rows with a thirteenth of them bare).
+// The lanes of a warp look at 32 of them at a time; the first ids are loaded when the kernel begins.
+__device__ inline int id_of_share(const AdapterArgs &P, int first)
 {
-    const int units = N / 8, total = count * units;
-    for (int u = first; u < total; u += 4 * step) {
-        float v[4][8];
+    const int64_t t = blockIdx.x + (int64_t)gridDim.x * (first + (threadIdx.x & 31));
+    return t < P.n ? P.ids[t] : 0;
+}
+
+template <int THREADS, typename OT> __device__ inline void copy_bare_rows(const AdapterArgs &P, int my_id, const OT *base, OT *out)
+{
+    if (out == base) return;
+    const int units = P.N / 8;
+    for (int first = 0;;) {
+        unsigned bare = __ballot_sync(0xffffffffu, (unsigned)my_id >= (unsigned)P.L);
+        int u = threadIdx.x;   // this thread's next unit, of the lowest row left in `bare`
+        while (true) {
+            float v[2][8];
+            size_t at[2];
+            int got = 0;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int k = u + i * step;
-            if (k < total) load_units<8>(base + (size_t)list[k / units] * N + k % units * 8, v[i]);
-        }
+            for (int k = 0; k < 2; k++) {
+                while (bare && u >= units) { u -= units; bare &= bare - 1; }
+                if (!bare) break;
+                at[k] = (size_t)(blockIdx.x + (int64_t)gridDim.x * (first + __ffs(bare) - 1)) * P.N + u * 8;
+                load_units<8>(base + at[k], v[k]);
+                u += THREADS;
+                got++;
+            }
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int k = u + i * step;
-            if (k < total) store_units<8>(out + (size_t)list[k / units] * N + k % units * 8, v[i]);
+            for (int k = 0; k < 2; k++)
+                if (k < got) store_units<8>(out + at[k], v[k]);
+            if (got < 2) break;
         }
+        first += 32;
+        if (blockIdx.x + (int64_t)gridDim.x * first >= P.n) return;
+        __syncwarp();
+        my_id = id_of_share(P, first);
     }
 }
 
@@ -125,12 +158,16 @@ template <typename XT, typename OT, int T, int RT> struct AdapterStage {
     static constexpr int KH = T == 16 ? 4 : SIZE == 4 && RT < 16 ? 4 : 2;
     static constexpr int WARPS = T / 16 * KH, THREADS = WARPS * 32, CPW = 4 / KH;
     static constexpr int MIN_CTAS = T == 16 ? 4 : WARPS == 8 && RT < 16 ? 2 : 1;
-    static constexpr int STAGES = T == 16 ? 4 : 2;
     static constexpr int WEIGHTS = 4 * RT * 32 * 16;                     // A: 4 chunks x RT rank groups; B: 4 chunks x 4 products x RT / 4 rank steps
     static constexpr int ROW_CHUNK = 2 * 32 * 8 * SIZE;                 // two rows of eight elements a lane
     static constexpr int ROWS = T / 16 * 4 * ROW_CHUNK;
     static constexpr int BYTES = WEIGHTS + ROWS;
-    static size_t smem(int r16) { return STAGES * BYTES + (size_t)(KH / 2 + 1) * T * h_stride(r16) * sizeof(float); }
+    static constexpr int HS = RT == 2 ? 16 : RT * 8 + 16;               // floats between two rows of h: no two rows of a quarter warp start in one bank
+    static constexpr int H_BYTES = (KH / 2 + 1) * T * HS * 4;
+    static constexpr int ROOM = (T == 16 ? (RT == 16 ? 222 : 110) : MIN_CTAS == 2 ? 112 : 222) * 1024 - H_BYTES;   // of the 227 KB of an SM, a CTA's part
+    static constexpr int STAGES = ROOM / BYTES < 2 ? 2 : ROOM / BYTES > 4 ? 4 : ROOM / BYTES;
+    static constexpr int SMEM = STAGES * BYTES + H_BYTES;
+    static_assert(SMEM <= 222 * 1024, "fits an SM beside the static arrays");
 };
 
 template <typename XT, typename OT, int T, int RT>
@@ -139,8 +176,7 @@ __global__ void __launch_bounds__(AdapterStage<XT, OT, T, RT>::THREADS, AdapterS
     using S = AdapterStage<XT, OT, T, RT>;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ int rows[T];
-    __shared__ int tile_id, tile_rows, tile_first, bare_list[T];
-    __shared__ unsigned bare_mask[2];
+    __shared__ int tile_id, tile_rows, tile_first;
     __shared__ int all_ids[T == 16 ? ADAPTER_ROWS_UNSORTED : 1];   // without an order T is 16
     constexpr int THREADS = S::THREADS, CPW = S::CPW;
     constexpr int HP = std::is_same<OT, float>::value ? 3 : 2;   // pieces of h: an f32 result keeps all of it, a bf16 result 16 bits
@@ -148,11 +184,13 @@ __global__ void __launch_bounds__(AdapterStage<XT, OT, T, RT>::THREADS, AdapterS
     const int rg = warp % (T / 16), kh = warp / (T / 16);   // this warp's sixteen rows and its chunks of a stage
     cg::cluster_group cluster = cg::this_cluster();
     const int ctas = (int)cluster.num_blocks(), c = (int)cluster.block_rank(), slot = blockIdx.x / ctas;
-    const int r16 = (P.r + 15) / 16 * 16, hs = h_stride(r16);
-    float *part = reinterpret_cast<float *>(smem + S::STAGES * S::BYTES);   // [KH / 2][T][hs] this CTA's share of h
-    float *h = part + S::KH / 2 * T * hs;                                   // [T][hs]
+    constexpr int HS = S::HS;
+    float *part = reinterpret_cast<float *>(smem + S::STAGES * S::BYTES);   // [KH / 2][T][HS] this CTA's share of h
+    float *h = part + S::KH / 2 * T * HS;                                   // [T][HS]
     pdl_wait();
     pdl_launch_dependents();
+
+    const int share_id = id_of_share(P, 0);
 
     // ---- the tile: its adapter and rows.  Every CTA of the cluster finds the same.
     if (P.order) {
@@ -168,32 +206,12 @@ __global__ void __launch_bounds__(AdapterStage<XT, OT, T, RT>::THREADS, AdapterS
                 tile_rows = min(T, to - from - nth * T);
             }
         }
-        // rows without an adapter are nowhere in the order: the slots pass over the batch once more for them
-        const int t = slot * T + tid;
-        const bool bare = tid < T && t < P.n && (unsigned)P.ids[min(t, P.n - 1)] >= (unsigned)P.L;
-        const unsigned bare_here = __ballot_sync(0xffffffffu, bare);
-        if (lane == 0 && warp < (T + 31) / 32) bare_mask[warp] = bare_here;
-        const int any = __syncthreads_count(bare);
-        if (tid < T) rows[tid] = tid < tile_rows ? P.order[tile_first + tid] : -1;
-        if (any && out != base) {
-            // listed in ascending order: the CTAs of the cluster share the list out among them
-            if (bare) bare_list[__popc(bare_here & ((1u << lane) - 1)) + (warp > 0 ? __popc(bare_mask[0]) : 0)] = t;
-            __syncthreads();
-            copy_rows_of(base, out, P.N, bare_list, any, c * THREADS + tid, ctas * THREADS);
-        }
         __syncthreads();
-        if (tile_rows == 0) return;
+        if (tid < T) rows[tid] = tid < tile_rows ? P.order[tile_first + tid] : -1;
+        __syncthreads();
     } else if constexpr (T == 16) {
         // slot t leads a tile when the number of earlier rows with its id is a multiple of T
         const int id = P.ids[slot];
-        if ((unsigned)id >= (unsigned)P.L) {
-            if (out != base) {
-                if (tid == 0) bare_list[0] = slot;
-                __syncthreads();
-                copy_rows_of(base, out, P.N, bare_list, 1, c * THREADS + tid, ctas * THREADS);
-            }
-            return;
-        }
         if (tid < T) rows[tid] = -1;
         for (int t = tid; t < P.n; t += THREADS) all_ids[t] = P.ids[t];
         __syncthreads();
@@ -210,11 +228,14 @@ __global__ void __launch_bounds__(AdapterStage<XT, OT, T, RT>::THREADS, AdapterS
             }
             if (lane == 0) {
                 tile_id = id;
-                tile_rows = before % T ? 0 : min(found, T);
+                tile_rows = (unsigned)id >= (unsigned)P.L || before % T ? 0 : min(found, T);
             }
         }
         __syncthreads();
-        if (tile_rows == 0) return;
+    }
+    if (tile_rows == 0) {
+        copy_bare_rows<THREADS>(P, share_id, base, out);
+        return;
     }
     const int id = tile_id, nrows = tile_rows;
     const int row_base = rg * 16;
@@ -227,94 +248,101 @@ __global__ void __launch_bounds__(AdapterStage<XT, OT, T, RT>::THREADS, AdapterS
     const int k0 = (int)((int64_t)kc * c / ctas), k1 = (int)((int64_t)kc * (c + 1) / ctas);
     const int n0 = (int)((int64_t)nc * c / ctas), n1 = (int)((int64_t)nc * (c + 1) / ctas);
     const int kstages = (k1 - k0 + 3) / 4, stages = kstages + (n1 - n0 + 3) / 4;
-    const int tiles = P.r / 8;
-    const XT *x0 = x + (has0 ? (size_t)t0 * P.K : 0), *x1 = x + (has1 ? (size_t)t1 * P.K : 0);
-    const OT *b0 = base + (has0 ? (size_t)t0 * P.N : 0), *b1 = base + (has1 ? (size_t)t1 * P.N : 0);
-    const __nv_bfloat16 *aw = P.a + ((size_t)id * P.r + g) * P.K;
-    const __nv_bfloat16 *bw = P.b + (size_t)id * P.N * P.r;
-    // chunk i of a stage: its weights are fetched by the warps i, i + 4, ...; its rows by the warp that uses them
-    auto weights_of = [&](int st, int i) { return reinterpret_cast<uint4 *>(smem + (st % S::STAGES) * S::BYTES + i * (S::WEIGHTS / 4)) + lane; };
-    auto rows_of = [&](int st, int i) {
-        return reinterpret_cast<uint4 *>(smem + (st % S::STAGES) * S::BYTES + S::WEIGHTS + (rg * 4 + i) * S::ROW_CHUNK) + lane;
-    };
     const int size0 = has0 ? 16 : 0, size1 = has1 ? 16 : 0;
-    auto copy_rows = [&](uint4 *dst, const auto *p0, const auto *p1, int n0, int n1) {
-        constexpr int V = sizeof(*p0) / 2;   // 16-byte units of eight elements
-#pragma unroll
-        for (int v = 0; v < V; v++) {
-            copy16(dst + v * 32, reinterpret_cast<const uint4 *>(p0) + v, n0);
-            copy16(dst + (V + v) * 32, reinterpret_cast<const uint4 *>(p1) + v, n1);
-        }
+    // Where this lane fetches from, a stage further after each: its two rows in x, later in base; weights of chunk wc,
+    // rank groups wj, wj + WARPS / 4, ... of A, later products wj * JW and following of B.
+    constexpr int JW = 16 / S::WARPS, WSTEP = S::WARPS / 4;
+    const int wc = warp % 4, wj = warp / 4, chunk0 = kh * CPW;
+    const XT *x0 = x + (has0 ? (size_t)t0 * P.K : 0) + (k0 + chunk0) * 32 + q * (16 / (int)sizeof(XT)), *x1 = x + (has1 ? (size_t)t1 * P.K : 0) + (k0 + chunk0) * 32 + q * (16 / (int)sizeof(XT));
+    const OT *b0 = base + (has0 ? (size_t)t0 * P.N : 0) + (n0 + chunk0) * 32 + q * (16 / (int)sizeof(OT)), *b1 = base + (has1 ? (size_t)t1 * P.N : 0) + (n0 + chunk0) * 32 + q * (16 / (int)sizeof(OT));
+    const __nv_bfloat16 *aw = P.a + ((size_t)id * P.r + wj * 8 + g) * P.K + (k0 + wc) * 32 + q * 8;
+    const size_t aw_step = (size_t)WSTEP * 8 * P.K;
+    const __nv_bfloat16 *bw = P.b + ((size_t)id * P.N + (n0 + wc) * 32 + (g >> 1) * (16 / (int)sizeof(OT)) + (g & 1)) * P.r + q * (RT == 2 ? 4 : 8);
+    const uint32_t to = smem_u32(smem), to_rows = to + S::WEIGHTS + (rg * 4 + chunk0) * S::ROW_CHUNK,
+                   to_weights = to + wc * (S::WEIGHTS / 4);
+    const bool all_ranks = P.r == RT * 8;
+
+    // Rows: a copy instruction takes 64 consecutive bytes of each of eight rows.  For f32 that is half a chunk (v = 0, 1);
+    // x's pieces go to the lane that multiplies them (eight consecutive elements, like the weights' sixteen bytes), base's
+    // stay with the lane that adds them: its columns are four and four, sixteen apart.
+    const uint32_t x_lane = sizeof(XT) == 2 ? lane * 16 : (q & 1) * 512 + (g * 4 + (q >> 1)) * 16;
+    constexpr int X_STEP = 32, B_STEP = 512;   // from v = 0 to v = 1
+    auto fetch_rows = [&](uint32_t dst, auto step, auto *p0, auto *p1, int ch, int ch_end, int limit) {
+        using VT = std::remove_cv_t<std::remove_pointer_t<decltype(p0)>>;
+        constexpr int V = sizeof(VT) / 2, STEP = decltype(step)();   // V units of sixteen bytes in eight elements
+        each<CPW>([&](auto u) {
+            each<V>([&](auto v) {
+                const bool in = ch + u < ch_end && (ch + u) * 32 + v * 16 + q * (16 / (int)sizeof(VT)) < limit;
+                constexpr int D = u * S::ROW_CHUNK + v * STEP, O = u * 32 * (int)sizeof(VT) + v * 64;
+                // a copy of nothing still gets an address inside a tensor
+                copy16<D, 0>(dst, in ? (const char *)p0 + O : (const char *)P.a, in ? size0 : 0);
+                copy16<D + V * 512, 0>(dst, in ? (const char *)p1 + O : (const char *)P.a, in ? size1 : 0);
+            });
+        });
     };
-    // WHOLE: every chunk of the stage lies inside the share and inside K or N
-    auto fetch_k = [&](int st, auto whole) {
-        constexpr bool WHOLE = decltype(whole)::value;
-        const int ch0 = k0 + st * 4;
-        {
-            const int wc = warp % 4, k = (ch0 + wc) * 32 + q * 8;
-            const bool in = WHOLE || (ch0 + wc < k1 && k < P.K);
-            uint4 *dst = weights_of(st, wc) + warp / 4 * 32;
-            const __nv_bfloat16 *src = in ? aw + (size_t)(warp / 4) * 8 * P.K + k : P.a;
-            const size_t step = in ? (size_t)(S::WARPS / 4) * 8 * P.K : 0;
-#pragma unroll
-            for (int i = 0; i < RT; i += S::WARPS / 4) {
-                if (i + warp / 4 >= tiles) break;
-                copy16(dst + i * 32, src, in ? 16 : 0);
-                src += step;
-            }
-        }
-        const XT *p0 = x0 + ch0 * 32 + q * 8, *p1 = x1 + ch0 * 32 + q * 8;
-#pragma unroll
-        for (int u = 0; u < CPW; u++) {
-            const int i = kh * CPW + u;
-            const bool in = WHOLE || (ch0 + i < k1 && (ch0 + i) * 32 + q * 8 < P.K);
-            copy_rows(rows_of(st, i), in ? p0 + i * 32 : x, in ? p1 + i * 32 : x, in ? size0 : 0, in ? size1 : 0);
-        }
+    auto fetch_rows_whole = [&](uint32_t dst, auto step, auto *p0, auto *p1) {
+        using VT = std::remove_cv_t<std::remove_pointer_t<decltype(p0)>>;
+        constexpr int V = sizeof(VT) / 2, STEP = decltype(step)();
+        each<CPW>([&](auto u) {
+            each<V>([&](auto v) {
+                constexpr int D = u * S::ROW_CHUNK + v * STEP, O = u * 32 * (int)sizeof(VT) + v * 64;
+                copy16<D, O>(dst, p0, size0);
+                copy16<D + V * 512, O>(dst, p1, size1);
+            });
+        });
     };
-    auto fetch_n = [&](int st, auto whole) {
-        constexpr bool WHOLE = decltype(whole)::value;
-        const int ch0 = n0 + (st - kstages) * 4;
-        constexpr int JW = 16 / S::WARPS;    // of the four products of a chunk, those that this warp fetches the weights of
-        const int wc = warp % 4, j0 = warp / 4 * JW;
-        uint4 *dst = weights_of(st, wc);
-        const int col0 = (ch0 + wc) * 32 + (g >> 1) * 8 + j0 * 2 + (g & 1);
-        const __nv_bfloat16 *br = bw + (size_t)col0 * P.r + q * (RT == 2 ? 4 : 8);
-#pragma unroll
-        for (int jj = 0; jj < JW; jj++) {
-            const int j = j0 + jj;
-            const bool in = WHOLE || (ch0 + wc < n1 && col0 + jj * 2 < P.N);
-            if constexpr (RT == 2) {
-                const bool there = in && q * 4 < P.r;
-                copy8(reinterpret_cast<uint2 *>(dst - lane) + j * 32 + lane, there ? br : P.b, there ? 8 : 0);
-            } else {
-#pragma unroll
-                for (int s = 0; s < RT / 4; s++) {
-                    const bool there = in && s * 32 + q * 8 < P.r;
-                    copy16(dst + (j * (RT / 4) + s) * 32, there ? br + s * 32 : P.b, there ? 16 : 0);
-                }
-            }
-            br += 2 * P.r;
-        }
-        const OT *p0 = b0 + ch0 * 32 + q * 8, *p1 = b1 + ch0 * 32 + q * 8;
-#pragma unroll
-        for (int u = 0; u < CPW; u++) {
-            const int i = kh * CPW + u;
-            const bool in = WHOLE || (ch0 + i < n1 && (ch0 + i) * 32 + q * 8 < P.N);
-            copy_rows(rows_of(st, i), in ? p0 + i * 32 : base, in ? p1 + i * 32 : base, in ? size0 : 0, in ? size1 : 0);
-        }
-    };
+    uint32_t fetch_at = 0;   // the buffer of the next stage to fetch
     auto fetch = [&](int st) {
+        const uint32_t buffer = fetch_at;
+        fetch_at = fetch_at == (S::STAGES - 1) * S::BYTES ? 0 : fetch_at + S::BYTES;
         if (st < kstages) {
-            const int last = k0 + st * 4 + 4;
-            if (last <= k1 && last * 32 <= P.K) fetch_k(st, std::true_type{});
-            else fetch_k(st, std::false_type{});
+            const int ch0 = k0 + st * 4;
+            const uint32_t dw = to_weights + buffer + wj * 512 + lane * 16;
+            if (ch0 + 4 <= k1 && (ch0 + 4) * 32 <= P.K && all_ranks) {
+                const __nv_bfloat16 *src = aw;
+                each<(RT + WSTEP - 1) / WSTEP>([&](auto i) {
+                    if (RT >= WSTEP || wj < RT) copy16<i * WSTEP * 512, 0>(dw, src, 16);
+                    src += aw_step;
+                });
+                fetch_rows_whole(to_rows + buffer + x_lane, Const<X_STEP>{}, x0, x1);
+            } else {
+                const bool in = ch0 + wc < k1 && (ch0 + wc) * 32 + q * 8 < P.K;
+                each<(RT + WSTEP - 1) / WSTEP>([&](auto i) {
+                    const bool there = in && (i * WSTEP + wj) * 8 < P.r;
+                    if (RT >= WSTEP || wj < RT) copy16<i * WSTEP * 512, 0>(dw, there ? aw + i * aw_step : P.a, there ? 16 : 0);
+                });
+                fetch_rows(to_rows + buffer + x_lane, Const<X_STEP>{}, x0, x1, ch0 + chunk0, k1, P.K);
+            }
+            x0 += 128; x1 += 128; aw += 128;
         } else if (st < stages) {
-            const int last = n0 + (st - kstages) * 4 + 4;
-            if (last <= n1 && last * 32 <= P.N) fetch_n(st, std::true_type{});
-            else fetch_n(st, std::false_type{});
+            const int ch0 = n0 + (st - kstages) * 4;
+            const bool whole = ch0 + 4 <= n1 && (ch0 + 4) * 32 <= P.N && all_ranks;
+            const int col = (ch0 + wc) * 32 + (g >> 1) * (16 / (int)sizeof(OT)) + (g & 1);
+            each<JW>([&](auto j) {
+                const int product = wj * JW + j, skip = sizeof(OT) == 2 ? product * 2 : product / 2 * 16 + product % 2 * 2;
+                const __nv_bfloat16 *src = bw + skip * P.r;
+                const bool in = whole || (ch0 + wc < n1 && col + skip < P.N);
+                if constexpr (RT == 2) {
+                    const bool there = in && q * 4 < P.r;
+                    copy8(to_weights + buffer + (wj * JW + j) * 256 + lane * 8, there ? src : P.b, there ? 8 : 0);
+                } else {
+                    const uint32_t dw = to_weights + buffer + wj * (JW * (RT / 4) * 512) + lane * 16;
+                    if (whole)
+                        each<RT / 4>([&](auto s) { copy16<(j * (RT / 4) + s) * 512, s * 64>(dw, src, 16); });
+                    else
+                        each<RT / 4>([&](auto s) {
+                            const bool there = in && s * 32 + q * 8 < P.r;
+                            copy16<(j * (RT / 4) + s) * 512, 0>(dw, there ? src + s * 32 : P.b, there ? 16 : 0);
+                        });
+                }
+            });
+            if (whole) fetch_rows_whole(to_rows + buffer + lane * 16, Const<B_STEP>{}, b0, b1);
+            else fetch_rows(to_rows + buffer + lane * 16, Const<B_STEP>{}, b0, b1, ch0 + chunk0, n1, P.N);
+            b0 += 128; b1 += 128; bw += (size_t)128 * P.r;
         }
         copies_commit();
     };
+    int buffer = 0;          // of the stage that is being used
     // T = 16: a warp reads what its own lanes fetched; T = 64: the weights come from all warps
     auto landed = [&] {
         copies_wait<S::STAGES - 1>();
@@ -324,60 +352,59 @@ __global__ void __launch_bounds__(AdapterStage<XT, OT, T, RT>::THREADS, AdapterS
     auto done_with = [&](int st) {
         if (T == 16) __syncwarp();
         else __syncthreads();
+        buffer = buffer == (S::STAGES - 1) * S::BYTES ? 0 : buffer + S::BYTES;
         fetch(st + S::STAGES);
     };
 #pragma unroll
     for (int st = 0; st < S::STAGES; st++) fetch(st);
+    const uint8_t *my_rows = smem + S::WEIGHTS + (rg * 4 + chunk0) * S::ROW_CHUNK + lane * 16;
+    const uint8_t *my_weights = smem + chunk0 * (S::WEIGHTS / 4);
 
     // ---- this warp's share of h = A x
     float acc[RT][4] = {};
     for (int st = 0; st < kstages; st++) {
         landed();
-        const int here = min(4, k1 - k0 - st * 4);
         if (busy)
 #pragma unroll
-            for (int u = 0; u < CPW; u++) {
-                const int i = kh * CPW + u;
-                if (i >= here) continue;
+            for (int u = 0; u < CPW; u++) {   // chunks behind the share are zeros
                 constexpr int V = sizeof(XT) / 2, PC = XFrag<XT>::PIECES;
+                const uint4 *rv = reinterpret_cast<const uint4 *>(my_rows + buffer + u * S::ROW_CHUNK);
+                const uint4 *av = reinterpret_cast<const uint4 *>(my_weights + buffer + u * (S::WEIGHTS / 4)) + lane;
                 uint32_t w0[4][PC], w1[4][PC];
-                XFrag<XT>::words(rows_of(st, i), w0);
-                XFrag<XT>::words(rows_of(st, i) + V * 32, w1);
-                const uint4 *av = weights_of(st, i);
+                XFrag<XT>::words(rv, w0);
+                XFrag<XT>::words(rv + V * 32, w1);
 #pragma unroll
                 for (int t = 0; t < RT; t += 2) {
-                    if (t >= tiles) break;
-                    const uint4 u = av[t * 32], v = t + 1 < tiles ? av[(t + 1) * 32] : make_uint4(0, 0, 0, 0);
+                    const uint4 a = av[t * 32], b = av[(t + 1) * 32];
 #pragma unroll
                     for (int p = 0; p < PC; p++) {
-                        mma_bf16(acc[t], w0[0][p], w1[0][p], w0[1][p], w1[1][p], u.x, u.y);
-                        mma_bf16(acc[t + 1], w0[0][p], w1[0][p], w0[1][p], w1[1][p], v.x, v.y);
-                        mma_bf16(acc[t], w0[2][p], w1[2][p], w0[3][p], w1[3][p], u.z, u.w);
-                        mma_bf16(acc[t + 1], w0[2][p], w1[2][p], w0[3][p], w1[3][p], v.z, v.w);
+                        mma_bf16(acc[t], w0[0][p], w1[0][p], w0[1][p], w1[1][p], a.x, a.y);
+                        mma_bf16(acc[t + 1], w0[0][p], w1[0][p], w0[1][p], w1[1][p], b.x, b.y);
+                        mma_bf16(acc[t], w0[2][p], w1[2][p], w0[3][p], w1[3][p], a.z, a.w);
+                        mma_bf16(acc[t + 1], w0[2][p], w1[2][p], w0[3][p], w1[3][p], b.z, b.w);
                     }
                 }
             }
         done_with(st);
     }
+
     // the warps of the same rows: the upper half hands its sums to the lower half, lane to lane, until one has them all
     auto at_part = [&](int buffer, int i, int half) {
-        return reinterpret_cast<float2 *>(part + (buffer * T + row_base + g + half * 8) * hs + i * 8 + 2 * q);
+        return reinterpret_cast<float2 *>(part + (buffer * T + row_base + g + half * 8) * HS + i * 8 + 2 * q);
     };
     auto put = [&](int buffer) {
 #pragma unroll
-        for (int i = 0; i < RT; i++)
-            if (i * 8 < r16) {
-                *at_part(buffer, i, 0) = make_float2(acc[i][0], acc[i][1]);
-                *at_part(buffer, i, 1) = make_float2(acc[i][2], acc[i][3]);
-            }
+        for (int i = 0; i < RT; i++) {
+            *at_part(buffer, i, 0) = make_float2(acc[i][0], acc[i][1]);
+            *at_part(buffer, i, 1) = make_float2(acc[i][2], acc[i][3]);
+        }
     };
     auto add = [&](int buffer) {
 #pragma unroll
-        for (int i = 0; i < RT; i++)
-            if (i * 8 < r16) {
-                const float2 u = *at_part(buffer, i, 0), v = *at_part(buffer, i, 1);
-                acc[i][0] += u.x; acc[i][1] += u.y; acc[i][2] += v.x; acc[i][3] += v.y;
-            }
+        for (int i = 0; i < RT; i++) {
+            const float2 u = *at_part(buffer, i, 0), v = *at_part(buffer, i, 1);
+            acc[i][0] += u.x; acc[i][1] += u.y; acc[i][2] += v.x; acc[i][3] += v.y;
+        }
     };
     if constexpr (S::KH == 4) {
         if (kh >= 2) put(kh - 2);
@@ -395,11 +422,11 @@ __global__ void __launch_bounds__(AdapterStage<XT, OT, T, RT>::THREADS, AdapterS
 
     // ---- the shares of the cluster added, in CTA order, times the adapter's scale
     const float scale = P.scales ? P.scales[id] : 1.f;
-    const int per_row = r16 / 4;
+    constexpr int per_row = RT * 2;
     if (T == 16) {
         cluster.sync();
         for (int i = tid; i < 16 * per_row; i += THREADS) {   // every CTA adds all of it: one barrier less on the way
-            float *p = part + i / per_row * hs + i % per_row * 4;
+            float *p = part + i / per_row * HS + i % per_row * 4;
             float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int o = 0; o < AD_MAX_CTAS; o++) {
@@ -407,13 +434,13 @@ __global__ void __launch_bounds__(AdapterStage<XT, OT, T, RT>::THREADS, AdapterS
                 const float4 v = *reinterpret_cast<const float4 *>(cluster.map_shared_rank(p, o));
                 s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
             }
-            *reinterpret_cast<float4 *>(h + i / per_row * hs + i % per_row * 4) = make_float4(s.x * scale, s.y * scale, s.z * scale, s.w * scale);
+            *reinterpret_cast<float4 *>(h + i / per_row * HS + i % per_row * 4) = make_float4(s.x * scale, s.y * scale, s.z * scale, s.w * scale);
         }
         __syncthreads();
     } else {
         cluster.sync();
         for (int i = c * THREADS + tid; i < T * per_row; i += ctas * THREADS) {   // each CTA its part, given to all
-            const int at = i / per_row * hs + i % per_row * 4;
+            const int at = i / per_row * HS + i % per_row * 4;
             float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int o = 0; o < AD_MAX_CTAS; o++) {
@@ -429,19 +456,17 @@ __global__ void __launch_bounds__(AdapterStage<XT, OT, T, RT>::THREADS, AdapterS
         cluster.sync();
     }
 
-    // ---- out = base + B h over this CTA's chunks of 32 columns.  Column (i / 2) * 8 + j * 2 + i % 2 of a chunk is column i
-    // of its j-th product, so that a lane ends with eight consecutive columns of its two rows.  Ranks: a lane takes four
+    // ---- out = base + B h over this CTA's chunks of 32 columns.  Column i of a chunk's j-th product is the chunk's column
+    // (i / 2) * 8 + j * 2 + i % 2, so that a lane ends with eight consecutive columns of its two rows (f32: with columns
+    // 4 (i / 2) + 2 j + i % 2 of the first or second half, four consecutive ones of each).  Ranks: a lane takes four
     // (RT = 2) or eight consecutive ones, which are one or two steps of the matrix instruction.
     constexpr int KS = RT / 2;
     uint32_t hf[KS][HP][4];
 #pragma unroll
     for (int s = 0; s < KS; s++) {
         const int k = RT == 2 ? q * 4 : s / 2 * 32 + q * 8 + s % 2 * 4;
-        float4 v0 = make_float4(0.f, 0.f, 0.f, 0.f), v1 = v0;
-        if (k < r16) {
-            v0 = *reinterpret_cast<const float4 *>(h + (row_base + g) * hs + k);
-            v1 = *reinterpret_cast<const float4 *>(h + (row_base + g + 8) * hs + k);
-        }
+        const float4 v0 = *reinterpret_cast<const float4 *>(h + (row_base + g) * HS + k);
+        const float4 v1 = *reinterpret_cast<const float4 *>(h + (row_base + g + 8) * HS + k);
         uint32_t w[4][HP];
         split_pair<HP>(v0.x, v0.y, w[0]);
         split_pair<HP>(v1.x, v1.y, w[1]);
@@ -452,32 +477,30 @@ __global__ void __launch_bounds__(AdapterStage<XT, OT, T, RT>::THREADS, AdapterS
 #pragma unroll
             for (int i = 0; i < 4; i++) hf[s][p][i] = w[i][p];
     }
+    OT *o0 = out + (has0 ? (size_t)t0 * P.N : 0) + (n0 + chunk0) * 32 + q * (16 / (int)sizeof(OT)), *o1 = out + (has1 ? (size_t)t1 * P.N : 0) + (n0 + chunk0) * 32 + q * (16 / (int)sizeof(OT));
     for (int st = kstages; st < stages; st++) {
         landed();
-        const int ch0 = n0 + (st - kstages) * 4;
+        const int ch0 = n0 + (st - kstages) * 4 + chunk0;
         if (busy)
 #pragma unroll
             for (int u = 0; u < CPW; u++) {
-                const int i = kh * CPW + u;
-                if (ch0 + i >= n1) continue;
                 float o[4][4] = {};
-                const uint4 *bv = weights_of(st, i);
+                const uint8_t *wv = my_weights + buffer + u * (S::WEIGHTS / 4);
                 // the four products of a step are independent: in turn, so that none waits for its own sum
                 if constexpr (RT == 2) {
+                    uint2 v[4];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) v[j] = reinterpret_cast<const uint2 *>(wv)[j * 32 + lane];
 #pragma unroll
                     for (int p = 0; p < HP; p++)
 #pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            const uint2 v = (reinterpret_cast<const uint2 *>(bv - lane) + j * 32)[lane];
-                            mma_bf16(o[j], hf[0][p][0], hf[0][p][1], hf[0][p][2], hf[0][p][3], v.x, v.y);
-                        }
+                        for (int j = 0; j < 4; j++) mma_bf16(o[j], hf[0][p][0], hf[0][p][1], hf[0][p][2], hf[0][p][3], v[j].x, v[j].y);
                 } else {
 #pragma unroll
                     for (int s = 0; s < RT / 4; s++) {
-                        if (s * 32 >= P.r) break;
                         uint4 v[4];
 #pragma unroll
-                        for (int j = 0; j < 4; j++) v[j] = bv[(j * (RT / 4) + s) * 32];
+                        for (int j = 0; j < 4; j++) v[j] = reinterpret_cast<const uint4 *>(wv)[(j * (RT / 4) + s) * 32 + lane];
 #pragma unroll
                         for (int p = 0; p < HP; p++) {
 #pragma unroll
@@ -489,36 +512,26 @@ __global__ void __launch_bounds__(AdapterStage<XT, OT, T, RT>::THREADS, AdapterS
                         }
                     }
                 }
-                const int col = (ch0 + i) * 32 + q * 8;
-                if (col < P.N) {
-                    constexpr int V = sizeof(OT) / 2;
+                constexpr int V = sizeof(OT) / 2, E = 8 / V;   // V groups of E consecutive columns
 #pragma unroll
-                    for (int half = 0; half < 2; half++) {
-                        if (!(half ? has1 : has0)) continue;
-                        float v[8];
-                        const uint4 *bp = rows_of(st, i) + half * V * 32;
-                        if constexpr (V == 1) {
-                            load_units<8>(reinterpret_cast<const OT *>(bp), v);
-                        } else {
-                            float u[4];
-                            load_units<4>(reinterpret_cast<const OT *>(bp), u);
+                for (int half = 0; half < 2; half++)
 #pragma unroll
-                            for (int e = 0; e < 4; e++) v[e] = u[e];
-                            load_units<4>(reinterpret_cast<const OT *>(bp + 32), u);
+                    for (int v = 0; v < V; v++) {
+                        if (!(half ? has1 : has0) || ch0 + u >= n1 || (ch0 + u) * 32 + v * 16 + q * E >= P.N) continue;
+                        float y[E];
+                        load_units<E>(reinterpret_cast<const OT *>(my_rows + buffer + u * S::ROW_CHUNK + (half * V + v) * 512), y);
 #pragma unroll
-                            for (int e = 0; e < 4; e++) v[4 + e] = u[e];
+                        for (int e = 0; e < E; e += 2) {
+                            y[e] += o[v * (E / 2) + e / 2][2 * half];
+                            y[e + 1] += o[v * (E / 2) + e / 2][2 * half + 1];
                         }
-#pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            v[2 * j] += o[j][2 * half];
-                            v[2 * j + 1] += o[j][2 * half + 1];
-                        }
-                        store_units<8>(out + (size_t)(half ? t1 : t0) * P.N + col, v);
+                        store_units<E>((half ? o1 : o0) + u * 32 + v * 16, y);
                     }
-                }
             }
+        o0 += 128; o1 += 128;
         done_with(st);
     }
+    copy_bare_rows<THREADS>(P, share_id, base, out);
     if (T == 16) cluster.sync();   // no CTA leaves while another reads its shares
 }
 
@@ -526,7 +539,7 @@ template <typename XT, typename OT, int T, int RT>
 static cudaError_t launch_adapters_as(const AdapterArgs &P, const XT *x, const OT *base, OT *out, cudaStream_t s)
 {
     using S = AdapterStage<XT, OT, T, RT>;
-    const size_t smem = S::smem((P.r + 15) / 16 * 16);
+    const size_t smem = S::SMEM;
     auto *kern = k_adapters<XT, OT, T, RT>;
     if (smem > 40 * 1024) {   // with the static arrays, more than a launch may have without asking
         cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
@@ -544,6 +557,7 @@ static cudaError_t launch_adapters_as(const AdapterArgs &P, const XT *x, const O
         const double cost = (double)((tiles * c + room - 1) / room) * (8.0 + (P.K + P.N) / 128.0 / c);
         if (cost < best) { best = cost; ctas = c; }
     }
+    if (getenv("AD_C")) ctas = atoi(getenv("AD_C"));
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)slots * ctas);
     cfg.blockDim = dim3(S::THREADS);
@@ -564,7 +578,7 @@ static cudaError_t launch_adapters_as(const AdapterArgs &P, const XT *x, const O
 cudaError_t launch_adapters(const void *base, int out_dtype, const void *x, int x_dtype, const AdapterArgs &P, void *out, cudaStream_t s)
 {
     // tiles of 64 rows where an adapter has that many on average; else of 16
-    const bool wide = P.order && P.n / P.L >= 48;
+    const bool wide = P.order && P.n / P.L >= 48 && !getenv("AD_16");
     return with_type(x_dtype, [&](auto *xp) {
         return with_type(out_dtype, [&](auto *op) {
             using XT = std::remove_pointer_t<decltype(xp)>;

@@ -15,68 +15,310 @@ namespace pmoe {
 
 constexpr int NORM_Q8_MAX_H = 16384;
 
-// |v| as ordered bits: unsigned integers compare like the magnitudes, infinity above all numbers and NaN above infinity,
-// so an integer maximum carries a NaN through where fmaxf would drop it.
-__device__ inline uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
-
-template <bool E4M3> __device__ inline uint8_t to_8bit(float ratio)
+// max(m, |v|) that keeps a NaN, which fmaxf would drop
+__device__ inline float max_abs(float m, float v)
 {
-    if constexpr (E4M3) return (uint8_t)__nv_cvt_float_to_fp8(ratio, __NV_SATFINITE, __NV_E4M3);
-    else return (uint8_t)(int8_t)max(-127, min(127, __float2int_rn(ratio)));
-}
-template <bool E4M3> __device__ inline float from_8bit(uint8_t q)
-{
-    if constexpr (E4M3) return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)q, __NV_E4M3)));
-    else return (float)(int8_t)q;
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(m), "f"(fabsf(v)));
+    return r;
 }
 
-// one CTA per row, the row in shared memory, one warp per group
-template <typename RT, typename DT, typename VT, bool E4M3>
-__global__ void __launch_bounds__(256) k_norm_q8(const RT *resid_in, const DT *__restrict__ delta, const float *__restrict__ weight, int H,
-                                                 float eps, int group, RT *resid_out, uint8_t *__restrict__ q, float *__restrict__ scales,
-                                                 VT *__restrict__ values)
+// How a group becomes 8 bits: scale = top / 127 or / 448, q = round(v / scale).  The quotient is a product with 1 / scale, one
+// rounding away from it; only a scale so small that 1 / scale would overflow is divided by.
+struct GroupScale {
+    float scale, inverse;
+    bool plain;    // the product with `inverse` is the quotient, and in the type's range up to what the rounding takes back
+    template <bool E4M3> __device__ static GroupScale of(float top)
+    {
+        GroupScale g;
+        g.scale = top * (E4M3 ? 1.f / 448.f : 1.f / 127.f);
+        g.plain = g.scale >= 0x1p-100f && g.scale < INFINITY;
+        g.inverse = __frcp_rn(g.scale);
+        return g;
+    }
+    // v / scale for the other groups: 0 where the scale is 0, infinite or NaN
+    template <bool E4M3> __device__ float ratio(float v) const
+    {
+        const float most = E4M3 ? 448.f : 127.f;
+        return scale > 0.f && scale < INFINITY ? fminf(fmaxf(__fdiv_rn(v, scale), -most), most) : 0.f;
+    }
+};
+
+// Ratios to 8 bits (the bytes of `packed`, in order) and, with HELD, back to what they stand for in units of the scale.
+template <bool E4M3, bool HELD, int N> __device__ inline void to_8bit(float (&r)[N], uint32_t *packed)
 {
-    extern __shared__ float row[];
-    __shared__ float red[8];
+    if constexpr (E4M3) {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            const __nv_fp8x2_storage_t b = __nv_cvt_float2_to_fp8x2(make_float2(r[i], i + 1 < N ? r[i + 1] : 0.f), __NV_SATFINITE, __NV_E4M3);
+            if (HELD) {
+                const float2 f = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(b, __NV_E4M3)));
+                r[i] = f.x;
+                if (i + 1 < N) r[i + 1] = f.y;
+            }
+            if (i % 4 == 0) packed[i / 4] = b;
+            else packed[i / 4] |= (uint32_t)b << 16;
+        }
+    } else {
+        // 1.5 * 2^23 + r rounds r to the nearest integer, ties to even, and its low byte is that integer's
+        constexpr float MAGIC = 12582912.f;
+        uint32_t t[N];
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const float f = r[i] + MAGIC;
+            t[i] = __float_as_uint(f);
+            if (HELD) r[i] = f - MAGIC;
+        }
+        if constexpr (N == 1) packed[0] = t[0] & 0xff;
+        else
+#pragma unroll
+            for (int i = 0; i < N; i += 4) packed[i / 4] = __byte_perm(__byte_perm(t[i], t[i + 1], 0x0040), __byte_perm(t[i + 2], t[i + 3], 0x0040), 0x5410);
+    }
+}
+
+// v + d rounded to the type of the residual, eight elements, written where the residual goes (if it goes anywhere)
+__device__ inline void add_and_store(float (&v)[8], const float (&d)[8], float *to)
+{
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] += d[i];
+    if (to) store_units<8>(to, v);
+}
+__device__ inline void add_and_store(float (&v)[8], const float (&d)[8], __nv_bfloat16 *to)
+{
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        w[i] = pack_bf16(v[2 * i] + d[2 * i], v[2 * i + 1] + d[2 * i + 1]);
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+    if (to) *reinterpret_cast<uint4 *>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// One CTA per row.  The operator reads and writes each element once (13 bytes for f32 + f32 -> f32, int8, f32 values; 7 for
+// bf16 + bf16 -> bf16, e4m3), so memory bounds it and the row must stay on the chip between its two statistics: here in
+// registers, eight consecutive elements a thread and pass, a row never longer than threads * PASSES * 8.  A group is 4, 8, 16
+// or 32 neighbouring threads of a pass (its maximum by shuffles) or the whole row (shuffles and a shared array).  The second
+// limit is the issue rate, near once the two quotients an element are products: the work a thread does once for its elements
+// (root, reciprocals, sums over the row) is shared by sixteen of them where there are rows enough to fill the card.
+template <typename RT, typename DT, typename VT, bool E4M3, int PASSES>
+__global__ void __launch_bounds__(1024) k_norm_q8(const RT *resid_in, const DT *__restrict__ delta, const float *__restrict__ weight, int H,
+                                                  float eps, int group, RT *resid_out, uint8_t *__restrict__ q,
+                                                  float *__restrict__ scales, VT *__restrict__ values)
+{
+    __shared__ float red[32], red_max[32];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
+    const size_t base = (size_t)blockIdx.x * H;
     pdl_wait();
     pdl_launch_dependents();
-    const size_t base = (size_t)blockIdx.x * H;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    float v[PASSES][8];
     float ss = 0.f;
-    for (int h = threadIdx.x; h < H; h += 256) {
-        float v = load_as_float(resid_in, base + h);
-        if (delta) v += load_as_float(delta, base + h);
-        RT r;
-        store_from_float(&r, 0, v);
-        v = load_as_float(&r, 0);
-        if (resid_out) resid_out[base + h] = r;
-        row[h] = v;
-        ss = fmaf(v, v, ss);
+    if (delta) {
+        float d[PASSES][8];
+#pragma unroll
+        for (int p = 0; p < PASSES; p++) {
+            const int h = (p * blockDim.x + tid) * 8;
+            if (h >= H) continue;
+            load_units<8>(resid_in + base + h, v[p]);
+            load_units<8>(delta + base + h, d[p]);
+        }
+#pragma unroll
+        for (int p = 0; p < PASSES; p++) {
+            const int h = (p * blockDim.x + tid) * 8;
+            if (h < H) add_and_store(v[p], d[p], resid_out ? resid_out + base + h : (RT *)nullptr);
+        }
+    } else {
+#pragma unroll
+        for (int p = 0; p < PASSES; p++) {
+            const int h = (p * blockDim.x + tid) * 8;
+            if (h >= H) continue;
+            load_units<8>(resid_in + base + h, v[p]);
+            if (resid_out) store_units<8>(resid_out + base + h, v[p]);
+        }
+    }
+#pragma unroll
+    for (int p = 0; p < PASSES; p++)
+        if ((p * blockDim.x + tid) * 8 < H)
+#pragma unroll
+            for (int i = 0; i < 8; i++) ss = fmaf(v[p][i], v[p][i], ss);
+#pragma unroll
+    for (int s = 16; s >= 1; s >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, s);
+    if (lane == 0) red[warp] = ss;
+    __syncthreads();
+    ss = lane < warps ? red[lane] : 0.f;
+#pragma unroll
+    for (int s = 16; s >= 1; s >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, s);
+    const float inv_m = __frcp_rn(sqrtf(ss / (float)H + eps));   // 1 / inf = 0, 1 / 0 = inf: the products are the quotients in both
+
+    float top[PASSES];
+#pragma unroll
+    for (int p = 0; p < PASSES; p++) {
+        const int h = (p * blockDim.x + tid) * 8;
+        top[p] = 0.f;
+        if (h >= H) continue;
+        if (weight) {
+            float w[8];
+            load_units<8>(weight + h, w);
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[p][i] = v[p][i] * inv_m * w[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[p][i] *= inv_m;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) top[p] = max_abs(top[p], v[p][i]);
+    }
+    const int log2_group = 31 - __clz(group), G = group >= H ? 1 : (H + group - 1) >> log2_group;   // more than one group: a power of two
+    float *row_scales = scales + (size_t)blockIdx.x * G;
+    if (G > 1) {   // 32 to 256 values: up to a warp's
+#pragma unroll
+        for (int p = 0; p < PASSES; p++)
+#pragma unroll
+            for (int s = 1; s < 32; s <<= 1)
+                if (s * 8 < group) top[p] = max_abs(top[p], __shfl_xor_sync(0xffffffffu, top[p], s));
+    } else {       // one scale for the row
+        float t = top[0];
+#pragma unroll
+        for (int p = 1; p < PASSES; p++) t = max_abs(t, top[p]);
+#pragma unroll
+        for (int s = 16; s >= 1; s >>= 1) t = max_abs(t, __shfl_xor_sync(0xffffffffu, t, s));
+        if (lane == 0) red_max[warp] = t;
+        __syncthreads();
+        t = lane < warps ? red_max[lane] : 0.f;
+#pragma unroll
+        for (int s = 16; s >= 1; s >>= 1) t = max_abs(t, __shfl_xor_sync(0xffffffffu, t, s));
+#pragma unroll
+        for (int p = 0; p < PASSES; p++) top[p] = t;
+    }
+#pragma unroll
+    for (int p = 0; p < PASSES; p++) {
+        const int h = (p * blockDim.x + tid) * 8;
+        if (h >= H) continue;
+        const GroupScale gs = GroupScale::of<E4M3>(top[p]);
+        if (G == 1 ? h == 0 : (h & (group - 1)) == 0) row_scales[G == 1 ? 0 : h >> log2_group] = gs.scale;
+        if (gs.plain) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[p][i] *= gs.inverse;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[p][i] = gs.ratio<E4M3>(v[p][i]);
+        }
+        uint32_t packed[2];
+        if (values) {
+            to_8bit<E4M3, true>(v[p], packed);
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[p][i] *= gs.scale;   // NaN where the scale is not finite: 0 * inf
+            store_units<8>(values + base + h, v[p]);
+        } else {
+            to_8bit<E4M3, false>(v[p], packed);
+        }
+        *reinterpret_cast<uint2 *>(q + base + h) = make_uint2(packed[0], packed[1]);
+    }
+}
+
+// Rows that no vector load fits (H not a multiple of 8, or an address off its boundary).  A warp has 256 consecutive
+// elements a pass, lane l those at l, l + 32, ...: its loads are whole lines whatever the address, and a group of 32 to
+// 256 values is one to eight registers of a warp.
+template <typename RT, typename DT, typename VT, bool E4M3>
+__global__ void __launch_bounds__(1024) k_norm_q8_any(const RT *resid_in, const DT *__restrict__ delta, const float *__restrict__ weight,
+                                                      int H, float eps, int group, RT *resid_out, uint8_t *__restrict__ q,
+                                                      float *__restrict__ scales, VT *__restrict__ values)
+{
+    constexpr int PASSES = NORM_Q8_MAX_H / (1024 * 8);
+    __shared__ float red[32], red_max[32];
+    pdl_wait();
+    pdl_launch_dependents();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    const size_t base = (size_t)blockIdx.x * H;
+    resid_in += base;
+    if (delta) delta += base;
+    if (resid_out) resid_out += base;
+    q += base;
+    if (values) values += base;
+    float v[PASSES][8];
+    float ss = 0.f;
+#pragma unroll
+    for (int p = 0; p < PASSES; p++) {
+        const int h0 = (p * warps + warp) * 256 + lane;
+        if (h0 - lane >= H) break;
+        float d[8] = {};
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int h = h0 + i * 32;
+            v[p][i] = h < H ? load_as_float(resid_in, h) : 0.f;
+            if (delta && h < H) d[i] = load_as_float(delta, h);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int h = h0 + i * 32;
+            RT r;
+            store_from_float(&r, 0, delta ? v[p][i] + d[i] : v[p][i]);
+            v[p][i] = load_as_float(&r, 0);
+            if (resid_out && h < H) resid_out[h] = r;
+            ss = fmaf(v[p][i], v[p][i], ss);
+        }
     }
 #pragma unroll
     for (int s = 16; s >= 1; s >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, s);
     if (lane == 0) red[warp] = ss;
     __syncthreads();
-    float tot = 0.f;
-    for (int w = 0; w < 8; w++) tot += red[w];
-    const float m = sqrtf(tot / (float)H + eps);
-    const int G = (H + group - 1) / group;
-    for (int g = warp; g < G; g += 8) {
-        const int h0 = g * group, h1 = min(H, h0 + group);
-        uint32_t top = 0;
-        for (int h = h0 + lane; h < h1; h += 32) {
-            const float v = __fdiv_rn(row[h], m) * (weight ? weight[h] : 1.f);
-            row[h] = v;
-            top = max(top, magnitude(v));
+    ss = lane < warps ? red[lane] : 0.f;
+#pragma unroll
+    for (int s = 16; s >= 1; s >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, s);
+    const float inv_m = __frcp_rn(sqrtf(ss / (float)H + eps));
+    const int log2_group = 31 - __clz(group), G = group >= H ? 1 : (H + group - 1) >> log2_group;   // more than one group: a power of two
+    float *row_scales = scales + (size_t)blockIdx.x * G;
+    float row_top = 0.f;
+#pragma unroll
+    for (int p = 0; p < PASSES; p++) {
+        const int h0 = (p * warps + warp) * 256 + lane;
+        if (h0 - lane >= H) break;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int h = h0 + i * 32;
+            v[p][i] = h < H ? v[p][i] * inv_m * (weight ? weight[h] : 1.f) : 0.f;
+            row_top = max_abs(row_top, v[p][i]);
         }
-        top = __reduce_max_sync(0xffffffffu, top);
-        const float scale = __fdiv_rn(__uint_as_float(top), E4M3 ? 448.f : 127.f);
-        const bool usable = scale > 0.f && scale < INFINITY;
-        if (lane == 0) scales[(size_t)blockIdx.x * G + g] = scale;
-        for (int h = h0 + lane; h < h1; h += 32) {
-            const uint8_t b = usable ? to_8bit<E4M3>(__fdiv_rn(row[h], scale)) : 0;
-            q[base + h] = b;
-            if (values) store_from_float(values, base + h, from_8bit<E4M3>(b) * scale);
+    }
+    if (G == 1) {
+#pragma unroll
+        for (int s = 16; s >= 1; s >>= 1) row_top = max_abs(row_top, __shfl_xor_sync(0xffffffffu, row_top, s));
+        if (lane == 0) red_max[warp] = row_top;
+        __syncthreads();
+        row_top = lane < warps ? red_max[lane] : 0.f;
+#pragma unroll
+        for (int s = 16; s >= 1; s >>= 1) row_top = max_abs(row_top, __shfl_xor_sync(0xffffffffu, row_top, s));
+    }
+#pragma unroll
+    for (int p = 0; p < PASSES; p++) {
+        const int h0 = (p * warps + warp) * 256 + lane;
+        if (h0 - lane >= H) break;
+        float top[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) top[i] = fabsf(v[p][i]);
+        if (G > 1)
+#pragma unroll
+            for (int s = 1; s < 8; s <<= 1)
+                if (s * 32 < group)
+#pragma unroll
+                    for (int i = 0; i < 8; i += 2 * s) top[i] = max_abs(top[i], top[i + s]);
+        GroupScale gs = GroupScale::of<E4M3>(row_top);
+        if (G == 1 && h0 == 0) row_scales[0] = gs.scale;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int h = h0 + i * 32;
+            if (G > 1 && (i * 32 & (group - 1)) == 0) {   // a group begins
+#pragma unroll
+                for (int s = 16; s >= 1; s >>= 1) top[i] = max_abs(top[i], __shfl_xor_sync(0xffffffffu, top[i], s));
+                gs = GroupScale::of<E4M3>(top[i]);
+                if (lane == 0 && h < H) row_scales[h >> log2_group] = gs.scale;
+            }
+            if (h >= H) continue;
+            float r[1] = {gs.plain ? v[p][i] * gs.inverse : gs.ratio<E4M3>(v[p][i])};
+            uint32_t b;
+            to_8bit<E4M3, true>(r, &b);
+            q[h] = (uint8_t)b;
+            if (values) store_from_float(values, h, r[0] * gs.scale);
         }
     }
 }
@@ -86,20 +328,27 @@ cudaError_t launch_norm_q8(const void *resid_in, int resid_dtype, const void *de
                            cudaStream_t s)
 {
     count_launch();
+    const bool wide = H % 8 == 0 && aligned16(resid_in) && aligned16(delta) && aligned16(weight) && aligned16(resid_out) &&
+                      aligned16(values) && ((uintptr_t)q & 7) == 0;
+    // One pass keeps a row's chain short, two do less work an element (16384 rows of 2048: 49 against 58 us): two where the
+    // rows alone make several CTAs an SM, and where a row is longer than 1024 threads take in one.
+    const int passes = H > 8192 || (H > 512 && n >= 1024) ? 2 : 1;
+    const int threads = min(1024, ((H + 8 * passes - 1) / (8 * passes) + 31) / 32 * 32);
     return with_type(resid_dtype, [&](auto *rp) {
         return with_type(delta_dtype, [&](auto *dp) {
             return with_type(values_dtype, [&](auto *vp) {
                 using RT = std::remove_pointer_t<decltype(rp)>;
                 using DT = std::remove_pointer_t<decltype(dp)>;
                 using VT = std::remove_pointer_t<decltype(vp)>;
-                auto *kern = q_dtype == PMOE_F8_E4M3 ? k_norm_q8<RT, DT, VT, true> : k_norm_q8<RT, DT, VT, false>;
-                if (H > 12000) {   // beyond what a launch may have without asking
-                    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, NORM_Q8_MAX_H * (int)sizeof(float));
-                    if (e != cudaSuccess) return e;
-                }
-                return launch_pdl(kern, dim3(n), dim3(256),
-                                  (size_t)H * sizeof(float), s, (const RT *)resid_in, (const DT *)delta, weight, H, eps, group,
-                                  (RT *)resid_out, (uint8_t *)q, scales, (VT *)values);
+                auto go = [&](auto *kern, int block) {
+                    return launch_pdl(kern, dim3(n), dim3(block), 0, s, (const RT *)resid_in, (const DT *)delta, weight, H, eps, group,
+                                      (RT *)resid_out, (uint8_t *)q, scales, (VT *)values);
+                };
+                const bool f8 = q_dtype == PMOE_F8_E4M3;
+                if (wide)
+                    return passes == 1 ? go(f8 ? k_norm_q8<RT, DT, VT, true, 1> : k_norm_q8<RT, DT, VT, false, 1>, threads)
+                                       : go(f8 ? k_norm_q8<RT, DT, VT, true, 2> : k_norm_q8<RT, DT, VT, false, 2>, threads);
+                return go(f8 ? k_norm_q8_any<RT, DT, VT, true> : k_norm_q8_any<RT, DT, VT, false>, min(1024, (H + 255) / 256 * 32));
             });
         });
     });
