@@ -9,6 +9,8 @@
 // The order is stable, so all of it is a function of idx alone (the block's grouping leaves the order inside an expert
 // to its atomics).
 #include <cooperative_groups.h>
+#include <initializer_list>
+#include <utility>
 
 #include "pmoe_internal.h"
 #include "pmoe_vec.cuh"
@@ -19,18 +21,20 @@ namespace cg = cooperative_groups;
 
 // ---------------------------------------------------------------- sort
 // A counting sort in one launch, by one CTA or by a cluster of eight.  Every warp owns a run of consecutive pairs, takes it
-// 32 pairs at a time, and ranks the pairs of such a step among those of the same expert with __match_any_sync: ranks
+// 32 pairs at a time, and ranks the pairs of such a step among those of the same expert: ranks
 // inside the step, steps, warps and CTAs are four levels of the same order, so the result is stable without atomics.
 //   1. cnt[w][e]  pairs of expert e in warp w's run
 //   2. the CTAs' totals are exchanged through distributed shared memory; exclusive scan over (e, CTA, w): cnt[w][e]
 //      becomes the place of that warp's first pair of e
 //   3. the runs once more: place = cnt[w][e] + rank inside the step
-// The pairs are few bytes (4 to read, 8 to write): what counts is latency, so a lane loads its keys of eight steps at once
-// and keeps them from 1. to 3. where the run is no longer than that.
+// The pairs are few bytes (4 to read, 8 to write): what counts is latency, so a lane loads its keys of sixteen steps at once
+// and keeps them, with their ranks, from 1. to 3. where the run is no longer than that.  The lanes of the same expert are
+// found with one ballot per bit of the expert's number: __match_any_sync gives them in one instruction, which with 32 warps on
+// it took most of the time (40960 pairs of 512 experts: 17 us).
 constexpr int SORT_MAX_E = 4096;
 constexpr int SORT_THREADS = 1024;
 constexpr int SORT_CTAS = 8;
-constexpr int SORT_BATCH = 8;
+constexpr int SORT_BATCH = 16;
 constexpr int SORT_ONE_CTA = 4096;   // pairs up to which one CTA sorts
 
 struct SortKeys {
@@ -43,9 +47,22 @@ struct SortKeys {
     }
 };
 
+// the lanes whose key equals this lane's, among the lanes with a key below E (others get no lane)
+__device__ inline unsigned lanes_of_key(uint32_t key, uint32_t E, int bits)
+{
+    unsigned same = __ballot_sync(0xffffffffu, key < E);
+    if (key >= E) same = 0;
+    for (int b = 0; b < bits; b++) {
+        const bool set = (key >> b) & 1;
+        const unsigned m = __ballot_sync(0xffffffffu, set);
+        same &= set ? m : ~m;
+    }
+    return same;
+}
+
 template <int CTAS>
 __global__ void __launch_bounds__(SORT_THREADS) k_sort_pairs(const uint32_t *__restrict__ idx, int P, uint32_t base, int E, int warps,
-                                                             int run, int *__restrict__ order, int *__restrict__ place,
+                                                             int bits, int run, int *__restrict__ order, int *__restrict__ place,
                                                              int *__restrict__ offsets)
 {
     extern __shared__ int cnt[];   // [warps][E], then this CTA's totals [E]
@@ -54,13 +71,15 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_pairs(const uint32_t *__r
     const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = CTAS > 1 ? (int)cluster.block_rank() : 0;
-    for (int i = tid; i < warps * E; i += SORT_THREADS) cnt[i] = 0;
+    for (int i = tid; i < warps * E / 4; i += SORT_THREADS) reinterpret_cast<int4 *>(cnt)[i] = make_int4(0, 0, 0, 0);
+    if (tid < warps * E % 4) cnt[warps * E / 4 * 4 + tid] = 0;
     pdl_wait();
     pdl_launch_dependents();
 
     const int64_t p0 = min((int64_t)P, (int64_t)(rank * warps + w) * run), p1 = w < warps ? min((int64_t)P, p0 + run) : p0;
     const bool once = run <= SORT_BATCH * 32;
     SortKeys keys;
+    uint16_t rank_of[SORT_BATCH];   // of the run's only batch: earlier lanes of the step with this key, and all of them << 8
     keys.load(idx, p0, p1, base, lane);
     __syncthreads();
     for (int64_t p = p0; p < p1; p += SORT_BATCH * 32) {
@@ -69,8 +88,10 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_pairs(const uint32_t *__r
         for (int i = 0; i < SORT_BATCH; i++) {
             if (p + i * 32 >= p1) break;
             const uint32_t key = keys.v[i];
-            const unsigned same = __match_any_sync(0xffffffffu, key);
-            if (key < (uint32_t)E && lane == __ffs(same) - 1) cnt[w * E + key] += __popc(same);
+            const unsigned same = lanes_of_key(key, E, bits);
+            const int nth = __popc(same & ((1u << lane) - 1)), all = __popc(same);
+            rank_of[i] = (uint16_t)(nth | all << 8);
+            if (same && nth == 0) cnt[w * E + key] += all;
             __syncwarp();
         }
     }
@@ -140,12 +161,16 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_pairs(const uint32_t *__r
             const int64_t pair = p + i * 32 + lane;
             if (p + i * 32 >= p1) break;
             const uint32_t key = keys.v[i];
-            const unsigned same = __match_any_sync(0xffffffffu, key);
-            const int nth = __popc(same & ((1u << lane) - 1));
+            int nth = rank_of[i] & 255, all = rank_of[i] >> 8;
+            if (!once) {
+                const unsigned same = lanes_of_key(key, E, bits);
+                nth = __popc(same & ((1u << lane) - 1));
+                all = __popc(same);
+            }
             int at = -1;
             if (key < (uint32_t)E) at = cnt[w * E + key] + nth;
             __syncwarp();
-            if (key < (uint32_t)E && nth == 0) cnt[w * E + key] = at + __popc(same);
+            if (key < (uint32_t)E && nth == 0) cnt[w * E + key] = at + all;
             __syncwarp();
             if (pair < p1) {
                 if (place) place[pair] = at;
@@ -165,6 +190,8 @@ cudaError_t launch_sort_pairs(const uint32_t *idx, int P, int base, int E, int *
     const bool one = P <= SORT_ONE_CTA;
     const int ctas = one ? 1 : SORT_CTAS;
     const int warps = min(most, max(1, (P + 31) / 32 / ctas));
+    int bits = 0;
+    while ((1 << bits) < E) bits++;
     const int run = (int)((((int64_t)P + ctas * warps - 1) / (ctas * warps) + 31) / 32 * 32);
     const size_t smem = (size_t)(warps + 1) * E * sizeof(int);
     auto *kern = one ? k_sort_pairs<1> : k_sort_pairs<SORT_CTAS>;
@@ -186,28 +213,57 @@ cudaError_t launch_sort_pairs(const uint32_t *idx, int P, int base, int E, int *
     cfg.attrs = at;
     cfg.numAttrs = one ? 1 : 2;
     count_launch();
-    return cudaLaunchKernelEx(&cfg, kern, idx, P, (uint32_t)base, E, warps, run, order, place, offsets);
+    return cudaLaunchKernelEx(&cfg, kern, idx, P, (uint32_t)base, E, warps, bits, run, order, place, offsets);
 }
 
-// ---------------------------------------------------------------- dispatch
-// Rows are moved as bytes, so any element type goes: one CTA per token reads the row once and writes it to the token's
-// places.  The rows behind the last kept pair are zeroed by the same CTAs.
+// ---------------------------------------------------------------- rows
+// Dispatch, combine and their gradients move every row once, so memory bounds them; what the kernels have to do is to keep
+// enough loads on their way for any row length and any number of rows.  A row is cut into units (16 bytes of a row where
+// its length and address allow), and a token gets as many threads as its row has units: 32 to 256 of them share a CTA with
+// other tokens' threads, a longer row takes several CTAs.
+struct RowThreads {
+    int log2_threads;   // threads of a token inside a CTA of 256
+    int ctas;           // CTAs of a token (1 unless its threads are all 256)
+    unsigned grid;
+    static RowThreads of(int64_t units, int n)
+    {
+        RowThreads r{5, 1, 0};
+        while ((1 << r.log2_threads) < units && r.log2_threads < 8) r.log2_threads++;
+        if (units > 256) r.ctas = (int)min((units + 255) / 256, (int64_t)max(1, (1 << 30) / n));
+        const int tokens = 256 >> r.log2_threads;
+        r.grid = (unsigned)((int64_t)((n + tokens - 1) / tokens) * r.ctas);
+        return r;
+    }
+    // the token of this thread, its first unit and the step to its next ones
+    __device__ void mine(int &t, int &first, int &step) const
+    {
+        t = (int)(blockIdx.x / ctas) * (256 >> log2_threads) + (threadIdx.x >> log2_threads);
+        first = (int)(blockIdx.x % ctas) * 256 + (threadIdx.x & ((1 << log2_threads) - 1));
+        step = ctas << log2_threads;
+    }
+};
+
+// Rows are moved as bytes, so any element type goes: a unit is read once and written to the token's places.  The rows behind
+// the last kept pair are zeroed by the same CTAs.
 template <typename V>
-__global__ void __launch_bounds__(256) k_dispatch_rows(const V *__restrict__ x, int units, int top_k, int P, const int *__restrict__ place,
-                                                       const int *__restrict__ offsets, int E, V *__restrict__ out)
+__global__ void __launch_bounds__(256) k_dispatch_rows(const V *__restrict__ x, int units, int n, int top_k, const int *__restrict__ place,
+                                                       const int *__restrict__ offsets, int E, V *__restrict__ out, RowThreads rt)
 {
     pdl_wait();
     pdl_launch_dependents();
-    const int t = blockIdx.x;
-    const int *pl = place + (size_t)t * top_k;
-    for (int u = threadIdx.x; u < units; u += 256) {
-        const V v = x[(size_t)t * units + u];
-        for (int j = 0; j < top_k; j++) {
-            const int at = pl[j];
-            if ((unsigned)at < (unsigned)P) out[(size_t)at * units + u] = v;
+    const int P = n * top_k;
+    int t, first, step;
+    rt.mine(t, first, step);
+    if (t < n)
+        for (int u = first; u < units; u += step) {
+            const V v = x[(size_t)t * units + u];
+#pragma unroll 4
+            for (int j = 0; j < top_k; j++) {
+                const int to = place[(size_t)t * top_k + j];
+                if ((unsigned)to < (unsigned)P) out[(size_t)to * units + u] = v;
+            }
         }
-    }
-    for (int64_t r = (int64_t)max(0, offsets[E]) + t; r < P; r += gridDim.x)
+    for (int64_t r = (int64_t)max(0, offsets[E]) + blockIdx.x; r < P; r += gridDim.x)
         for (int u = threadIdx.x; u < units; u += 256) out[(size_t)r * units + u] = V{};
 }
 
@@ -217,65 +273,102 @@ cudaError_t launch_dispatch_rows(const void *x, size_t row_bytes, int n, int top
     const uintptr_t a = (uintptr_t)x | (uintptr_t)out | row_bytes;
     auto go = [&](auto v) {
         using V = decltype(v);
-        return launch_pdl(k_dispatch_rows<V>, dim3(n), dim3(256), 0, s, (const V *)x, (int)(row_bytes / sizeof(V)), top_k, n * top_k,
-                          place, offsets, E, (V *)out);
+        const int units = (int)(row_bytes / sizeof(V));
+        const RowThreads rt = RowThreads::of(units, n);
+        return launch_pdl(k_dispatch_rows<V>, dim3(rt.grid), dim3(256), 0, s, (const V *)x, units, n, top_k, place, offsets, E, (V *)out, rt);
     };
     count_launch();
     return a % 16 == 0 ? go(uint4{}) : a % 8 == 0 ? go(uint2{}) : a % 4 == 0 ? go(0u) : a % 2 == 0 ? go((uint16_t)0) : go((uint8_t)0);
 }
 
-// ---------------------------------------------------------------- combine
-// out_t = extra_t + sum_j w_tj rows[place_tj], f32 in slot order, one CTA per token.  Without weights it is the
-// gradient of the dispatch.  (extra may be out: a thread reads the elements it later writes.)
+// out_t = extra_t + sum_j w_tj rows[place_tj], f32 in slot order.  Without weights it is the gradient of the dispatch.
+// Four rows are loaded before the first is added.  (extra may be out: a thread reads the elements it later writes.)
 template <int U, typename RT, typename ET, typename OT>
-__global__ void __launch_bounds__(256) k_combine_rows(const RT *__restrict__ rows, int H, int top_k, int n_rows,
+__global__ void __launch_bounds__(256) k_combine_rows(const RT *__restrict__ rows, int H, int n, int top_k, int n_rows,
                                                       const int *__restrict__ place, const float *__restrict__ w, const ET *extra,
-                                                      OT *out)
+                                                      OT *out, RowThreads rt)
 {
     pdl_wait();
     pdl_launch_dependents();
-    const int t = blockIdx.x;
-    for (int h = threadIdx.x * U; h < H; h += 256 * U) {
+    const int units = H / U;
+    int t, first, step;
+    rt.mine(t, first, step);
+    if (t >= n) return;
+    place += (size_t)t * top_k;
+    if (w) w += (size_t)t * top_k;
+    for (int u = first; u < units; u += step) {
         float acc[U] = {};
-        for (int j = 0; j < top_k; j++) {
-            const int at = place[(size_t)t * top_k + j];
-            if ((unsigned)at >= (unsigned)n_rows) continue;
-            const float wt = w ? w[(size_t)t * top_k + j] : 1.f;
-            float v[U];
-            load_units<U>(rows + (size_t)at * H + h, v);
+        for (int j = 0; j < top_k && n_rows > 0; j += 4) {
+            float v[4][U], f[4];
+            bool there[4];
 #pragma unroll
-            for (int i = 0; i < U; i++) acc[i] = fmaf(wt, v[i], acc[i]);
+            for (int i = 0; i < 4; i++) {
+                // four loads without a branch between them: the first row stands in for one that does not count
+                const int r = j + i < top_k ? place[j + i] : -1;
+                there[i] = (unsigned)r < (unsigned)n_rows;
+                f[i] = w && j + i < top_k ? w[j + i] : 1.f;
+                load_units<U>(rows + (size_t)(there[i] ? r : 0) * H + u * U, v[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (there[i])
+#pragma unroll
+                    for (int e = 0; e < U; e++) acc[e] = fmaf(f[i], v[i][e], acc[e]);
         }
         if (extra) {
             float v[U];
-            load_units<U>(extra + (size_t)t * H + h, v);
+            load_units<U>(extra + (size_t)t * H + u * U, v);
 #pragma unroll
-            for (int i = 0; i < U; i++) acc[i] += v[i];
+            for (int e = 0; e < U; e++) acc[e] += v[e];
         }
-        store_units<U>(out + (size_t)t * H + h, acc);
+        store_units<U>(out + (size_t)t * H + u * U, acc);
     }
+}
+
+// Elements of a unit: 16 bytes of the widest type among those given, fewer where H or an address does not allow it.
+static int unit_elements(int H, bool any_f32, std::initializer_list<std::pair<const void *, int>> tensors)
+{
+    for (int u = any_f32 ? 4 : 8; u > 1; u /= 2) {
+        bool fits = H % u == 0;
+        for (auto &t : tensors) fits = fits && (uintptr_t)t.first % min(16, u * (t.second == PMOE_F32 ? 4 : 2)) == 0;
+        if (fits) return u;
+    }
+    return 1;
+}
+
+// f(Units<u>) for a unit of u elements; eight only where all types are bf16
+template <int U_> struct Units { static constexpr int U = U_; };
+template <bool EIGHT, typename F> static auto with_units(int u, F &&f)
+{
+    if constexpr (EIGHT)
+        if (u == 8) return f(Units<8>{});
+    return u == 4 ? f(Units<4>{}) : u == 2 ? f(Units<2>{}) : f(Units<1>{});
 }
 
 cudaError_t launch_combine_rows(const void *rows, int rows_dtype, int n_rows, int n, int top_k, int H, const int *place, const float *w,
                                 const void *extra, int extra_dtype, void *out, int out_dtype, cudaStream_t s)
 {
     count_launch();
-    const bool wide = H % 8 == 0 && aligned16(rows) && aligned16(extra) && aligned16(out);
+    const int u = unit_elements(H, rows_dtype == PMOE_F32 || extra_dtype == PMOE_F32 || out_dtype == PMOE_F32,
+                                {{rows, rows_dtype}, {extra, extra_dtype}, {out, out_dtype}});
+    const RowThreads rt = RowThreads::of(H / u, n);
     return with_type(rows_dtype, [&](auto *rp) {
         return with_type(extra_dtype, [&](auto *ep) {
             return with_type(out_dtype, [&](auto *op) {
                 using RT = std::remove_pointer_t<decltype(rp)>;
                 using ET = std::remove_pointer_t<decltype(ep)>;
                 using OT = std::remove_pointer_t<decltype(op)>;
-                return launch_pdl(wide ? k_combine_rows<8, RT, ET, OT> : k_combine_rows<1, RT, ET, OT>, dim3(n), dim3(256), 0, s,
-                                  (const RT *)rows, H, top_k, n_rows, place, w, (const ET *)extra, (OT *)out);
+                return with_units<sizeof(RT) + sizeof(ET) + sizeof(OT) == 6>(u, [&](auto units) {
+                    return launch_pdl(k_combine_rows<decltype(units)::U, RT, ET, OT>, dim3(rt.grid), dim3(256), 0, s, (const RT *)rows, H, n,
+                                      top_k, n_rows, place, w, (const ET *)extra, (OT *)out, rt);
+                });
             });
         });
     });
 }
 
-// ---------------------------------------------------------------- gradient of combine
-// grad_rows[place_p] = w_p grad_out[t],  grad_w_p = <grad_out[t], rows[place_p]> for pair p = (t, j): one warp per pair.
+// Gradient of combine: grad_rows[place_p] = w_p grad_out[t],  grad_w_p = <grad_out[t], rows[place_p]> for pair p = (t, j): one
+// warp per pair, whose token's row comes from the cache for all slots but one.
 template <int U, typename GT, typename RT>
 __global__ void __launch_bounds__(256) k_combine_grad(const GT *__restrict__ grad_out, const RT *__restrict__ rows, int H, int top_k, int P,
                                                       const int *__restrict__ place, const int *__restrict__ offsets, int E,
@@ -292,18 +385,21 @@ __global__ void __launch_bounds__(256) k_combine_grad(const GT *__restrict__ gra
     if (kept) {
         const float wt = w ? w[p] : 1.f;
         const GT *g = grad_out + (size_t)(p / top_k) * H;
+        const RT *r = rows + (size_t)at * H;
+        RT *gr = grad_rows + (size_t)at * H;
+#pragma unroll 4
         for (int h = lane * U; h < H; h += 32 * U) {
             float a[U], b[U];
             load_units<U>(g + h, a);
             if (grad_w) {
-                load_units<U>(rows + (size_t)at * H + h, b);
+                load_units<U>(r + h, b);
 #pragma unroll
                 for (int i = 0; i < U; i++) dot = fmaf(a[i], b[i], dot);
             }
             if (grad_rows) {
 #pragma unroll
                 for (int i = 0; i < U; i++) a[i] *= wt;
-                store_units<U>(grad_rows + (size_t)at * H + h, a);
+                store_units<U>(gr + h, a);
             }
         }
     }
@@ -325,13 +421,15 @@ cudaError_t launch_combine_grad(const void *grad_out, int grad_dtype, const void
 {
     count_launch();
     const int P = n * top_k;
-    const bool wide = H % 8 == 0 && aligned16(rows) && aligned16(grad_out) && aligned16(grad_rows);
+    const int u = unit_elements(H, grad_dtype == PMOE_F32 || rows_dtype == PMOE_F32, {{grad_out, grad_dtype}, {rows, rows_dtype}, {grad_rows, rows_dtype}});
     return with_type(grad_dtype, [&](auto *gp) {
         return with_type(rows_dtype, [&](auto *rp) {
             using GT = std::remove_pointer_t<decltype(gp)>;
             using RT = std::remove_pointer_t<decltype(rp)>;
-            return launch_pdl(wide ? k_combine_grad<8, GT, RT> : k_combine_grad<1, GT, RT>, dim3((P + 7) / 8), dim3(256), 0, s,
-                              (const GT *)grad_out, (const RT *)rows, H, top_k, P, place, offsets, E, w, (RT *)grad_rows, grad_w);
+            return with_units<sizeof(GT) + sizeof(RT) == 4>(u, [&](auto units) {
+                return launch_pdl(k_combine_grad<decltype(units)::U, GT, RT>, dim3((P + 7) / 8), dim3(256), 0, s, (const GT *)grad_out,
+                                  (const RT *)rows, H, top_k, P, place, offsets, E, w, (RT *)grad_rows, grad_w);
+            });
         });
     });
 }
