@@ -22,11 +22,20 @@ from typing import Optional, Tuple
 import torch
 
 from ._lib import BF16, F32, F8_E4M3, I8, PmoeError, check, lib
-from .moe import _check_buffer, _stream_ptr
+from .moe import _check_buffer
 
 _TYPES = {torch.float32: F32, torch.bfloat16: BF16}
 _Q_TYPES = {torch.int8: I8, torch.float8_e4m3fn: F8_E4M3}
 _MAX_EXPERTS = 4096
+
+
+# The current stream's handle by device index: what torch.cuda.current_stream(device).cuda_stream gives, without making the
+# stream object (2 us a call, as long as a small operator's launch).
+_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _f32(t: torch.Tensor) -> torch.Tensor:
+    return t.contiguous() if t.dtype == torch.float32 else t.to(torch.float32).contiguous()
 
 
 def _on_gpu(what: str, t: torch.Tensor) -> torch.device:
@@ -81,17 +90,15 @@ class ExpertOrder:
 
     @property
     def order(self) -> torch.Tensor:
-        return self._data[:self.n * self.top_k]
+        return self._data.as_strided((self.n * self.top_k,), (1,))
 
     @property
     def place(self) -> torch.Tensor:
-        pairs = self.n * self.top_k
-        step = (pairs + 3) // 4 * 4
-        return self._data[step:step + pairs].view(self.n, self.top_k)
+        return self._data.as_strided((self.n, self.top_k), (self.top_k, 1), (self.n * self.top_k + 3) // 4 * 4)
 
     @property
     def offsets(self) -> torch.Tensor:
-        return self._data[self._data.numel() - self.num_experts - 1:]
+        return self._data.as_strided((self.num_experts + 1,), (1,), (self.n * self.top_k + 3) // 4 * 8)
 
 
 def sort_by_expert(indices: torch.Tensor, num_experts: int, expert_base: int = 0) -> ExpertOrder:
@@ -111,7 +118,7 @@ def sort_by_expert(indices: torch.Tensor, num_experts: int, expert_base: int = 0
     idx = _ids("indices", indices)
     o = ExpertOrder(n, top_k, int(num_experts), device)
     check(lib().pmoe_sort_pairs(device.index, idx.data_ptr(), n, top_k, int(expert_base), o.num_experts, o._order, o._place, o._offsets,
-                                _stream_ptr(device)))
+                                _stream(device.index)))
     return o
 
 
@@ -132,20 +139,20 @@ def dispatch_rows(x: torch.Tensor, order: ExpertOrder, out: Optional[torch.Tenso
     x = x.contiguous()
     rows = (order.n * order.top_k, x.shape[1])
     if out is None:
-        out = torch.empty(rows, dtype=x.dtype, device=device)
+        out = torch.empty(*rows, dtype=x.dtype, device=device)
     else:
         _check_buffer("out", out, rows, x.dtype, device)
     if x.shape[1] == 0:
         return out
     check(lib().pmoe_dispatch_rows(device.index, x.data_ptr(), x.shape[1] * x.element_size(), order.n, order.top_k, order._place,
-                                   order._offsets, order.num_experts, out.data_ptr(), _stream_ptr(device)))
+                                   order._offsets, order.num_experts, out.data_ptr(), _stream(device.index)))
     return out
 
 
 def _pair_weights(weights: torch.Tensor, order: ExpertOrder, device) -> torch.Tensor:
     if not isinstance(weights, torch.Tensor) or weights.device != device or weights.numel() != order.n * order.top_k:
         raise ValueError(f"weights must be [{order.n}, {order.top_k}] on {device}")
-    return weights.to(torch.float32).contiguous()
+    return _f32(weights)
 
 
 def _pair_rows(what: str, rows: torch.Tensor, order: ExpertOrder) -> torch.Tensor:
@@ -173,14 +180,14 @@ def combine_rows(rows: torch.Tensor, order: ExpertOrder, weights: Optional[torch
             raise ValueError(f"extra must be {shape}, got {tuple(extra.shape)}")
         e = extra.contiguous()
     if out is None:
-        out = torch.empty(shape, dtype=out_dtype or rows.dtype, device=device)
+        out = torch.empty(*shape, dtype=out_dtype or rows.dtype, device=device)
         od = _out_type("out_dtype", out.dtype)
     else:
         _check_buffer("out", out, shape, tuple(_TYPES), device)
         od = _TYPES[out.dtype]
     check(lib().pmoe_combine_rows(device.index, rows.data_ptr(), rd, rows.shape[0], order.n, order.top_k, rows.shape[1], order._place,
                                   None if w is None else w.data_ptr(), None if e is None else e.data_ptr(),
-                                  0 if e is None else _TYPES[e.dtype], out.data_ptr(), od, _stream_ptr(device)))
+                                  0 if e is None else _TYPES[e.dtype], out.data_ptr(), od, _stream(device.index)))
     return out
 
 
@@ -203,10 +210,10 @@ def combine_rows_grad(grad_out: torch.Tensor, rows: torch.Tensor, order: ExpertO
     g = grad_out.contiguous()
     w = None if weights is None else _pair_weights(weights, order, device)
     grad_rows = torch.empty_like(rows)
-    grad_w = torch.empty((order.n, order.top_k), dtype=torch.float32, device=device)
+    grad_w = torch.empty(order.n, order.top_k, dtype=torch.float32, device=device)
     check(lib().pmoe_combine_rows_grad(device.index, g.data_ptr(), gd, rows.data_ptr(), rd, order.n, order.top_k, rows.shape[1],
                                        order._place, order._offsets, order.num_experts, None if w is None else w.data_ptr(),
-                                       grad_rows.data_ptr(), grad_w.data_ptr(), _stream_ptr(device)))
+                                       grad_rows.data_ptr(), grad_w.data_ptr(), _stream(device.index)))
     return grad_rows, grad_w
 
 
@@ -235,7 +242,7 @@ def add_rms_norm_q8(resid: torch.Tensor, delta: Optional[torch.Tensor], weight: 
     if weight is not None:
         if not isinstance(weight, torch.Tensor) or weight.device != device or tuple(weight.shape) != (H,):
             raise ValueError(f"weight must be [{H}] on {device}")
-        w = weight.to(torch.float32).contiguous()
+        w = _f32(weight)
     if q_dtype not in _Q_TYPES:
         raise PmoeError(-2, f"q_dtype must be int8 or float8_e4m3fn, got {q_dtype}")
     if group not in (0, 32, 64, 128, 256):
@@ -244,13 +251,13 @@ def add_rms_norm_q8(resid: torch.Tensor, delta: Optional[torch.Tensor], weight: 
         raise ValueError("resid must have columns")
     vd = 0 if values_dtype is None else _out_type("values_dtype", values_dtype)
     new_resid = torch.empty_like(r)
-    q = torch.empty((n, H), dtype=q_dtype, device=device)
-    scales = torch.empty((n, (H + group - 1) // group if group else 1), dtype=torch.float32, device=device)
-    values = None if values_dtype is None else torch.empty((n, H), dtype=values_dtype, device=device)
+    q = torch.empty_like(r, dtype=q_dtype)
+    scales = torch.empty(n, (H + group - 1) // group if group else 1, dtype=torch.float32, device=device)
+    values = None if values_dtype is None else torch.empty_like(r, dtype=values_dtype)
     check(lib().pmoe_add_rms_norm_q8(device.index, r.data_ptr(), rd, None if d is None else d.data_ptr(), dd or 0,
                                      None if w is None else w.data_ptr(), n, H, float(eps), group, new_resid.data_ptr(), _Q_TYPES[q_dtype],
                                      q.data_ptr(), scales.data_ptr(), None if values is None else values.data_ptr(), vd,
-                                     _stream_ptr(device)))
+                                     _stream(device.index)))
     return new_resid, q, scales, values
 
 
@@ -290,7 +297,7 @@ def adapters_add(base: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.
     if scales is not None:
         if not isinstance(scales, torch.Tensor) or scales.device != device or scales.numel() != L:
             raise ValueError(f"scales must be [{L}] on {device}")
-        s = scales.to(torch.float32).contiguous()
+        s = _f32(scales)
     x, a, b, ids = _aligned(x), _aligned(a), _aligned(b), _ids("ids", ids.reshape(-1))
     if order is not None:
         _ordered(order, device)
@@ -300,7 +307,7 @@ def adapters_add(base: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.
         order = sort_by_expert(ids, L)
     if out is None:
         base = _aligned(base)
-        out = torch.empty((n, N), dtype=base.dtype, device=device)
+        out = torch.empty_like(base)
     else:
         _check_buffer("out", out, (n, N), base.dtype, device)
         if out.data_ptr() % 16:
@@ -308,7 +315,7 @@ def adapters_add(base: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.
         base = _aligned(base)
     check(lib().pmoe_adapters_add(device.index, base.data_ptr(), x.data_ptr(), xd, n, K, N, r, L, a.data_ptr(), b.data_ptr(),
                                   None if s is None else s.data_ptr(), ids.data_ptr(), None if order is None else order._order,
-                                  None if order is None else order._offsets, out.data_ptr(), od, _stream_ptr(device)))
+                                  None if order is None else order._offsets, out.data_ptr(), od, _stream(device.index)))
     return out
 
 
