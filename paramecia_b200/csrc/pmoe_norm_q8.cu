@@ -23,26 +23,32 @@ __device__ inline float max_abs(float m, float v)
     return r;
 }
 
-// How a group becomes 8 bits: scale = top / 127 or / 448, q = round(v / scale).  The quotient is a product with 1 / scale, one
-// rounding away from it; only a scale so small that 1 / scale would overflow is divided by.
+// How a group becomes 8 bits.  With u = r * weight and top = max |u| over the group, v = u / m and
+//   scale = max |v| / 127 = top * (1 / m) / 127,   v / scale = u * (127 / top):
+// the quotient needs neither m nor the rounded scale, which saves two products an element, lets both statistics be
+// reduced at once, and takes three roundings where dividing v by its scale takes five (each moves values over a border
+// of the 8-bit numbers).
 struct GroupScale {
-    float scale, inverse;
+    float scale, inverse, top;
     bool plain;    // the product with `inverse` is the quotient, and in the type's range up to what the rounding takes back
-    template <bool E4M3> __device__ static GroupScale of(float top)
+    template <bool E4M3> __device__ static GroupScale of(float top, float inv_m)
     {
         GroupScale g;
-        g.scale = top * (E4M3 ? 1.f / 448.f : 1.f / 127.f);
-        g.plain = g.scale >= 0x1p-100f && g.scale < INFINITY;
-        g.inverse = __frcp_rn(g.scale);
+        g.scale = __fdiv_rn(top * inv_m, E4M3 ? 448.f : 127.f);
+        g.top = top;
+        g.plain = top >= 0x1p-100f && g.scale > 0.f && g.scale < INFINITY;
+        g.inverse = __fdiv_rn(E4M3 ? 448.f : 127.f, top);
         return g;
     }
-    // v / scale for the other groups: 0 where the scale is 0, infinite or NaN
-    template <bool E4M3> __device__ float ratio(float v) const
+    // v / scale for the other groups: 0 where the scale is 0, infinite or NaN, else without the inverse, which may overflow
+    template <bool E4M3> __device__ float ratio(float u) const
     {
-        const float most = E4M3 ? 448.f : 127.f;
-        return scale > 0.f && scale < INFINITY ? fminf(fmaxf(__fdiv_rn(v, scale), -most), most) : 0.f;
+        return scale > 0.f && scale < INFINITY ? __fdiv_rn(u, top) * (E4M3 ? 448.f : 127.f) : 0.f;
     }
 };
+
+// 1 / sqrt(mean + eps); of 0 it is infinite and of an infinity 0, so that u * inv_m is u / m there too
+__device__ inline float inverse_rms(float ss, int H, float eps) { return __frcp_rn(sqrtf(ss / (float)H + eps)); }
 
 // Ratios to 8 bits (the bytes of `packed`, in order) and, with HELD, back to what they stand for in units of the scale.
 template <bool E4M3, bool HELD, int N> __device__ inline void to_8bit(float (&r)[N], uint32_t *packed)
@@ -99,8 +105,8 @@ __device__ inline void add_and_store(float (&v)[8], const float (&d)[8], __nv_bf
 // bf16 + bf16 -> bf16, e4m3), so memory bounds it and the row must stay on the chip between its two statistics: here in
 // registers, eight consecutive elements a thread and pass, a row never longer than threads * PASSES * 8.  A group is 4, 8, 16
 // or 32 neighbouring threads of a pass (its maximum by shuffles) or the whole row (shuffles and a shared array).  The second
-// limit is the issue rate, near once the two quotients an element are products: the work a thread does once for its elements
-// (root, reciprocals, sums over the row) is shared by sixteen of them where there are rows enough to fill the card.
+// limit is the issue rate: with two quotients an element 16384 rows of 2048 took 126 us.  Now 46 us, 0.79 of the
+// measured copy rate (sixteen elements a thread and half the threads: 50 us).
 template <typename RT, typename DT, typename VT, bool E4M3, int PASSES>
 __global__ void __launch_bounds__(1024) k_norm_q8(const RT *resid_in, const DT *__restrict__ delta, const float *__restrict__ weight, int H,
                                                   float eps, int group, RT *resid_out, uint8_t *__restrict__ q,
@@ -136,65 +142,53 @@ __global__ void __launch_bounds__(1024) k_norm_q8(const RT *resid_in, const DT *
             if (resid_out) store_units<8>(resid_out + base + h, v[p]);
         }
     }
-#pragma unroll
-    for (int p = 0; p < PASSES; p++)
-        if ((p * blockDim.x + tid) * 8 < H)
-#pragma unroll
-            for (int i = 0; i < 8; i++) ss = fmaf(v[p][i], v[p][i], ss);
-#pragma unroll
-    for (int s = 16; s >= 1; s >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, s);
-    if (lane == 0) red[warp] = ss;
-    __syncthreads();
-    ss = lane < warps ? red[lane] : 0.f;
-#pragma unroll
-    for (int s = 16; s >= 1; s >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, s);
-    const float inv_m = __frcp_rn(sqrtf(ss / (float)H + eps));   // 1 / inf = 0, 1 / 0 = inf: the products are the quotients in both
-
-    float top[PASSES];
+    float top[PASSES], row_top = 0.f;
 #pragma unroll
     for (int p = 0; p < PASSES; p++) {
         const int h = (p * blockDim.x + tid) * 8;
         top[p] = 0.f;
         if (h >= H) continue;
+#pragma unroll
+        for (int i = 0; i < 8; i++) ss = fmaf(v[p][i], v[p][i], ss);
         if (weight) {
             float w[8];
             load_units<8>(weight + h, w);
 #pragma unroll
-            for (int i = 0; i < 8; i++) v[p][i] = v[p][i] * inv_m * w[i];
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; i++) v[p][i] *= inv_m;
+            for (int i = 0; i < 8; i++) v[p][i] *= w[i];
         }
 #pragma unroll
         for (int i = 0; i < 8; i++) top[p] = max_abs(top[p], v[p][i]);
+        if (group >= H) row_top = max_abs(row_top, top[p]);
     }
     const int log2_group = 31 - __clz(group), G = group >= H ? 1 : (H + group - 1) >> log2_group;   // more than one group: a power of two
     float *row_scales = scales + (size_t)blockIdx.x * G;
-    if (G > 1) {   // 32 to 256 values: up to a warp's
+#pragma unroll
+    for (int s = 16; s >= 1; s >>= 1) {
+        ss += __shfl_xor_sync(0xffffffffu, ss, s);
+        if (G == 1) row_top = max_abs(row_top, __shfl_xor_sync(0xffffffffu, row_top, s));
+    }
+    if (lane == 0) { red[warp] = ss; red_max[warp] = row_top; }
+    if (G > 1) {   // groups of 32 to 256 values: up to a warp's
 #pragma unroll
         for (int p = 0; p < PASSES; p++)
 #pragma unroll
             for (int s = 1; s < 32; s <<= 1)
                 if (s * 8 < group) top[p] = max_abs(top[p], __shfl_xor_sync(0xffffffffu, top[p], s));
-    } else {       // one scale for the row
-        float t = top[0];
-#pragma unroll
-        for (int p = 1; p < PASSES; p++) t = max_abs(t, top[p]);
-#pragma unroll
-        for (int s = 16; s >= 1; s >>= 1) t = max_abs(t, __shfl_xor_sync(0xffffffffu, t, s));
-        if (lane == 0) red_max[warp] = t;
-        __syncthreads();
-        t = lane < warps ? red_max[lane] : 0.f;
-#pragma unroll
-        for (int s = 16; s >= 1; s >>= 1) t = max_abs(t, __shfl_xor_sync(0xffffffffu, t, s));
-#pragma unroll
-        for (int p = 0; p < PASSES; p++) top[p] = t;
     }
+    __syncthreads();
+    ss = lane < warps ? red[lane] : 0.f;
+    row_top = lane < warps ? red_max[lane] : 0.f;
+#pragma unroll
+    for (int s = 16; s >= 1; s >>= 1) {
+        ss += __shfl_xor_sync(0xffffffffu, ss, s);
+        if (G == 1) row_top = max_abs(row_top, __shfl_xor_sync(0xffffffffu, row_top, s));
+    }
+    const float inv_m = inverse_rms(ss, H, eps);
 #pragma unroll
     for (int p = 0; p < PASSES; p++) {
         const int h = (p * blockDim.x + tid) * 8;
         if (h >= H) continue;
-        const GroupScale gs = GroupScale::of<E4M3>(top[p]);
+        const GroupScale gs = GroupScale::of<E4M3>(G == 1 ? row_top : top[p], inv_m);
         if (G == 1 ? h == 0 : (h & (group - 1)) == 0) row_scales[G == 1 ? 0 : h >> log2_group] = gs.scale;
         if (gs.plain) {
 #pragma unroll
@@ -236,17 +230,18 @@ __global__ void __launch_bounds__(1024) k_norm_q8_any(const RT *resid_in, const 
     q += base;
     if (values) values += base;
     float v[PASSES][8];
-    float ss = 0.f;
+    float ss = 0.f, row_top = 0.f;
 #pragma unroll
     for (int p = 0; p < PASSES; p++) {
         const int h0 = (p * warps + warp) * 256 + lane;
         if (h0 - lane >= H) break;
-        float d[8] = {};
+        float d[8] = {}, w[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             const int h = h0 + i * 32;
             v[p][i] = h < H ? load_as_float(resid_in, h) : 0.f;
             if (delta && h < H) d[i] = load_as_float(delta, h);
+            w[i] = weight && h < H ? weight[h] : 1.f;
         }
 #pragma unroll
         for (int i = 0; i < 8; i++) {
@@ -256,39 +251,27 @@ __global__ void __launch_bounds__(1024) k_norm_q8_any(const RT *resid_in, const 
             v[p][i] = load_as_float(&r, 0);
             if (resid_out && h < H) resid_out[h] = r;
             ss = fmaf(v[p][i], v[p][i], ss);
+            v[p][i] *= w[i];
+            if (group >= H) row_top = max_abs(row_top, v[p][i]);
         }
     }
-#pragma unroll
-    for (int s = 16; s >= 1; s >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, s);
-    if (lane == 0) red[warp] = ss;
-    __syncthreads();
-    ss = lane < warps ? red[lane] : 0.f;
-#pragma unroll
-    for (int s = 16; s >= 1; s >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, s);
-    const float inv_m = __frcp_rn(sqrtf(ss / (float)H + eps));
     const int log2_group = 31 - __clz(group), G = group >= H ? 1 : (H + group - 1) >> log2_group;   // more than one group: a power of two
     float *row_scales = scales + (size_t)blockIdx.x * G;
-    float row_top = 0.f;
 #pragma unroll
-    for (int p = 0; p < PASSES; p++) {
-        const int h0 = (p * warps + warp) * 256 + lane;
-        if (h0 - lane >= H) break;
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const int h = h0 + i * 32;
-            v[p][i] = h < H ? v[p][i] * inv_m * (weight ? weight[h] : 1.f) : 0.f;
-            row_top = max_abs(row_top, v[p][i]);
-        }
+    for (int s = 16; s >= 1; s >>= 1) {
+        ss += __shfl_xor_sync(0xffffffffu, ss, s);
+        if (G == 1) row_top = max_abs(row_top, __shfl_xor_sync(0xffffffffu, row_top, s));
     }
-    if (G == 1) {
+    if (lane == 0) { red[warp] = ss; red_max[warp] = row_top; }
+    __syncthreads();
+    ss = lane < warps ? red[lane] : 0.f;
+    row_top = lane < warps ? red_max[lane] : 0.f;
 #pragma unroll
-        for (int s = 16; s >= 1; s >>= 1) row_top = max_abs(row_top, __shfl_xor_sync(0xffffffffu, row_top, s));
-        if (lane == 0) red_max[warp] = row_top;
-        __syncthreads();
-        row_top = lane < warps ? red_max[lane] : 0.f;
-#pragma unroll
-        for (int s = 16; s >= 1; s >>= 1) row_top = max_abs(row_top, __shfl_xor_sync(0xffffffffu, row_top, s));
+    for (int s = 16; s >= 1; s >>= 1) {
+        ss += __shfl_xor_sync(0xffffffffu, ss, s);
+        if (G == 1) row_top = max_abs(row_top, __shfl_xor_sync(0xffffffffu, row_top, s));
     }
+    const float inv_m = inverse_rms(ss, H, eps);
 #pragma unroll
     for (int p = 0; p < PASSES; p++) {
         const int h0 = (p * warps + warp) * 256 + lane;
@@ -302,7 +285,7 @@ __global__ void __launch_bounds__(1024) k_norm_q8_any(const RT *resid_in, const 
                 if (s * 32 < group)
 #pragma unroll
                     for (int i = 0; i < 8; i += 2 * s) top[i] = max_abs(top[i], top[i + s]);
-        GroupScale gs = GroupScale::of<E4M3>(row_top);
+        GroupScale gs = GroupScale::of<E4M3>(row_top, inv_m);
         if (G == 1 && h0 == 0) row_scales[0] = gs.scale;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
@@ -310,7 +293,7 @@ __global__ void __launch_bounds__(1024) k_norm_q8_any(const RT *resid_in, const 
             if (G > 1 && (i * 32 & (group - 1)) == 0) {   // a group begins
 #pragma unroll
                 for (int s = 16; s >= 1; s >>= 1) top[i] = max_abs(top[i], __shfl_xor_sync(0xffffffffu, top[i], s));
-                gs = GroupScale::of<E4M3>(top[i]);
+                gs = GroupScale::of<E4M3>(top[i], inv_m);
                 if (lane == 0 && h < H) row_scales[h >> log2_group] = gs.scale;
             }
             if (h >= H) continue;
@@ -330,9 +313,7 @@ cudaError_t launch_norm_q8(const void *resid_in, int resid_dtype, const void *de
     count_launch();
     const bool wide = H % 8 == 0 && aligned16(resid_in) && aligned16(delta) && aligned16(weight) && aligned16(resid_out) &&
                       aligned16(values) && ((uintptr_t)q & 7) == 0;
-    // One pass keeps a row's chain short, two do less work an element (16384 rows of 2048: 49 against 58 us): two where the
-    // rows alone make several CTAs an SM, and where a row is longer than 1024 threads take in one.
-    const int passes = H > 8192 || (H > 512 && n >= 1024) ? 2 : 1;
+    const int passes = H > 8192 ? 2 : 1;   // 1024 threads take 8192 elements at once
     const int threads = min(1024, ((H + 8 * passes - 1) / (8 * passes) + 31) / 32 * 32);
     return with_type(resid_dtype, [&](auto *rp) {
         return with_type(delta_dtype, [&](auto *dp) {
