@@ -553,11 +553,10 @@ static cudaError_t launch_adapters_as(const AdapterArgs &P, const XT *x, const O
     int ctas = AD_MAX_CTAS;
     double best = 1e30;
     for (int c = AD_MAX_CTAS; c >= 1; c /= 2) {
-        const int64_t tiles = P.order ? (P.n + T - 1) / T + min(P.L, (P.n + T - 1) / T) / 2 : min(P.n, P.L);
-        const double cost = (double)((tiles * c + room - 1) / room) * (8.0 + (P.K + P.N) / 128.0 / c);
+        const int64_t tiles = P.order ? min(P.n, (P.n + T - 1) / T + min(P.L, P.n) / 2) : min(P.n, P.L);
+        const double cost = max(1.0, (double)(tiles * c) / room) * (8.0 + (P.K + P.N) / 128.0 / c);
         if (cost < best) { best = cost; ctas = c; }
     }
-    if (getenv("AD_C")) ctas = atoi(getenv("AD_C"));
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)slots * ctas);
     cfg.blockDim = dim3(S::THREADS);
@@ -578,7 +577,7 @@ static cudaError_t launch_adapters_as(const AdapterArgs &P, const XT *x, const O
 cudaError_t launch_adapters(const void *base, int out_dtype, const void *x, int x_dtype, const AdapterArgs &P, void *out, cudaStream_t s)
 {
     // tiles of 64 rows where an adapter has that many on average; else of 16
-    const bool wide = P.order && P.n / P.L >= 48 && !getenv("AD_16");
+    const bool wide = P.order && P.n / P.L >= 48;
     return with_type(x_dtype, [&](auto *xp) {
         return with_type(out_dtype, [&](auto *op) {
             using XT = std::remove_pointer_t<decltype(xp)>;
