@@ -366,6 +366,11 @@ int pmoe_adapters_add(int device, const void *base, const void *x, int x_dtype, 
                       const void *a, const void *b, const float *scales, const int *ids, const int *order, const int *offsets, void *out,
                       int out_dtype, void *stream);
 
+/* Synchronises the stream and reports the device-side status word of pmoe_adapters_add (PMOE_OK, or PMOE_ERR_TIMEOUT when a
+ * bounded wait inside a kernel ran out and its output is not to be used), clearing it: pmoe_layer_status for the operators
+ * that have no handle. */
+int pmoe_rows_status(int device, void *stream);
+
 /*
  * Home-rank side of the expert-parallel combine: out[t] = sum_r parts[r][t] (+ extra[t]).
  * parts [n_parts, n, H] f32 are the per-rank partial sums a token's expert owners returned,

@@ -80,6 +80,7 @@ SYMBOLS = [
     ("pmoe_combine_rows", _I, [_I, _V, _I, _I, _I, _I, _I, _V, _V, _V, _I, _V, _I, _V]),
     ("pmoe_combine_rows_grad", _I, [_I, _V, _I, _V, _I, _I, _I, _I, _V, _V, _I, _V, _V, _V, _V]),
     ("pmoe_adapters_add", _I, [_I, _V, _V, _I, _I, _I, _I, _I, _I, _V, _V, _V, _V, _V, _V, _V, _I, _V]),
+    ("pmoe_rows_status", _I, [_I, _V]),
     ("pmoe_layer_status", _I, [_V, _V]),
     ("pmoe_layer_trace", _I, [_V, _I]),
     ("pmoe_layer_trace_read", _I, [_V, _V]),

@@ -14,6 +14,7 @@
 #include <cooperative_groups.h>
 
 #include "pmoe_internal.h"
+#include "pmoe_tcgen05.cuh"
 #include "pmoe_vec.cuh"
 
 namespace pmoe {
@@ -144,6 +145,28 @@ template <int THREADS, typename OT> __device__ inline void copy_bare_rows(const 
     }
 }
 
+// The tile of a slot, from the sorted ids: its adapter and rows (-1: none), the same for every CTA that asks for it.  Tile slots
+// of adapter e begin at offsets[e] / T + e: with one slot more than whole multiples of T inside its range that is never
+// fewer than it has tiles, and needs no scan over the adapters.
+template <int T, int THREADS>
+__device__ inline void find_tile(const AdapterArgs &P, int slot, int *rows, int &tile_id, int &tile_rows, int &tile_first)
+{
+    const int tid = threadIdx.x;
+    if (tid == 0) tile_rows = 0;
+    __syncthreads();
+    for (int e = tid; e < P.L; e += THREADS) {
+        const int from = P.offsets[e], to = min(P.offsets[e + 1], P.n), nth = slot - (from / T + e);
+        if (from >= 0 && nth >= 0 && nth < (to - from + T - 1) / T) {   // one adapter at most
+            tile_id = e;
+            tile_first = from + nth * T;
+            tile_rows = min(T, to - from - nth * T);
+        }
+    }
+    __syncthreads();
+    if (tid < T) rows[tid] = tid < tile_rows ? P.order[tile_first + tid] : -1;
+    __syncthreads();
+}
+
 // A CTA walks its share of K and then its share of N in stages of four chunks of 32: a stage holds what the matrix
 // instructions of those chunks need, as the lanes need it (sixteen bytes per lane, lanes side by side, so no
 // access meets a bank twice).  The copies are asynchronous and STAGES stages are on their way, the first ones of N
@@ -194,21 +217,7 @@ __global__ void __launch_bounds__(AdapterStage<XT, OT, T, RT>::THREADS, AdapterS
 
     // ---- the tile: its adapter and rows.  Every CTA of the cluster finds the same.
     if (P.order) {
-        // Tile slots of adapter e begin at offsets[e] / T + e: with one slot more than whole multiples of T inside its
-        // range that is never fewer than it has tiles, and needs no scan over the adapters.
-        if (tid == 0) tile_rows = 0;
-        __syncthreads();
-        for (int e = tid; e < P.L; e += THREADS) {
-            const int from = P.offsets[e], to = min(P.offsets[e + 1], P.n), nth = slot - (from / T + e);
-            if (from >= 0 && nth >= 0 && nth < (to - from + T - 1) / T) {   // one adapter at most
-                tile_id = e;
-                tile_first = from + nth * T;
-                tile_rows = min(T, to - from - nth * T);
-            }
-        }
-        __syncthreads();
-        if (tid < T) rows[tid] = tid < tile_rows ? P.order[tile_first + tid] : -1;
-        __syncthreads();
+        find_tile<T, THREADS>(P, slot, rows, tile_id, tile_rows, tile_first);
     } else if constexpr (T == 16) {
         // slot t leads a tile when the number of earlier rows with its id is a multiple of T
         const int id = P.ids[slot];
@@ -535,31 +544,315 @@ __global__ void __launch_bounds__(AdapterStage<XT, OT, T, RT>::THREADS, AdapterS
     if (T == 16) cluster.sync();   // no CTA leaves while another reads its shares
 }
 
-template <typename XT, typename OT, int T, int RT>
-static cudaError_t launch_adapters_as(const AdapterArgs &P, const XT *x, const OT *base, OT *out, cudaStream_t s)
+// ---------------------------------------------------------------- many rows of an adapter: tcgen05
+// For prompts the warp-level instructions become the limit: their operands pass through registers, once for every sixteen
+// rows, and at rank 64 the second product alone keeps them busy for longer than the rows' bytes take (8192 rows of 2048 bf16:
+// 42 us for this part).  Here a tile of 128 rows of one adapter is the M of tcgen05.mma, read from shared memory and summed in
+// tensor memory:
+//   h[128, r]     = X[128, K] A^T   stages of 64 of K: the rows' and A's pieces of 128 bytes, 128-byte swizzle
+//   out[128, 128] = H B^T + base    chunks of 128 columns, h as two bf16 pieces (16 bits of it; three for an
+//                                 f32 result, all of it), each its own product
+// with the cluster's exchange of h between them as above.  All threads copy (asynchronously, STAGES - 1 stages ahead), one
+// issues the products, and a chunk's sums are read, added to base and stored while the next chunk's product runs.  The
+// columns of B lie permuted in shared memory so that a lane reads eight consecutive ones of a row.
+constexpr int TC_M = 128, TC_THREADS = 256;
+constexpr int TC_MIN_ROWS = 96;   // rows an adapter has on average
+
+__device__ DevStatus g_rows_status;   // a wait that ran out (pmoe_rows_status)
+
+template <typename OT, int RT> struct TcTile {
+    static constexpr int R = RT * 8, KB = (R + 63) / 64;              // ranks, blocks of 64 of them
+    static constexpr int X_BYTES = TC_M * 128, A_BYTES = R * 128, B_BYTES = KB * 128 * 128;
+    static constexpr int STAGE = X_BYTES + A_BYTES > B_BYTES ? X_BYTES + A_BYTES : B_BYTES;
+    static constexpr int PS = R + 4;                                  // floats between two rows of this CTA's share of h
+    static constexpr int HP = sizeof(OT) == 4 ? 3 : 2;                // pieces of h
+    static constexpr int PART = TC_M * PS * 4, H_BYTES = HP * KB * TC_M * 128;
+    static constexpr bool OVERLAY = RT == 16;                         // the share lies over the stages, which wait for the exchange
+    static constexpr int ROOM = 218 * 1024 - H_BYTES - (OVERLAY ? 0 : PART);
+    static constexpr int STAGES = ROOM / STAGE > 6 ? 6 : ROOM / STAGE;
+    static constexpr int SMEM = 1024 + STAGES * STAGE + H_BYTES + (OVERLAY ? 0 : PART);
+    static_assert(STAGES >= 3 && (!OVERLAY || PART <= STAGES * STAGE), "room for the pipeline");
+};
+
+// The row of B's tile that holds a column of a chunk: in groups of 32, row 8 j + i is the column that k_adapters gives to column
+// i of its j-th product.
+template <typename OT> __device__ inline int row_of(int col)
 {
-    using S = AdapterStage<XT, OT, T, RT>;
-    const size_t smem = S::SMEM;
-    auto *kern = k_adapters<XT, OT, T, RT>;
+    const int c = col % 32;
+    return col / 32 * 32 + (sizeof(OT) == 2 ? c / 2 % 4 * 8 + c / 8 * 2 + c % 2 : (c / 16 * 2 + c / 2 % 2) * 8 + c / 4 % 4 * 2 + c % 2);
+}
+
+template <typename OT, int RT>
+__global__ void __launch_bounds__(TC_THREADS, 1) k_adapters_tc(AdapterArgs P, const __nv_bfloat16 *__restrict__ x, const OT *base, OT *out)
+{
+    using S = TcTile<OT, RT>;
+    extern __shared__ __align__(16) uint8_t smem_raw[];
+    __shared__ int rows[TC_M];
+    __shared__ int tile_id, tile_rows, tile_first;
+    __shared__ uint64_t bars[S::STAGES];
+    __shared__ uint32_t tmem_at;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int ctas = (int)cluster.num_blocks(), c = (int)cluster.block_rank(), slot = blockIdx.x / ctas;
+    uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);   // the swizzle counts from 1024-byte boundaries
+    uint8_t *hs = smem + S::STAGES * S::STAGE;                                      // [HP][KB][128 rows of 128 bytes]
+    float *part = reinterpret_cast<float *>(S::OVERLAY ? smem : hs + S::H_BYTES);   // [128][PS]
+    pdl_wait();
+    pdl_launch_dependents();
+    const int share_id = id_of_share(P, 0);
+    find_tile<TC_M, TC_THREADS>(P, slot, rows, tile_id, tile_rows, tile_first);
+    if (tile_rows == 0) {
+        copy_bare_rows<TC_THREADS>(P, share_id, base, out);
+        return;
+    }
+    const int id = tile_id;
+    if (tid == 0) {
+        for (int i = 0; i < S::STAGES; i++) mbar_init(&bars[i], 1);
+        fence_mbar_init();
+    }
+    if (warp == 0) tmem_alloc(&tmem_at, 256);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_at;
+    bool ok = true;
+    // the product of stage `use` (counted over both parts) is complete, and its buffer free
+    auto product_done = [&](int use) {
+        if (ok && !mbar_wait_spin(&bars[use % S::STAGES], (use / S::STAGES) & 1)) {
+            ok = false;
+            set_status(&g_rows_status, PMOE_ERR_TIMEOUT, 40, use);
+        }
+    };
+
+    // ---- what this CTA takes of K and of N
+    const int kc = (P.K + 63) / 64, nc = (P.N + 127) / 128;
+    const int k0 = (int)((int64_t)kc * c / ctas), kst = (int)((int64_t)kc * (c + 1) / ctas) - k0;
+    const int n0 = (int)((int64_t)nc * c / ctas), nst = (int)((int64_t)nc * (c + 1) / ctas) - n0;
+
+    // copies: eight lanes take the 128 bytes of a row; this thread's rows are tid / 8 + 32 i
+    const int chunk = tid & 7, row8 = tid >> 3;
+    const uint32_t to = smem_u32(smem) + row8 * 128 + ((chunk ^ (row8 & 7)) << 4);
+    const __nv_bfloat16 *xr[4];
+    int x_size[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int t = rows[row8 + 32 * i];
+        x_size[i] = (unsigned)t < (unsigned)P.n ? 16 : 0;
+        xr[i] = x + (x_size[i] ? (size_t)t * P.K : 0);
+    }
+    const __nv_bfloat16 *aw = P.a + ((size_t)id * P.r + row8) * P.K;
+    const __nv_bfloat16 *bw = P.b + (size_t)id * P.N * P.r;
+    auto fetch_k = [&](int st) {
+        if (st < kst) {
+            const uint32_t dst = to + (st % S::STAGES) * S::STAGE;
+            const int k = (k0 + st) * 64 + chunk * 8;
+            const bool in = k < P.K;
+            each<4>([&](auto i) { copy16<i * 32 * 128, 0>(dst, in ? xr[i] + k : x, in ? x_size[i] : 0); });
+            each<(S::R + 31) / 32>([&](auto i) {
+                const bool there = in && row8 + i * 32 < P.r;
+                if (S::R >= 32 || row8 < S::R) copy16<S::X_BYTES + i * 32 * 128, 0>(dst, there ? aw + (size_t)i * 32 * P.K + k : P.a, there ? 16 : 0);
+            });
+        }
+        copies_commit();
+    };
+    auto fetch_n = [&](int st) {
+        if (st < nst) {
+            const uint32_t dst = smem_u32(smem) + ((kst + st) % S::STAGES) * S::STAGE;
+            const int col0 = (n0 + st) * 128;
+#pragma unroll
+            for (int i = 0; i < RT / 2; i++) {
+                const int m = tid + i * TC_THREADS, col = m / RT, k8 = m % RT, n = row_of<OT>(col);
+                const bool there = col0 + col < P.N && k8 * 8 < P.r;
+                copy16<0, 0>(dst + k8 / 8 * 16384 + n * 128 + ((k8 % 8 ^ n % 8) << 4), there ? bw + (size_t)(col0 + col) * P.r + k8 * 8 : P.b, there ? 16 : 0);
+            }
+        }
+        copies_commit();
+    };
+
+    // ---- this CTA's share of h
+    constexpr uint32_t IDESC_H = make_idesc(1, 1, 1, S::R, TC_M), IDESC_OUT = make_idesc(1, 1, 1, 128, TC_M);   // bf16 x bf16 -> f32
+    for (int st = 0; st < S::STAGES - 1; st++) fetch_k(st);
+    for (int st = 0; st < kst; st++) {
+        copies_wait<S::STAGES - 2>();
+        fence_proxy_async();
+        __syncthreads();
+        if (tid == 0) {
+            tc_fence_after();
+            const uint8_t *buffer = smem + (st % S::STAGES) * S::STAGE;
+            const uint64_t da = smem_desc_sw128(buffer), db = smem_desc_sw128(buffer + S::X_BYTES);
+#pragma unroll
+            for (int ks = 0; ks < 4; ks++) mma_f16(tmem, da + ks * 2, db + ks * 2, IDESC_H, st > 0 || ks > 0);
+            tc_commit(&bars[st % S::STAGES]);
+        }
+        if (st > 0) product_done(st - 1);
+        fetch_k(st + S::STAGES - 1);
+    }
+    if (kst > 0) product_done(kst - 1);
+    tc_fence_after();
+    if (!S::OVERLAY)
+        for (int st = 0; st < S::STAGES - 1; st++) fetch_n(st);
+    else
+        __syncthreads();
+
+    // ---- the shares of the cluster added, in CTA order, times the adapter's scale, and given to all as bf16 pieces
+    for (int i = warp / 4; i < S::R / 16; i += 2) {
+        uint32_t v[16];
+        if (kst > 0) {
+            tmem_ld16(tmem + ((uint32_t)(warp % 4 * 32) << 16) + i * 16, v);
+            tmem_ld_wait();
+        }
+        float4 *p = reinterpret_cast<float4 *>(part + (warp % 4 * 32 + lane) * S::PS + i * 16);
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            p[e] = kst > 0 ? make_float4(__uint_as_float(v[4 * e]), __uint_as_float(v[4 * e + 1]), __uint_as_float(v[4 * e + 2]), __uint_as_float(v[4 * e + 3]))
+                           : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    tc_fence_before();
+    cluster.sync();
+    const float scale = P.scales ? P.scales[id] : 1.f;
+    for (int i = c * TC_THREADS + tid; i < TC_M * RT; i += ctas * TC_THREADS) {   // eight ranks of a row
+        const int row = i / RT, k8 = i % RT;
+        float s[8] = {};
+#pragma unroll
+        for (int o = 0; o < AD_MAX_CTAS; o++) {
+            if (o >= ctas) break;
+            const float4 *p = reinterpret_cast<const float4 *>(cluster.map_shared_rank(part + row * S::PS + k8 * 8, o));
+            const float4 u = p[0], v = p[1];
+            s[0] += u.x; s[1] += u.y; s[2] += u.z; s[3] += u.w;
+            s[4] += v.x; s[5] += v.y; s[6] += v.z; s[7] += v.w;
+        }
+        uint32_t w[4][S::HP];
+#pragma unroll
+        for (int e = 0; e < 4; e++) split_pair<S::HP>(s[2 * e] * scale, s[2 * e + 1] * scale, w[e]);
+        uint8_t *at = hs + k8 / 8 * (TC_M * 128) + row * 128 + ((k8 % 8 ^ row % 8) << 4);
+#pragma unroll
+        for (int o = 0; o < AD_MAX_CTAS; o++) {
+            if (o >= ctas) break;
+            uint8_t *there = cluster.map_shared_rank(at, o);
+#pragma unroll
+            for (int p = 0; p < S::HP; p++)
+                *reinterpret_cast<uint4 *>(there + p * S::KB * TC_M * 128) = make_uint4(w[0][p], w[1][p], w[2][p], w[3][p]);
+        }
+    }
+    asm volatile("fence.proxy.async;" ::: "memory");   // h is read by the tensor cores, here and in the other CTAs
+    cluster.sync();
+    asm volatile("fence.proxy.async;" ::: "memory");
+    if (S::OVERLAY)
+        for (int st = 0; st < S::STAGES - 1; st++) fetch_n(st);
+
+    // ---- out = base + h B.  Warp w reads the rows of quarter w % 4 and the columns of half w / 4: two groups of 32 columns
+    // times two of sixteen rows, a lane eight columns of rows g and g + 8 of each.
+    constexpr int V = sizeof(OT) / 2, E = 8 / V;    // V groups of E consecutive columns
+    const OT *bp[4];
+    OT *op[4];
+    bool has[4];
+    const int first_col = warp / 4 * 64 + q * E;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {                    // rows g, g + 8, g + 16, g + 24 of the quarter
+        const int t = rows[warp % 4 * 32 + g + i * 8];
+        has[i] = (unsigned)t < (unsigned)P.n;
+        bp[i] = base + (has[i] ? (size_t)t * P.N : 0);
+        op[i] = out + (has[i] ? (size_t)t * P.N : 0);
+    }
+    float4 held[2][4][V];                            // base, as loaded: [32 columns][row][16 bytes]
+    auto load_base = [&](int st) {
+        const int col = (n0 + st) * 128 + first_col;
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int v = 0; v < V; v++)
+                    if (has[i] && col + u * 32 + v * 16 < P.N) held[u][i][v] = *reinterpret_cast<const float4 *>(bp[i] + col + u * 32 + v * 16);
+    };
+    auto ahead_base = [&](int st) {                  // towards L2, one lane for the bytes of four
+        const int col = (n0 + st) * 128 + first_col;
+        if (q == 0 && st < nst)
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (has[i] && col + u * 32 < P.N) asm volatile("prefetch.global.L2 [%0];" ::"l"(bp[i] + col + u * 32));
+    };
+    auto finish = [&](int st) {
+        const int col = (n0 + st) * 128 + first_col;
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+                uint32_t o[16];
+                tmem_ld_16x32(tmem + (st & 1) * 128 + warp / 4 * 64 + u * 32 + ((uint32_t)(warp % 4 * 32 + half * 16) << 16), o);
+                tmem_ld_wait();
+#pragma unroll
+                for (int r = 0; r < 2; r++)
+#pragma unroll
+                    for (int v = 0; v < V; v++) {
+                        const int i = half * 2 + r;
+                        if (!has[i] || col + u * 32 + v * 16 >= P.N) continue;
+                        float y[E];
+                        load_units<E>(reinterpret_cast<const OT *>(&held[u][i][v]), y);
+#pragma unroll
+                        for (int e = 0; e < E; e += 2) {
+                            const int j = v * (E / 2) + e / 2;
+                            y[e] += __uint_as_float(o[4 * j + 2 * r]);
+                            y[e + 1] += __uint_as_float(o[4 * j + 2 * r + 1]);
+                        }
+                        store_units<E>(op[i] + col + u * 32 + v * 16, y);
+                    }
+            }
+        tc_fence_before();
+    };
+    for (int st = 0; st < 3; st++) ahead_base(st);
+    for (int st = 0; st < nst; st++) {
+        copies_wait<S::STAGES - 2>();
+        fence_proxy_async();
+        __syncthreads();   // the copies of all threads, and their reads of this half of tensor memory
+        if (tid == 0) {
+            tc_fence_after();
+            const uint8_t *buffer = smem + ((kst + st) % S::STAGES) * S::STAGE;
+#pragma unroll
+            for (int p = 0; p < S::HP; p++)
+#pragma unroll
+                for (int kb = 0; kb < S::KB; kb++) {
+                    const uint64_t da = smem_desc_sw128(hs + (p * S::KB + kb) * TC_M * 128), db = smem_desc_sw128(buffer + kb * 16384);
+#pragma unroll
+                    for (int ks = 0; ks < (S::R < 64 ? S::R / 16 : 4); ks++)
+                        mma_f16(tmem + (st & 1) * 128, da + ks * 2, db + ks * 2, IDESC_OUT, p > 0 || kb > 0 || ks > 0);
+                }
+            tc_commit(&bars[(kst + st) % S::STAGES]);
+        }
+        if (st > 0) product_done(kst + st - 1);
+        fetch_n(st + S::STAGES - 1);
+        if (st > 0) {
+            tc_fence_after();
+            finish(st - 1);
+        }
+        load_base(st);
+        ahead_base(st + 3);
+    }
+    if (nst > 0) {
+        product_done(kst + nst - 1);
+        tc_fence_after();
+        finish(nst - 1);
+    }
+    copies_wait<0>();
+    __syncthreads();
+    if (warp == 0) tmem_dealloc(tmem, 256);
+    copy_bare_rows<TC_THREADS>(P, share_id, base, out);
+}
+
+// slots clusters of `ctas` CTAs
+template <typename Kern, typename XT, typename OT>
+static cudaError_t launch_clusters(Kern kern, int slots, int ctas, int threads, size_t smem, const AdapterArgs &P, const XT *x, const OT *base, OT *out,
+                                   cudaStream_t s)
+{
     if (smem > 40 * 1024) {   // with the static arrays, more than a launch may have without asking
         cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return e;
     }
-    // The cluster's size: more CTAs share a tile's K and N, each with the same work around it (finding the tile, the
-    // exchange of h: about as long as eight stages).  Taken is the size with the shortest sum over the waves
-    // that the grid makes: eight where the rows are few, one or two where the tiles alone fill the card.
-    const int slots = P.order ? P.n / T + P.L : P.n;
-    const int64_t room = 148 * (int64_t)max(1, min(2 * S::MIN_CTAS, (int)(227 * 1024 / (smem + 6144))));
-    int ctas = AD_MAX_CTAS;
-    double best = 1e30;
-    for (int c = AD_MAX_CTAS; c >= 1; c /= 2) {
-        const int64_t tiles = P.order ? min(P.n, (P.n + T - 1) / T + min(P.L, P.n) / 2) : min(P.n, P.L);
-        const double cost = max(1.0, (double)(tiles * c) / room) * (8.0 + (P.K + P.N) / 128.0 / c);
-        if (cost < best) { best = cost; ctas = c; }
-    }
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)slots * ctas);
-    cfg.blockDim = dim3(S::THREADS);
+    cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cudaLaunchAttribute at[2];
@@ -574,26 +867,60 @@ static cudaError_t launch_adapters_as(const AdapterArgs &P, const XT *x, const O
     return cudaLaunchKernelEx(&cfg, kern, P, x, base, out);
 }
 
+// The cluster's size: more CTAs share a tile's K and N (`shared` of work), each with the same work around it (finding the
+// tile, the exchange of h: `around`).  Taken is the size with the shortest sum over the waves that the grid makes: eight where
+// the rows are few, one or two where the tiles alone fill the card's `room`.
+static int cluster_size(int64_t tiles, int64_t room, double around, double shared)
+{
+    int ctas = AD_MAX_CTAS;
+    double best = 1e30;
+    for (int c = AD_MAX_CTAS; c >= 1; c /= 2) {
+        const double cost = max(1.0, (double)(tiles * c) / room) * (around + shared / c);
+        if (cost < best) { best = cost; ctas = c; }
+    }
+    return ctas;
+}
+// tiles of T rows, about: an adapter's last one is half full
+static int64_t tiles_of(const AdapterArgs &P, int T) { return min((int64_t)P.n, (int64_t)(P.n + T - 1) / T + min(P.L, P.n) / 2); }
+
+template <typename XT, typename OT, int RT>
+static cudaError_t launch_adapters_as(const AdapterArgs &P, const XT *x, const OT *base, OT *out, cudaStream_t s)
+{
+    using S = AdapterStage<XT, OT, 16, RT>;
+    const int64_t room = 148 * (int64_t)max(1, min(2 * S::MIN_CTAS, (int)(227 * 1024 / (S::SMEM + 6144))));
+    const int ctas = cluster_size(P.order ? tiles_of(P, 16) : min(P.n, P.L), room, 8.0, (P.K + P.N) / 128.0);   // in stages
+    return launch_clusters(k_adapters<XT, OT, 16, RT>, P.order ? P.n / 16 + P.L : P.n, ctas, S::THREADS, S::SMEM, P, x, base, out, s);
+}
+
+template <typename OT, int RT>
+static cudaError_t launch_adapters_tc(const AdapterArgs &P, const __nv_bfloat16 *x, const OT *base, OT *out, cudaStream_t s)
+{
+    const int ctas = cluster_size(tiles_of(P, TC_M), 148, 6.0, P.K / 64 * 0.35 + P.N / 128 * 0.9);   // in microseconds
+    return launch_clusters(k_adapters_tc<OT, RT>, P.n / TC_M + P.L, ctas, TC_THREADS, TcTile<OT, RT>::SMEM, P, x, base, out, s);
+}
+
 cudaError_t launch_adapters(const void *base, int out_dtype, const void *x, int x_dtype, const AdapterArgs &P, void *out, cudaStream_t s)
 {
-    // tiles of 64 rows where an adapter has that many on average; else of 16
-    const bool wide = P.order && P.n / P.L >= 48;
-    return with_type(x_dtype, [&](auto *xp) {
-        return with_type(out_dtype, [&](auto *op) {
+    // tiles of 128 rows where an adapter has enough of them and the rows are the tensor cores' own type; else of 16
+    const bool wide = P.order && P.n / P.L >= TC_MIN_ROWS && x_dtype == PMOE_BF16;
+    return with_type(out_dtype, [&](auto *op) {
+        using OT = std::remove_pointer_t<decltype(op)>;
+        const OT *bb = (const OT *)base;
+        OT *oo = (OT *)out;
+        if (wide) {
+            const __nv_bfloat16 *xx = (const __nv_bfloat16 *)x;
+            return P.r <= 16   ? launch_adapters_tc<OT, 2>(P, xx, bb, oo, s)
+                   : P.r <= 32 ? launch_adapters_tc<OT, 4>(P, xx, bb, oo, s)
+                   : P.r <= 64 ? launch_adapters_tc<OT, 8>(P, xx, bb, oo, s)
+                               : launch_adapters_tc<OT, 16>(P, xx, bb, oo, s);
+        }
+        return with_type(x_dtype, [&](auto *xp) {
             using XT = std::remove_pointer_t<decltype(xp)>;
-            using OT = std::remove_pointer_t<decltype(op)>;
             const XT *xx = (const XT *)x;
-            const OT *bb = (const OT *)base;
-            OT *oo = (OT *)out;
-            if (wide)
-                return P.r <= 16   ? launch_adapters_as<XT, OT, 64, 2>(P, xx, bb, oo, s)
-                       : P.r <= 32 ? launch_adapters_as<XT, OT, 64, 4>(P, xx, bb, oo, s)
-                       : P.r <= 64 ? launch_adapters_as<XT, OT, 64, 8>(P, xx, bb, oo, s)
-                                   : launch_adapters_as<XT, OT, 64, 16>(P, xx, bb, oo, s);
-            return P.r <= 16   ? launch_adapters_as<XT, OT, 16, 2>(P, xx, bb, oo, s)
-                   : P.r <= 32 ? launch_adapters_as<XT, OT, 16, 4>(P, xx, bb, oo, s)
-                   : P.r <= 64 ? launch_adapters_as<XT, OT, 16, 8>(P, xx, bb, oo, s)
-                               : launch_adapters_as<XT, OT, 16, 16>(P, xx, bb, oo, s);
+            return P.r <= 16   ? launch_adapters_as<XT, OT, 2>(P, xx, bb, oo, s)
+                   : P.r <= 32 ? launch_adapters_as<XT, OT, 4>(P, xx, bb, oo, s)
+                   : P.r <= 64 ? launch_adapters_as<XT, OT, 8>(P, xx, bb, oo, s)
+                               : launch_adapters_as<XT, OT, 16>(P, xx, bb, oo, s);
         });
     });
 }
@@ -624,5 +951,21 @@ extern "C" int pmoe_adapters_add(int device, const void *base, const void *x, in
     if (!guard.ok) return fail(PMOE_ERR_NO_DEVICE, "cannot select device %d", device);
     const AdapterArgs args{n, K, N, rank, n_adapters, (const __nv_bfloat16 *)a, (const __nv_bfloat16 *)b, scales, ids, order, offsets};
     CU(launch_adapters(base, out_dtype, x, x_dtype, args, out, (cudaStream_t)stream));
+    return PMOE_OK;
+}
+
+extern "C" int pmoe_rows_status(int device, void *stream)
+{
+    DeviceGuard guard(device);
+    if (!guard.ok) return fail(PMOE_ERR_NO_DEVICE, "cannot select device %d", device);
+    cudaStream_t s = (cudaStream_t)stream;
+    DevStatus st{}, zero{};
+    CU(cudaMemcpyFromSymbolAsync(&st, g_rows_status, sizeof st, 0, cudaMemcpyDeviceToHost, s));
+    CU(cudaStreamSynchronize(s));
+    if (st.code) {
+        CU(cudaMemcpyToSymbolAsync(g_rows_status, &zero, sizeof zero, 0, cudaMemcpyHostToDevice, s));
+        CU(cudaStreamSynchronize(s));
+        return fail(st.code, "device status %d raised by kernel tag %d (detail %d)", st.code, st.where, st.detail);
+    }
     return PMOE_OK;
 }

@@ -325,3 +325,13 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
     """Contiguous, from a 16-byte boundary on (a view may begin anywhere)."""
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def rows_status(device="cuda") -> None:
+    """Synchronises the current stream of `device` and raises PmoeError if a bounded wait inside ``adapters_add`` ran out
+    (its output is then not to be used): ``MoeBlock.status`` for the operators that have no handle."""
+    d = torch.device(device)
+    if d.type != "cuda":
+        raise PmoeError(-9, "rows_status needs a CUDA device; libpmoe has no CPU path")
+    index = torch.cuda.current_device() if d.index is None else d.index
+    check(lib().pmoe_rows_status(index, _stream(index)))
