@@ -121,11 +121,11 @@ template <int THREADS, typename OT> __device__ inline void copy_bare_rows(const 
         unsigned bare = __ballot_sync(0xffffffffu, (unsigned)my_id >= (unsigned)P.L);
         int u = threadIdx.x;   // this thread's next unit, of the lowest row left in `bare`
         while (true) {
-            float v[2][8];
-            size_t at[2];
+            float v[4][8];
+            size_t at[4];
             int got = 0;
 #pragma unroll
-            for (int k = 0; k < 2; k++) {
+            for (int k = 0; k < 4; k++) {
                 while (bare && u >= units) { u -= units; bare &= bare - 1; }
                 if (!bare) break;
                 at[k] = (size_t)(blockIdx.x + (int64_t)gridDim.x * (first + __ffs(bare) - 1)) * P.N + u * 8;
@@ -134,15 +134,35 @@ template <int THREADS, typename OT> __device__ inline void copy_bare_rows(const 
                 got++;
             }
 #pragma unroll
-            for (int k = 0; k < 2; k++)
+            for (int k = 0; k < 4; k++)
                 if (k < got) store_units<8>(out + at[k], v[k]);
-            if (got < 2) break;
+            if (got < 4) break;
         }
         first += 32;
         if (blockIdx.x + (int64_t)gridDim.x * first >= P.n) return;
         __syncwarp();
         my_id = id_of_share(P, first);
     }
+}
+
+// The sum of four floats at the same place in CTAS CTAs of the cluster, in CTA order; the loads are independent
+template <int CTAS> __device__ inline float4 sum_of_cluster(cg::cluster_group &cluster, const float *p)
+{
+    float4 v[CTAS], s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int o = 0; o < CTAS; o++) v[o] = *reinterpret_cast<const float4 *>(cluster.map_shared_rank(const_cast<float *>(p), o));
+#pragma unroll
+    for (int o = 0; o < CTAS; o++) { s.x += v[o].x; s.y += v[o].y; s.z += v[o].z; s.w += v[o].w; }
+    return s;
+}
+
+// f(Const<ctas>): clusters are of 1, 2, 4 or 8 CTAs
+template <typename F> __device__ __forceinline__ void with_cluster_size(int ctas, F &&f)
+{
+    if (ctas == 1) f(Const<1>{});
+    else if (ctas == 2) f(Const<2>{});
+    else if (ctas == 4) f(Const<4>{});
+    else f(Const<8>{});
 }
 
 // The tile of a slot, from the sorted ids: its adapter and rows (-1: none), the same for every CTA that asks for it.  Tile slots
@@ -434,17 +454,14 @@ __global__ void __launch_bounds__(AdapterStage<XT, OT, T, RT>::THREADS, AdapterS
     constexpr int per_row = RT * 2;
     if (T == 16) {
         cluster.sync();
-        for (int i = tid; i < 16 * per_row; i += THREADS) {   // every CTA adds all of it: one barrier less on the way
-            float *p = part + i / per_row * HS + i % per_row * 4;
-            float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int o = 0; o < AD_MAX_CTAS; o++) {
-                if (o >= ctas) break;
-                const float4 v = *reinterpret_cast<const float4 *>(cluster.map_shared_rank(p, o));
-                s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+        with_cluster_size(ctas, [&](auto n) {   // every CTA adds all of it: one barrier less on the way
+            constexpr int CTAS = decltype(n)();
+            for (int i = tid; i < 16 * per_row; i += THREADS) {
+                const int at = i / per_row * HS + i % per_row * 4;
+                const float4 s = sum_of_cluster<CTAS>(cluster, part + at);
+                *reinterpret_cast<float4 *>(h + at) = make_float4(s.x * scale, s.y * scale, s.z * scale, s.w * scale);
             }
-            *reinterpret_cast<float4 *>(h + i / per_row * HS + i % per_row * 4) = make_float4(s.x * scale, s.y * scale, s.z * scale, s.w * scale);
-        }
+        });
         __syncthreads();
     } else {
         cluster.sync();
@@ -571,6 +588,9 @@ template <typename OT, int RT> struct TcTile {
     static constexpr int ROOM = 218 * 1024 - H_BYTES - (OVERLAY ? 0 : PART);
     static constexpr int STAGES = ROOM / STAGE > 6 ? 6 : ROOM / STAGE;
     static constexpr int SMEM = 1024 + STAGES * STAGE + H_BYTES + (OVERLAY ? 0 : PART);
+    // A stage is fetched into the buffer of the stage LAG before the last: with a lag of two its product has had a whole step
+    // to end; where the buffers are few they are worth more as stages on their way.
+    static constexpr int LAG = STAGES >= 5 ? 2 : 1, LEAD = STAGES - LAG;
     static_assert(STAGES >= 3 && (!OVERLAY || PART <= STAGES * STAGE), "room for the pipeline");
 };
 
@@ -671,9 +691,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_adapters_tc(AdapterArgs P, co
 
     // ---- this CTA's share of h
     constexpr uint32_t IDESC_H = make_idesc(1, 1, 1, S::R, TC_M), IDESC_OUT = make_idesc(1, 1, 1, 128, TC_M);   // bf16 x bf16 -> f32
-    for (int st = 0; st < S::STAGES - 1; st++) fetch_k(st);
+    for (int st = 0; st < S::LEAD; st++) fetch_k(st);
     for (int st = 0; st < kst; st++) {
-        copies_wait<S::STAGES - 2>();
+        copies_wait<S::LEAD - 1>();
         fence_proxy_async();
         __syncthreads();
         if (tid == 0) {
@@ -684,13 +704,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_adapters_tc(AdapterArgs P, co
             for (int ks = 0; ks < 4; ks++) mma_f16(tmem, da + ks * 2, db + ks * 2, IDESC_H, st > 0 || ks > 0);
             tc_commit(&bars[st % S::STAGES]);
         }
-        if (st > 0) product_done(st - 1);
-        fetch_k(st + S::STAGES - 1);
+        if (st >= S::LAG) product_done(st - S::LAG);
+        fetch_k(st + S::LEAD);
     }
     if (kst > 0) product_done(kst - 1);
     tc_fence_after();
     if (!S::OVERLAY)
-        for (int st = 0; st < S::STAGES - 1; st++) fetch_n(st);
+        for (int st = 0; st < S::LEAD; st++) fetch_n(st);
     else
         __syncthreads();
 
@@ -710,35 +730,31 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_adapters_tc(AdapterArgs P, co
     tc_fence_before();
     cluster.sync();
     const float scale = P.scales ? P.scales[id] : 1.f;
-    for (int i = c * TC_THREADS + tid; i < TC_M * RT; i += ctas * TC_THREADS) {   // eight ranks of a row
-        const int row = i / RT, k8 = i % RT;
-        float s[8] = {};
+    with_cluster_size(ctas, [&](auto n) {
+        constexpr int CTAS = decltype(n)();
+        for (int i = c * TC_THREADS + tid; i < TC_M * RT; i += CTAS * TC_THREADS) {   // eight ranks of a row
+            const int row = i / RT, k8 = i % RT;
+            const float4 u = sum_of_cluster<CTAS>(cluster, part + row * S::PS + k8 * 8), v = sum_of_cluster<CTAS>(cluster, part + row * S::PS + k8 * 8 + 4);
+            uint32_t w[4][S::HP];
+            split_pair<S::HP>(u.x * scale, u.y * scale, w[0]);
+            split_pair<S::HP>(u.z * scale, u.w * scale, w[1]);
+            split_pair<S::HP>(v.x * scale, v.y * scale, w[2]);
+            split_pair<S::HP>(v.z * scale, v.w * scale, w[3]);
+            uint8_t *at = hs + k8 / 8 * (TC_M * 128) + row * 128 + ((k8 % 8 ^ row % 8) << 4);
 #pragma unroll
-        for (int o = 0; o < AD_MAX_CTAS; o++) {
-            if (o >= ctas) break;
-            const float4 *p = reinterpret_cast<const float4 *>(cluster.map_shared_rank(part + row * S::PS + k8 * 8, o));
-            const float4 u = p[0], v = p[1];
-            s[0] += u.x; s[1] += u.y; s[2] += u.z; s[3] += u.w;
-            s[4] += v.x; s[5] += v.y; s[6] += v.z; s[7] += v.w;
+            for (int o = 0; o < CTAS; o++) {
+                uint8_t *there = cluster.map_shared_rank(at, o);
+#pragma unroll
+                for (int p = 0; p < S::HP; p++)
+                    *reinterpret_cast<uint4 *>(there + p * S::KB * TC_M * 128) = make_uint4(w[0][p], w[1][p], w[2][p], w[3][p]);
+            }
         }
-        uint32_t w[4][S::HP];
-#pragma unroll
-        for (int e = 0; e < 4; e++) split_pair<S::HP>(s[2 * e] * scale, s[2 * e + 1] * scale, w[e]);
-        uint8_t *at = hs + k8 / 8 * (TC_M * 128) + row * 128 + ((k8 % 8 ^ row % 8) << 4);
-#pragma unroll
-        for (int o = 0; o < AD_MAX_CTAS; o++) {
-            if (o >= ctas) break;
-            uint8_t *there = cluster.map_shared_rank(at, o);
-#pragma unroll
-            for (int p = 0; p < S::HP; p++)
-                *reinterpret_cast<uint4 *>(there + p * S::KB * TC_M * 128) = make_uint4(w[0][p], w[1][p], w[2][p], w[3][p]);
-        }
-    }
+    });
     asm volatile("fence.proxy.async;" ::: "memory");   // h is read by the tensor cores, here and in the other CTAs
     cluster.sync();
     asm volatile("fence.proxy.async;" ::: "memory");
     if (S::OVERLAY)
-        for (int st = 0; st < S::STAGES - 1; st++) fetch_n(st);
+        for (int st = 0; st < S::LEAD; st++) fetch_n(st);
 
     // ---- out = base + h B.  Warp w reads the rows of quarter w % 4 and the columns of half w / 4: two groups of 32 columns
     // times two of sixteen rows, a lane eight columns of rows g and g + 8 of each.
@@ -754,17 +770,6 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_adapters_tc(AdapterArgs P, co
         bp[i] = base + (has[i] ? (size_t)t * P.N : 0);
         op[i] = out + (has[i] ? (size_t)t * P.N : 0);
     }
-    float4 held[2][4][V];                            // base, as loaded: [32 columns][row][16 bytes]
-    auto load_base = [&](int st) {
-        const int col = (n0 + st) * 128 + first_col;
-#pragma unroll
-        for (int u = 0; u < 2; u++)
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int v = 0; v < V; v++)
-                    if (has[i] && col + u * 32 + v * 16 < P.N) held[u][i][v] = *reinterpret_cast<const float4 *>(bp[i] + col + u * 32 + v * 16);
-    };
     auto ahead_base = [&](int st) {                  // towards L2, one lane for the bytes of four
         const int col = (n0 + st) * 128 + first_col;
         if (q == 0 && st < nst)
@@ -774,37 +779,48 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_adapters_tc(AdapterArgs P, co
                 for (int i = 0; i < 4; i++)
                     if (has[i] && col + u * 32 < P.N) asm volatile("prefetch.global.L2 [%0];" ::"l"(bp[i] + col + u * 32));
     };
-    auto finish = [&](int st) {
+    float4 held[2][2][4][V];                         // base of two chunks, as loaded: [32 columns][row][16 bytes]
+    auto load_base = [&](int st, auto which) {
         const int col = (n0 + st) * 128 + first_col;
+        if (st < nst)
 #pragma unroll
-        for (int u = 0; u < 2; u++)
+            for (int u = 0; u < 2; u++)
 #pragma unroll
-            for (int half = 0; half < 2; half++) {
-                uint32_t o[16];
-                tmem_ld_16x32(tmem + (st & 1) * 128 + warp / 4 * 64 + u * 32 + ((uint32_t)(warp % 4 * 32 + half * 16) << 16), o);
-                tmem_ld_wait();
+                for (int i = 0; i < 4; i++)
 #pragma unroll
-                for (int r = 0; r < 2; r++)
+                    for (int v = 0; v < V; v++)
+                        if (has[i] && col + u * 32 + v * 16 < P.N) held[which][u][i][v] = *reinterpret_cast<const float4 *>(bp[i] + col + u * 32 + v * 16);
+    };
+    auto finish = [&](int st, auto which) {          // `which` is st % 2
+        const int col = (n0 + st) * 128 + first_col;
+        uint32_t o[2][16];                           // the sums of sixteen rows, read while those before are stored
+        auto read = [&](auto k) { tmem_ld_16x32(tmem + which * 128 + warp / 4 * 64 + k / 2 * 32 + ((uint32_t)(warp % 4 * 32 + k % 2 * 16) << 16), o[k % 2]); };
+        read(Const<0>{});
+        each<4>([&](auto k) {
+            constexpr int u = k / 2, half = k % 2;
+            tmem_ld_wait();
+            if constexpr (k < 3) read(Const<k + 1>{});
 #pragma unroll
-                    for (int v = 0; v < V; v++) {
-                        const int i = half * 2 + r;
-                        if (!has[i] || col + u * 32 + v * 16 >= P.N) continue;
-                        float y[E];
-                        load_units<E>(reinterpret_cast<const OT *>(&held[u][i][v]), y);
+            for (int r = 0; r < 2; r++)
 #pragma unroll
-                        for (int e = 0; e < E; e += 2) {
-                            const int j = v * (E / 2) + e / 2;
-                            y[e] += __uint_as_float(o[4 * j + 2 * r]);
-                            y[e + 1] += __uint_as_float(o[4 * j + 2 * r + 1]);
-                        }
-                        store_units<E>(op[i] + col + u * 32 + v * 16, y);
+                for (int v = 0; v < V; v++) {
+                    constexpr int i0 = half * 2;
+                    if (!has[i0 + r] || col + u * 32 + v * 16 >= P.N) continue;
+                    float y[E];
+                    load_units<E>(reinterpret_cast<const OT *>(&held[which][u][i0 + r][v]), y);
+#pragma unroll
+                    for (int e = 0; e < E; e += 2) {
+                        const int j = v * (E / 2) + e / 2;
+                        y[e] += __uint_as_float(o[half][4 * j + 2 * r]);
+                        y[e + 1] += __uint_as_float(o[half][4 * j + 2 * r + 1]);
                     }
-            }
+                    store_units<E>(op[i0 + r] + col + u * 32 + v * 16, y);
+                }
+        });
         tc_fence_before();
     };
-    for (int st = 0; st < 3; st++) ahead_base(st);
-    for (int st = 0; st < nst; st++) {
-        copies_wait<S::STAGES - 2>();
+    auto step = [&](int st, auto which) {            // `which` is st % 2
+        copies_wait<S::LEAD - 1>();
         fence_proxy_async();
         __syncthreads();   // the copies of all threads, and their reads of this half of tensor memory
         if (tid == 0) {
@@ -817,23 +833,30 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_adapters_tc(AdapterArgs P, co
                     const uint64_t da = smem_desc_sw128(hs + (p * S::KB + kb) * TC_M * 128), db = smem_desc_sw128(buffer + kb * 16384);
 #pragma unroll
                     for (int ks = 0; ks < (S::R < 64 ? S::R / 16 : 4); ks++)
-                        mma_f16(tmem + (st & 1) * 128, da + ks * 2, db + ks * 2, IDESC_OUT, p > 0 || kb > 0 || ks > 0);
+                        mma_f16(tmem + which * 128, da + ks * 2, db + ks * 2, IDESC_OUT, p > 0 || kb > 0 || ks > 0);
                 }
             tc_commit(&bars[(kst + st) % S::STAGES]);
         }
         if (st > 0) product_done(kst + st - 1);
-        fetch_n(st + S::STAGES - 1);
+        fetch_n(st + S::LEAD);
         if (st > 0) {
             tc_fence_after();
-            finish(st - 1);
+            finish(st - 1, Const<1 - which>{});
         }
-        load_base(st);
+        load_base(st + 1, Const<1 - which>{});
         ahead_base(st + 3);
+    };
+    for (int st = 1; st < 3; st++) ahead_base(st);
+    load_base(0, Const<0>{});
+    for (int st = 0; st < nst; st += 2) {
+        step(st, Const<0>{});
+        if (st + 1 < nst) step(st + 1, Const<1>{});
     }
     if (nst > 0) {
         product_done(kst + nst - 1);
         tc_fence_after();
-        finish(nst - 1);
+        if (nst % 2) finish(nst - 1, Const<0>{});
+        else finish(nst - 1, Const<1>{});
     }
     copies_wait<0>();
     __syncthreads();
@@ -895,7 +918,7 @@ static cudaError_t launch_adapters_as(const AdapterArgs &P, const XT *x, const O
 template <typename OT, int RT>
 static cudaError_t launch_adapters_tc(const AdapterArgs &P, const __nv_bfloat16 *x, const OT *base, OT *out, cudaStream_t s)
 {
-    const int ctas = cluster_size(tiles_of(P, TC_M), 148, 6.0, P.K / 64 * 0.35 + P.N / 128 * 0.9);   // in microseconds
+    const int ctas = cluster_size(tiles_of(P, TC_M), 148, 8.0, P.K / 64 * 0.35 + P.N / 128 * 0.9);   // in microseconds
     return launch_clusters(k_adapters_tc<OT, RT>, P.n / TC_M + P.L, ctas, TC_THREADS, TcTile<OT, RT>::SMEM, P, x, base, out, s);
 }
 
