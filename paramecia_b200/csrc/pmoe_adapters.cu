@@ -4,13 +4,12 @@
 // (paramecia-model/src/models/with_tracing.rs:103-337).
 //
 // What bounds it: 2 r (K + N) flops over K x + 2 N out elements a row, at most r flops a byte, below the ridge of the card
-// for every rank served (r <= 128), so the rows' stream from memory is the limit for prompts, and latency for single
-// tokens.  The warp-level matrix instructions are fast enough for that rate and take their operands from registers, where
-// the loads put them: no shared-memory staging of x, A or B at all.
+// (258) for every rank served (r <= 128): the rows' stream from memory for prompts, latency for single tokens.
 //
-// One kernel does both products.  A tile of up to T rows of one adapter belongs to a cluster of eight CTAs: each takes an
-// eighth of K for its share of h = A x, the shares are added through distributed shared memory, and each CTA
-// then takes an eighth of the N output columns.  h never goes to memory, and a single token still uses eight SMs.
+// One kernel does both products.  A tile of rows of one adapter belongs to a cluster of one to eight CTAs: each takes a part of
+// K for its share of h = A x, the shares are added through distributed shared memory, and each CTA then takes a part of the N
+// output columns.  h never goes to memory, and a single token still uses eight SMs.  Two kernels of that form: tiles of
+// sixteen rows on the warp-level matrix instructions (k_adapters), and of 128 rows on tcgen05 (k_adapters_tc).
 #include <cooperative_groups.h>
 
 #include "pmoe_internal.h"
@@ -21,8 +20,9 @@ namespace pmoe {
 
 namespace cg = cooperative_groups;
 
-constexpr int ADAPTER_MAX_RANK = 128;
+constexpr int ADAPTER_MAX_RANK = 128, ADAPTER_MAX = 4096;
 constexpr int ADAPTER_ROWS_UNSORTED = 1024;   // rows that are grouped by id without pmoe_sort_pairs
+constexpr int ADAPTER_ROWS_LEADER = 128;       // ... where every row looks for the rows of its own id alone
 constexpr int AD_MAX_CTAS = 8;                // CTAs of a cluster
 
 // c += a b, 16 x 8 x 16, bf16 operands, f32 sums.  Lane l, g = l / 4, q = l % 4: a0 / a1 = rows g / g + 8 at the inner pair
@@ -165,71 +165,134 @@ template <typename F> __device__ __forceinline__ void with_cluster_size(int ctas
     else f(Const<8>{});
 }
 
-// The tile of a slot, from the sorted ids: its adapter and rows (-1: none), the same for every CTA that asks for it.  Tile slots
-// of adapter e begin at offsets[e] / T + e: with one slot more than whole multiples of T inside its range that is never
-// fewer than it has tiles, and needs no scan over the adapters.
+// The tile of a slot: its adapter and rows (-1: none), the same for every CTA that asks for it.  With the adapters' rows one
+// after another (the first of adapter e at offsets[e]), its tile slots begin at offsets[e] / T + e: with one slot more than whole
+// multiples of T inside its range that is never fewer than it has tiles, and each adapter finds its own without a scan.
 template <int T, int THREADS>
-__device__ inline void find_tile(const AdapterArgs &P, int slot, int *rows, int &tile_id, int &tile_rows, int &tile_first)
+__device__ inline void tile_of_slot(const AdapterArgs &P, const int *offsets, int slot, int &tile_id, int &tile_rows, int &tile_first)
 {
-    const int tid = threadIdx.x;
-    if (tid == 0) tile_rows = 0;
-    __syncthreads();
-    for (int e = tid; e < P.L; e += THREADS) {
-        const int from = P.offsets[e], to = min(P.offsets[e + 1], P.n), nth = slot - (from / T + e);
+    for (int e = threadIdx.x; e < P.L; e += THREADS) {
+        const int from = offsets[e], to = min(offsets[e + 1], P.n), nth = slot - (from / T + e);
         if (from >= 0 && nth >= 0 && nth < (to - from + T - 1) / T) {   // one adapter at most
             tile_id = e;
             tile_first = from + nth * T;
             tile_rows = min(T, to - from - nth * T);
         }
     }
+}
+
+// From pmoe_sort_pairs's arrays
+template <int T, int THREADS>
+__device__ inline void find_tile(const AdapterArgs &P, int slot, int *rows, int &tile_id, int &tile_rows, int &tile_first)
+{
+    const int tid = threadIdx.x;
+    if (tid == 0) tile_rows = 0;
+    __syncthreads();
+    tile_of_slot<T, THREADS>(P, P.offsets, slot, tile_id, tile_rows, tile_first);
     __syncthreads();
     if (tid < T) rows[tid] = tid < tile_rows ? P.order[tile_first + tid] : -1;
     __syncthreads();
 }
 
-// A CTA walks its share of K and then its share of N in stages of four chunks of 32: a stage holds what the matrix
-// instructions of those chunks need, as the lanes need it (sixteen bytes per lane, lanes side by side, so no
-// access meets a bank twice).  The copies are asynchronous and STAGES stages are on their way, the first ones of N
-// while the shares of h are still being added.
-//
-// A warp has sixteen rows and KH of them share a stage's four chunks: what a warp does per chunk is a chain of dependent
-// steps (read, multiply, add the base, write), so it takes about sixteen warps an SM to fill each other's gaps.  With one warp
-// per sixteen rows (four to eight an SM) 8192 rows of 2048 bf16, rank 64, took 82 us.
+// From the ids alone: every CTA counts them, then looks for the rows of its own tile.  A sort in front is a launch of its own,
+// 4 us for few rows (1000 rows, 4 adapters of rank 64: 16.3 us without it, 20.7 us with it), but it reads the ids once where
+// here every CTA does: 8192 rows take 56 us without and 47 us with it.
+// offsets: L + 1 words of shared memory
+template <int T, int THREADS>
+__device__ inline void find_tile_by_ids(const AdapterArgs &P, int slot, int *rows, int &tile_id, int &tile_rows, int &tile_first, int *offsets)
+{
+    constexpr int WARPS = THREADS / 32;
+    __shared__ int found_by[WARPS];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    for (int e = tid; e <= P.L; e += THREADS) offsets[e] = 0;
+    if (tid == 0) tile_rows = 0;
+    __syncthreads();
+#pragma unroll 4
+    for (int t = tid; t - lane < P.n; t += THREADS) {
+        const int id = t < P.n ? P.ids[t] : -1;
+        const int same = __all_sync(0xffffffffu, id == __shfl_sync(0xffffffffu, id, 0));   // a prompt's rows
+        if ((unsigned)id < (unsigned)P.L && (!same || lane == 0)) atomicAdd(offsets + id, same ? 32 : 1);
+    }
+    __syncthreads();
+    if (warp == 0) {   // the counts become their exclusive sums
+        int before = 0;
+        for (int e = lane; e - lane <= P.L; e += 32) {
+            const int count = e < P.L ? offsets[e] : 0;
+            int incl = count;
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, incl, off);
+                if (lane >= off) incl += y;
+            }
+            if (e <= P.L) offsets[e] = before + incl - count;
+            before += __shfl_sync(0xffffffffu, incl, 31);
+        }
+    }
+    __syncthreads();
+    tile_of_slot<T, THREADS>(P, offsets, slot, tile_id, tile_rows, tile_first);
+    if (tid < T) rows[tid] = -1;
+    __syncthreads();
+    if (tile_rows == 0) return;
+    // a warp's part of the ids; its rows of this adapter are counted, then those of the tile's range written down
+    const int id = tile_id, first = tile_first - offsets[id], part = (P.n + THREADS - 1) / THREADS * 32;
+    const int t0 = warp * part, t1 = min(P.n, t0 + part);
+    int count = 0;
+#pragma unroll 4
+    for (int t = t0 + lane; t - lane < t1; t += 32) count += __popc(__ballot_sync(0xffffffffu, t < t1 && P.ids[t] == id));
+    if (lane == 0) found_by[warp] = count;
+    __syncthreads();
+    int nth = -first;
+#pragma unroll
+    for (int w = 0; w < WARPS; w++)
+        if (w < warp) nth += found_by[w];
+    if (nth < T && nth + count > 0)
+        for (int t = t0 + lane; t - lane < t1 && nth < T; t += 32) {
+            const bool mine = t < t1 && P.ids[t] == id;
+            const unsigned m = __ballot_sync(0xffffffffu, mine);
+            const int at = nth + __popc(m & ((1u << lane) - 1));
+            if (mine && at >= 0 && at < T) rows[at] = t;
+            nth += __popc(m);
+        }
+    __syncthreads();
+}
+
+// ---------------------------------------------------------------- few rows of an adapter, or f32 rows: sixteen rows a tile
+// A CTA of four warps walks its share of K and then its share of N in stages of four chunks of 32, a chunk a warp: a stage
+// holds what the matrix instructions of a chunk need, as the lanes need it (sixteen bytes per lane, lanes side by side, so no
+// access meets a bank twice), and a warp reads what its own lanes fetched.  The copies are asynchronous and STAGES stages are on
+// their way, the first ones of N while the shares of h are still being added: one decoding row of 2048 x 2048 takes 5.2 us, 64
+// rows with 36 adapters of rank 32 (2048 to 4096) 11 us, which is the chain id -> rows -> h -> exchange -> columns.
 // RT: groups of eight ranks that the accumulators are sized for.
-template <typename XT, typename OT, int T, int RT> struct AdapterStage {
+constexpr int FEW_M = 16, FEW_THREADS = 128;
+
+template <typename XT, typename OT, int RT> struct AdapterStage {
     static constexpr int SIZE = sizeof(XT) > sizeof(OT) ? sizeof(XT) : sizeof(OT);
-    static constexpr int KH = T == 16 ? 4 : SIZE == 4 && RT < 16 ? 4 : 2;
-    static constexpr int WARPS = T / 16 * KH, THREADS = WARPS * 32, CPW = 4 / KH;
-    static constexpr int MIN_CTAS = T == 16 ? 4 : WARPS == 8 && RT < 16 ? 2 : 1;
     static constexpr int WEIGHTS = 4 * RT * 32 * 16;                     // A: 4 chunks x RT rank groups; B: 4 chunks x 4 products x RT / 4 rank steps
     static constexpr int ROW_CHUNK = 2 * 32 * 8 * SIZE;                 // two rows of eight elements a lane
-    static constexpr int ROWS = T / 16 * 4 * ROW_CHUNK;
-    static constexpr int BYTES = WEIGHTS + ROWS;
+    static constexpr int BYTES = WEIGHTS + 4 * ROW_CHUNK;
     static constexpr int HS = RT == 2 ? 16 : RT * 8 + 16;               // floats between two rows of h: no two rows of a quarter warp start in one bank
-    static constexpr int H_BYTES = (KH / 2 + 1) * T * HS * 4;
-    static constexpr int ROOM = (T == 16 ? (RT == 16 ? 222 : 110) : MIN_CTAS == 2 ? 112 : 222) * 1024 - H_BYTES;   // of the 227 KB of an SM, a CTA's part
+    static constexpr int H_BYTES = 3 * FEW_M * HS * 4;
+    static constexpr int ROOM = (RT == 16 ? 222 : 110) * 1024 - H_BYTES;   // of the 227 KB of an SM: one or two CTAs at least
     static constexpr int STAGES = ROOM / BYTES < 2 ? 2 : ROOM / BYTES > 4 ? 4 : ROOM / BYTES;
     static constexpr int SMEM = STAGES * BYTES + H_BYTES;
     static_assert(SMEM <= 222 * 1024, "fits an SM beside the static arrays");
 };
 
-template <typename XT, typename OT, int T, int RT>
-__global__ void __launch_bounds__(AdapterStage<XT, OT, T, RT>::THREADS, AdapterStage<XT, OT, T, RT>::MIN_CTAS) k_adapters(AdapterArgs P, const XT *__restrict__ x, const OT *base, OT *out)
+template <typename XT, typename OT, int RT>
+__global__ void __launch_bounds__(FEW_THREADS, RT == 16 ? 1 : 4) k_adapters(AdapterArgs P, const XT *__restrict__ x, const OT *base, OT *out)
 {
-    using S = AdapterStage<XT, OT, T, RT>;
+    using S = AdapterStage<XT, OT, RT>;
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ int rows[T];
+    __shared__ int rows[FEW_M];
     __shared__ int tile_id, tile_rows, tile_first;
-    __shared__ int all_ids[T == 16 ? ADAPTER_ROWS_UNSORTED : 1];   // without an order T is 16
-    constexpr int THREADS = S::THREADS, CPW = S::CPW;
-    constexpr int HP = std::is_same<OT, float>::value ? 3 : 2;   // pieces of h: an f32 result keeps all of it, a bf16 result 16 bits
+    __shared__ int all_ids[ADAPTER_ROWS_LEADER];
+    constexpr int HP = sizeof(OT) == 4 ? 3 : 2;   // pieces of h: an f32 result keeps all of it, a bf16 result 16 bits
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3;
-    const int rg = warp % (T / 16), kh = warp / (T / 16);   // this warp's sixteen rows and its chunks of a stage
     cg::cluster_group cluster = cg::this_cluster();
     const int ctas = (int)cluster.num_blocks(), c = (int)cluster.block_rank(), slot = blockIdx.x / ctas;
     constexpr int HS = S::HS;
-    float *part = reinterpret_cast<float *>(smem + S::STAGES * S::BYTES);   // [KH / 2][T][HS] this CTA's share of h
-    float *h = part + S::KH / 2 * T * HS;                                   // [T][HS]
+    float *part = reinterpret_cast<float *>(smem + S::STAGES * S::BYTES);   // [2][16][HS] this CTA's share of h
+    float *h = part + 2 * FEW_M * HS;                                       // [16][HS]
     pdl_wait();
     pdl_launch_dependents();
 
@@ -237,40 +300,39 @@ __global__ void __launch_bounds__(AdapterStage<XT, OT, T, RT>::THREADS, AdapterS
 
     // ---- the tile: its adapter and rows.  Every CTA of the cluster finds the same.
     if (P.order) {
-        find_tile<T, THREADS>(P, slot, rows, tile_id, tile_rows, tile_first);
-    } else if constexpr (T == 16) {
-        // slot t leads a tile when the number of earlier rows with its id is a multiple of T
+        find_tile<FEW_M, FEW_THREADS>(P, slot, rows, tile_id, tile_rows, tile_first);
+    } else if (P.n > ADAPTER_ROWS_LEADER) {
+        find_tile_by_ids<FEW_M, FEW_THREADS>(P, slot, rows, tile_id, tile_rows, tile_first, reinterpret_cast<int *>(smem));
+    } else {
+        // slot t leads a tile when the number of earlier rows with its id is a multiple of sixteen
         const int id = P.ids[slot];
-        if (tid < T) rows[tid] = -1;
-        for (int t = tid; t < P.n; t += THREADS) all_ids[t] = P.ids[t];
+        if (tid < FEW_M) rows[tid] = -1;
+        for (int t = tid; t < P.n; t += FEW_THREADS) all_ids[t] = P.ids[t];
         __syncthreads();
         if (warp == 0) {
             int before = 0, found = 0;
-            for (int t = 0; t < P.n && found < T; t += 32) {
+            for (int t = 0; t < P.n && found < FEW_M; t += 32) {
                 const bool same = t + lane < P.n && all_ids[t + lane] == id;
                 const unsigned m = __ballot_sync(0xffffffffu, same);
                 const unsigned early = t + 32 <= slot ? m : t > slot ? 0u : m & ((1u << (slot - t)) - 1);
                 before += __popc(early);
                 const int at = found + __popc(m & ~early & ((1u << lane) - 1));
-                if (same && !(early >> lane & 1) && at < T) rows[at] = t + lane;
+                if (same && !(early >> lane & 1) && at < FEW_M) rows[at] = t + lane;
                 found += __popc(m & ~early);
             }
             if (lane == 0) {
                 tile_id = id;
-                tile_rows = (unsigned)id >= (unsigned)P.L || before % T ? 0 : min(found, T);
+                tile_rows = (unsigned)id >= (unsigned)P.L || before % FEW_M ? 0 : min(found, FEW_M);
             }
         }
         __syncthreads();
     }
     if (tile_rows == 0) {
-        copy_bare_rows<THREADS>(P, share_id, base, out);
+        copy_bare_rows<FEW_THREADS>(P, share_id, base, out);
         return;
     }
-    const int id = tile_id, nrows = tile_rows;
-    const int row_base = rg * 16;
-    const int t0 = rows[row_base + g], t1 = rows[row_base + g + 8];
+    const int id = tile_id, t0 = rows[g], t1 = rows[g + 8];
     const bool has0 = (unsigned)t0 < (unsigned)P.n, has1 = (unsigned)t1 < (unsigned)P.n;
-    const bool busy = row_base < nrows;       // a warp of a T = 64 tile may have no rows
 
     // ---- the stages of this CTA
     const int kc = (P.K + 31) / 32, nc = (P.N + 31) / 32;
@@ -278,17 +340,15 @@ __global__ void __launch_bounds__(AdapterStage<XT, OT, T, RT>::THREADS, AdapterS
     const int n0 = (int)((int64_t)nc * c / ctas), n1 = (int)((int64_t)nc * (c + 1) / ctas);
     const int kstages = (k1 - k0 + 3) / 4, stages = kstages + (n1 - n0 + 3) / 4;
     const int size0 = has0 ? 16 : 0, size1 = has1 ? 16 : 0;
-    // Where this lane fetches from, a stage further after each: its two rows in x, later in base; weights of chunk wc,
-    // rank groups wj, wj + WARPS / 4, ... of A, later products wj * JW and following of B.
-    constexpr int JW = 16 / S::WARPS, WSTEP = S::WARPS / 4;
-    const int wc = warp % 4, wj = warp / 4, chunk0 = kh * CPW;
-    const XT *x0 = x + (has0 ? (size_t)t0 * P.K : 0) + (k0 + chunk0) * 32 + q * (16 / (int)sizeof(XT)), *x1 = x + (has1 ? (size_t)t1 * P.K : 0) + (k0 + chunk0) * 32 + q * (16 / (int)sizeof(XT));
-    const OT *b0 = base + (has0 ? (size_t)t0 * P.N : 0) + (n0 + chunk0) * 32 + q * (16 / (int)sizeof(OT)), *b1 = base + (has1 ? (size_t)t1 * P.N : 0) + (n0 + chunk0) * 32 + q * (16 / (int)sizeof(OT));
-    const __nv_bfloat16 *aw = P.a + ((size_t)id * P.r + wj * 8 + g) * P.K + (k0 + wc) * 32 + q * 8;
-    const size_t aw_step = (size_t)WSTEP * 8 * P.K;
-    const __nv_bfloat16 *bw = P.b + ((size_t)id * P.N + (n0 + wc) * 32 + (g >> 1) * (16 / (int)sizeof(OT)) + (g & 1)) * P.r + q * (RT == 2 ? 4 : 8);
-    const uint32_t to = smem_u32(smem), to_rows = to + S::WEIGHTS + (rg * 4 + chunk0) * S::ROW_CHUNK,
-                   to_weights = to + wc * (S::WEIGHTS / 4);
+    // Where this lane fetches from, a stage further after each: its two rows in x, later in base; the weights of this warp's
+    // chunk in A, later in B.  EX, EO: elements of x and base in sixteen bytes.
+    constexpr int EX = 16 / sizeof(XT), EO = 16 / sizeof(OT);
+    const XT *x0 = x + (has0 ? (size_t)t0 * P.K : 0) + (k0 + warp) * 32 + q * EX, *x1 = x + (has1 ? (size_t)t1 * P.K : 0) + (k0 + warp) * 32 + q * EX;
+    const OT *b0 = base + (has0 ? (size_t)t0 * P.N : 0) + (n0 + warp) * 32 + q * EO, *b1 = base + (has1 ? (size_t)t1 * P.N : 0) + (n0 + warp) * 32 + q * EO;
+    const __nv_bfloat16 *aw = P.a + ((size_t)id * P.r + g) * P.K + (k0 + warp) * 32 + q * 8;
+    const size_t aw_step = (size_t)8 * P.K;
+    const __nv_bfloat16 *bw = P.b + ((size_t)id * P.N + (n0 + warp) * 32 + (g >> 1) * EO + (g & 1)) * P.r + q * (RT == 2 ? 4 : 8);
+    const uint32_t to_weights = smem_u32(smem) + warp * (S::WEIGHTS / 4), to_rows = smem_u32(smem) + S::WEIGHTS + warp * S::ROW_CHUNK;
     const bool all_ranks = P.r == RT * 8;
 
     // Rows: a copy instruction takes 64 consecutive bytes of each of eight rows.  For f32 that is half a chunk (v = 0, 1);
@@ -296,66 +356,56 @@ __global__ void __launch_bounds__(AdapterStage<XT, OT, T, RT>::THREADS, AdapterS
     // stay with the lane that adds them: its columns are four and four, sixteen apart.
     const uint32_t x_lane = sizeof(XT) == 2 ? lane * 16 : (q & 1) * 512 + (g * 4 + (q >> 1)) * 16;
     constexpr int X_STEP = 32, B_STEP = 512;   // from v = 0 to v = 1
-    auto fetch_rows = [&](uint32_t dst, auto step, auto *p0, auto *p1, int ch, int ch_end, int limit) {
+    auto fetch_rows = [&](uint32_t dst, auto step, auto *p0, auto *p1, bool whole, int first, int limit) {
         using VT = std::remove_cv_t<std::remove_pointer_t<decltype(p0)>>;
         constexpr int V = sizeof(VT) / 2, STEP = decltype(step)();   // V units of sixteen bytes in eight elements
-        each<CPW>([&](auto u) {
-            each<V>([&](auto v) {
-                const bool in = ch + u < ch_end && (ch + u) * 32 + v * 16 + q * (16 / (int)sizeof(VT)) < limit;
-                constexpr int D = u * S::ROW_CHUNK + v * STEP, O = u * 32 * (int)sizeof(VT) + v * 64;
-                // a copy of nothing still gets an address inside a tensor
-                copy16<D, 0>(dst, in ? (const char *)p0 + O : (const char *)P.a, in ? size0 : 0);
-                copy16<D + V * 512, 0>(dst, in ? (const char *)p1 + O : (const char *)P.a, in ? size1 : 0);
-            });
+        each<V>([&](auto v) {
+            if (whole) {
+                copy16<v * STEP, v * 64>(dst, p0, size0);
+                copy16<v * STEP + V * 512, v * 64>(dst, p1, size1);
+            } else {   // a copy of nothing still gets an address inside a tensor
+                const bool in = first + v * 16 < limit;
+                copy16<v * STEP, 0>(dst, in ? (const char *)p0 + v * 64 : (const char *)P.a, in ? size0 : 0);
+                copy16<v * STEP + V * 512, 0>(dst, in ? (const char *)p1 + v * 64 : (const char *)P.a, in ? size1 : 0);
+            }
         });
     };
-    auto fetch_rows_whole = [&](uint32_t dst, auto step, auto *p0, auto *p1) {
-        using VT = std::remove_cv_t<std::remove_pointer_t<decltype(p0)>>;
-        constexpr int V = sizeof(VT) / 2, STEP = decltype(step)();
-        each<CPW>([&](auto u) {
-            each<V>([&](auto v) {
-                constexpr int D = u * S::ROW_CHUNK + v * STEP, O = u * 32 * (int)sizeof(VT) + v * 64;
-                copy16<D, O>(dst, p0, size0);
-                copy16<D + V * 512, O>(dst, p1, size1);
-            });
-        });
-    };
-    uint32_t fetch_at = 0;   // the buffer of the next stage to fetch
+    int fetch_at = 0;   // the buffer of the next stage to fetch
     auto fetch = [&](int st) {
-        const uint32_t buffer = fetch_at;
+        const int buffer = fetch_at;
         fetch_at = fetch_at == (S::STAGES - 1) * S::BYTES ? 0 : fetch_at + S::BYTES;
         if (st < kstages) {
-            const int ch0 = k0 + st * 4;
-            const uint32_t dw = to_weights + buffer + wj * 512 + lane * 16;
-            if (ch0 + 4 <= k1 && (ch0 + 4) * 32 <= P.K && all_ranks) {
+            const int ch = k0 + st * 4 + warp;
+            const bool whole = ch < k1 && ch * 32 + 32 <= P.K && all_ranks;   // nothing of the chunk is missing
+            const int limit = ch < k1 ? P.K : 0;
+            const uint32_t dw = to_weights + buffer + lane * 16;
+            if (whole) {
                 const __nv_bfloat16 *src = aw;
-                each<(RT + WSTEP - 1) / WSTEP>([&](auto i) {
-                    if (RT >= WSTEP || wj < RT) copy16<i * WSTEP * 512, 0>(dw, src, 16);
+                each<RT>([&](auto i) {
+                    copy16<i * 512, 0>(dw, src, 16);
                     src += aw_step;
                 });
-                fetch_rows_whole(to_rows + buffer + x_lane, Const<X_STEP>{}, x0, x1);
             } else {
-                const bool in = ch0 + wc < k1 && (ch0 + wc) * 32 + q * 8 < P.K;
-                each<(RT + WSTEP - 1) / WSTEP>([&](auto i) {
-                    const bool there = in && (i * WSTEP + wj) * 8 < P.r;
-                    if (RT >= WSTEP || wj < RT) copy16<i * WSTEP * 512, 0>(dw, there ? aw + i * aw_step : P.a, there ? 16 : 0);
+                each<RT>([&](auto i) {
+                    const bool there = ch * 32 + q * 8 < limit && i * 8 < P.r;
+                    copy16<i * 512, 0>(dw, there ? aw + i * aw_step : P.a, there ? 16 : 0);
                 });
-                fetch_rows(to_rows + buffer + x_lane, Const<X_STEP>{}, x0, x1, ch0 + chunk0, k1, P.K);
             }
+            fetch_rows(to_rows + buffer + x_lane, Const<X_STEP>{}, x0, x1, whole, ch * 32 + q * EX, limit);
             x0 += 128; x1 += 128; aw += 128;
         } else if (st < stages) {
-            const int ch0 = n0 + (st - kstages) * 4;
-            const bool whole = ch0 + 4 <= n1 && (ch0 + 4) * 32 <= P.N && all_ranks;
-            const int col = (ch0 + wc) * 32 + (g >> 1) * (16 / (int)sizeof(OT)) + (g & 1);
-            each<JW>([&](auto j) {
-                const int product = wj * JW + j, skip = sizeof(OT) == 2 ? product * 2 : product / 2 * 16 + product % 2 * 2;
+            const int ch = n0 + (st - kstages) * 4 + warp;
+            const bool whole = ch < n1 && ch * 32 + 32 <= P.N && all_ranks;
+            const int limit = ch < n1 ? P.N : 0, col = ch * 32 + (g >> 1) * EO + (g & 1);
+            each<4>([&](auto j) {
+                constexpr int skip = sizeof(OT) == 2 ? j * 2 : j / 2 * 16 + j % 2 * 2;
                 const __nv_bfloat16 *src = bw + skip * P.r;
-                const bool in = whole || (ch0 + wc < n1 && col + skip < P.N);
+                const bool in = col + skip < limit;
                 if constexpr (RT == 2) {
                     const bool there = in && q * 4 < P.r;
-                    copy8(to_weights + buffer + (wj * JW + j) * 256 + lane * 8, there ? src : P.b, there ? 8 : 0);
+                    copy8(to_weights + buffer + j * 256 + lane * 8, there ? src : P.b, there ? 8 : 0);
                 } else {
-                    const uint32_t dw = to_weights + buffer + wj * (JW * (RT / 4) * 512) + lane * 16;
+                    const uint32_t dw = to_weights + buffer + lane * 16;
                     if (whole)
                         each<RT / 4>([&](auto s) { copy16<(j * (RT / 4) + s) * 512, s * 64>(dw, src, 16); });
                     else
@@ -365,61 +415,52 @@ __global__ void __launch_bounds__(AdapterStage<XT, OT, T, RT>::THREADS, AdapterS
                         });
                 }
             });
-            if (whole) fetch_rows_whole(to_rows + buffer + lane * 16, Const<B_STEP>{}, b0, b1);
-            else fetch_rows(to_rows + buffer + lane * 16, Const<B_STEP>{}, b0, b1, ch0 + chunk0, n1, P.N);
+            fetch_rows(to_rows + buffer + lane * 16, Const<B_STEP>{}, b0, b1, whole, ch * 32 + q * EO, limit);
             b0 += 128; b1 += 128; bw += (size_t)128 * P.r;
         }
         copies_commit();
     };
     int buffer = 0;          // of the stage that is being used
-    // T = 16: a warp reads what its own lanes fetched; T = 64: the weights come from all warps
     auto landed = [&] {
         copies_wait<S::STAGES - 1>();
-        if (T == 16) __syncwarp();
-        else __syncthreads();
+        __syncwarp();
     };
     auto done_with = [&](int st) {
-        if (T == 16) __syncwarp();
-        else __syncthreads();
+        __syncwarp();
         buffer = buffer == (S::STAGES - 1) * S::BYTES ? 0 : buffer + S::BYTES;
         fetch(st + S::STAGES);
     };
 #pragma unroll
     for (int st = 0; st < S::STAGES; st++) fetch(st);
-    const uint8_t *my_rows = smem + S::WEIGHTS + (rg * 4 + chunk0) * S::ROW_CHUNK + lane * 16;
-    const uint8_t *my_weights = smem + chunk0 * (S::WEIGHTS / 4);
+    const uint8_t *my_rows = smem + S::WEIGHTS + warp * S::ROW_CHUNK + lane * 16, *my_weights = smem + warp * (S::WEIGHTS / 4);
 
-    // ---- this warp's share of h = A x
+    // ---- this warp's share of h = A x; chunks behind the CTA's share are zeros
     float acc[RT][4] = {};
     for (int st = 0; st < kstages; st++) {
         landed();
-        if (busy)
+        constexpr int V = sizeof(XT) / 2, PC = XFrag<XT>::PIECES;
+        const uint4 *rv = reinterpret_cast<const uint4 *>(my_rows + buffer);
+        const uint4 *av = reinterpret_cast<const uint4 *>(my_weights + buffer) + lane;
+        uint32_t w0[4][PC], w1[4][PC];
+        XFrag<XT>::words(rv, w0);
+        XFrag<XT>::words(rv + V * 32, w1);
 #pragma unroll
-            for (int u = 0; u < CPW; u++) {   // chunks behind the share are zeros
-                constexpr int V = sizeof(XT) / 2, PC = XFrag<XT>::PIECES;
-                const uint4 *rv = reinterpret_cast<const uint4 *>(my_rows + buffer + u * S::ROW_CHUNK);
-                const uint4 *av = reinterpret_cast<const uint4 *>(my_weights + buffer + u * (S::WEIGHTS / 4)) + lane;
-                uint32_t w0[4][PC], w1[4][PC];
-                XFrag<XT>::words(rv, w0);
-                XFrag<XT>::words(rv + V * 32, w1);
+        for (int t = 0; t < RT; t += 2) {
+            const uint4 a = av[t * 32], b = av[(t + 1) * 32];
 #pragma unroll
-                for (int t = 0; t < RT; t += 2) {
-                    const uint4 a = av[t * 32], b = av[(t + 1) * 32];
-#pragma unroll
-                    for (int p = 0; p < PC; p++) {
-                        mma_bf16(acc[t], w0[0][p], w1[0][p], w0[1][p], w1[1][p], a.x, a.y);
-                        mma_bf16(acc[t + 1], w0[0][p], w1[0][p], w0[1][p], w1[1][p], b.x, b.y);
-                        mma_bf16(acc[t], w0[2][p], w1[2][p], w0[3][p], w1[3][p], a.z, a.w);
-                        mma_bf16(acc[t + 1], w0[2][p], w1[2][p], w0[3][p], w1[3][p], b.z, b.w);
-                    }
-                }
+            for (int p = 0; p < PC; p++) {
+                mma_bf16(acc[t], w0[0][p], w1[0][p], w0[1][p], w1[1][p], a.x, a.y);
+                mma_bf16(acc[t + 1], w0[0][p], w1[0][p], w0[1][p], w1[1][p], b.x, b.y);
+                mma_bf16(acc[t], w0[2][p], w1[2][p], w0[3][p], w1[3][p], a.z, a.w);
+                mma_bf16(acc[t + 1], w0[2][p], w1[2][p], w0[3][p], w1[3][p], b.z, b.w);
             }
+        }
         done_with(st);
     }
 
-    // the warps of the same rows: the upper half hands its sums to the lower half, lane to lane, until one has them all
+    // the four warps have the same rows: the upper half hands its sums to the lower half, lane to lane, until one has them all
     auto at_part = [&](int buffer, int i, int half) {
-        return reinterpret_cast<float2 *>(part + (buffer * T + row_base + g + half * 8) * HS + i * 8 + 2 * q);
+        return reinterpret_cast<float2 *>(part + (buffer * FEW_M + g + half * 8) * HS + i * 8 + 2 * q);
     };
     auto put = [&](int buffer) {
 #pragma unroll
@@ -435,52 +476,29 @@ __global__ void __launch_bounds__(AdapterStage<XT, OT, T, RT>::THREADS, AdapterS
             acc[i][0] += u.x; acc[i][1] += u.y; acc[i][2] += v.x; acc[i][3] += v.y;
         }
     };
-    if constexpr (S::KH == 4) {
-        if (kh >= 2) put(kh - 2);
-        __syncthreads();
-        if (kh < 2) add(kh);
-        if (kh == 1) put(1);
-        __syncthreads();
-        if (kh == 0) add(1);
-    } else {
-        if (kh == 1) put(0);
-        __syncthreads();
-        if (kh == 0) add(0);
+    if (warp >= 2) put(warp - 2);
+    __syncthreads();
+    if (warp < 2) add(warp);
+    if (warp == 1) put(1);
+    __syncthreads();
+    if (warp == 0) {
+        add(1);
+        put(0);
     }
-    if (kh == 0) put(0);
 
     // ---- the shares of the cluster added, in CTA order, times the adapter's scale
     const float scale = P.scales ? P.scales[id] : 1.f;
     constexpr int per_row = RT * 2;
-    if (T == 16) {
-        cluster.sync();
-        with_cluster_size(ctas, [&](auto n) {   // every CTA adds all of it: one barrier less on the way
-            constexpr int CTAS = decltype(n)();
-            for (int i = tid; i < 16 * per_row; i += THREADS) {
-                const int at = i / per_row * HS + i % per_row * 4;
-                const float4 s = sum_of_cluster<CTAS>(cluster, part + at);
-                *reinterpret_cast<float4 *>(h + at) = make_float4(s.x * scale, s.y * scale, s.z * scale, s.w * scale);
-            }
-        });
-        __syncthreads();
-    } else {
-        cluster.sync();
-        for (int i = c * THREADS + tid; i < T * per_row; i += ctas * THREADS) {   // each CTA its part, given to all
+    cluster.sync();
+    with_cluster_size(ctas, [&](auto n) {   // every CTA adds all of it: one barrier less on the way
+        constexpr int CTAS = decltype(n)();
+        for (int i = tid; i < FEW_M * per_row; i += FEW_THREADS) {
             const int at = i / per_row * HS + i % per_row * 4;
-            float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int o = 0; o < AD_MAX_CTAS; o++) {
-                if (o >= ctas) break;
-                const float4 v = *reinterpret_cast<const float4 *>(cluster.map_shared_rank(part + at, o));
-                s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
-            }
-            s = make_float4(s.x * scale, s.y * scale, s.z * scale, s.w * scale);
-#pragma unroll
-            for (int o = 0; o < AD_MAX_CTAS; o++)
-                if (o < ctas) *reinterpret_cast<float4 *>(cluster.map_shared_rank(h + at, o)) = s;
+            const float4 s = sum_of_cluster<CTAS>(cluster, part + at);
+            *reinterpret_cast<float4 *>(h + at) = make_float4(s.x * scale, s.y * scale, s.z * scale, s.w * scale);
         }
-        cluster.sync();
-    }
+    });
+    __syncthreads();
 
     // ---- out = base + B h over this CTA's chunks of 32 columns.  Column i of a chunk's j-th product is the chunk's column
     // (i / 2) * 8 + j * 2 + i % 2, so that a lane ends with eight consecutive columns of its two rows (f32: with columns
@@ -491,8 +509,8 @@ __global__ void __launch_bounds__(AdapterStage<XT, OT, T, RT>::THREADS, AdapterS
 #pragma unroll
     for (int s = 0; s < KS; s++) {
         const int k = RT == 2 ? q * 4 : s / 2 * 32 + q * 8 + s % 2 * 4;
-        const float4 v0 = *reinterpret_cast<const float4 *>(h + (row_base + g) * HS + k);
-        const float4 v1 = *reinterpret_cast<const float4 *>(h + (row_base + g + 8) * HS + k);
+        const float4 v0 = *reinterpret_cast<const float4 *>(h + g * HS + k);
+        const float4 v1 = *reinterpret_cast<const float4 *>(h + (g + 8) * HS + k);
         uint32_t w[4][HP];
         split_pair<HP>(v0.x, v0.y, w[0]);
         split_pair<HP>(v1.x, v1.y, w[1]);
@@ -503,62 +521,58 @@ __global__ void __launch_bounds__(AdapterStage<XT, OT, T, RT>::THREADS, AdapterS
 #pragma unroll
             for (int i = 0; i < 4; i++) hf[s][p][i] = w[i][p];
     }
-    OT *o0 = out + (has0 ? (size_t)t0 * P.N : 0) + (n0 + chunk0) * 32 + q * (16 / (int)sizeof(OT)), *o1 = out + (has1 ? (size_t)t1 * P.N : 0) + (n0 + chunk0) * 32 + q * (16 / (int)sizeof(OT));
+    OT *o0 = out + (has0 ? (size_t)t0 * P.N : 0) + (n0 + warp) * 32 + q * EO, *o1 = out + (has1 ? (size_t)t1 * P.N : 0) + (n0 + warp) * 32 + q * EO;
     for (int st = kstages; st < stages; st++) {
         landed();
-        const int ch0 = n0 + (st - kstages) * 4 + chunk0;
-        if (busy)
+        const int ch = n0 + (st - kstages) * 4 + warp;
+        float o[4][4] = {};
+        const uint8_t *wv = my_weights + buffer;
+        // the four products of a step are independent: in turn, so that none waits for its own sum
+        if constexpr (RT == 2) {
+            uint2 v[4];
 #pragma unroll
-            for (int u = 0; u < CPW; u++) {
-                float o[4][4] = {};
-                const uint8_t *wv = my_weights + buffer + u * (S::WEIGHTS / 4);
-                // the four products of a step are independent: in turn, so that none waits for its own sum
-                if constexpr (RT == 2) {
-                    uint2 v[4];
+            for (int j = 0; j < 4; j++) v[j] = reinterpret_cast<const uint2 *>(wv)[j * 32 + lane];
 #pragma unroll
-                    for (int j = 0; j < 4; j++) v[j] = reinterpret_cast<const uint2 *>(wv)[j * 32 + lane];
+            for (int p = 0; p < HP; p++)
 #pragma unroll
-                    for (int p = 0; p < HP; p++)
+                for (int j = 0; j < 4; j++) mma_bf16(o[j], hf[0][p][0], hf[0][p][1], hf[0][p][2], hf[0][p][3], v[j].x, v[j].y);
+        } else {
 #pragma unroll
-                        for (int j = 0; j < 4; j++) mma_bf16(o[j], hf[0][p][0], hf[0][p][1], hf[0][p][2], hf[0][p][3], v[j].x, v[j].y);
-                } else {
+            for (int s = 0; s < RT / 4; s++) {
+                uint4 v[4];
 #pragma unroll
-                    for (int s = 0; s < RT / 4; s++) {
-                        uint4 v[4];
+                for (int j = 0; j < 4; j++) v[j] = reinterpret_cast<const uint4 *>(wv)[(j * (RT / 4) + s) * 32 + lane];
 #pragma unroll
-                        for (int j = 0; j < 4; j++) v[j] = reinterpret_cast<const uint4 *>(wv)[(j * (RT / 4) + s) * 32 + lane];
+                for (int p = 0; p < HP; p++) {
 #pragma unroll
-                        for (int p = 0; p < HP; p++) {
+                    for (int j = 0; j < 4; j++)
+                        mma_bf16(o[j], hf[2 * s][p][0], hf[2 * s][p][1], hf[2 * s][p][2], hf[2 * s][p][3], v[j].x, v[j].y);
 #pragma unroll
-                            for (int j = 0; j < 4; j++)
-                                mma_bf16(o[j], hf[2 * s][p][0], hf[2 * s][p][1], hf[2 * s][p][2], hf[2 * s][p][3], v[j].x, v[j].y);
-#pragma unroll
-                            for (int j = 0; j < 4; j++)
-                                mma_bf16(o[j], hf[2 * s + 1][p][0], hf[2 * s + 1][p][1], hf[2 * s + 1][p][2], hf[2 * s + 1][p][3], v[j].z, v[j].w);
-                        }
-                    }
+                    for (int j = 0; j < 4; j++)
+                        mma_bf16(o[j], hf[2 * s + 1][p][0], hf[2 * s + 1][p][1], hf[2 * s + 1][p][2], hf[2 * s + 1][p][3], v[j].z, v[j].w);
                 }
-                constexpr int V = sizeof(OT) / 2, E = 8 / V;   // V groups of E consecutive columns
+            }
+        }
+        constexpr int V = sizeof(OT) / 2, E = 8 / V;   // V groups of E consecutive columns
 #pragma unroll
-                for (int half = 0; half < 2; half++)
+        for (int half = 0; half < 2; half++)
 #pragma unroll
-                    for (int v = 0; v < V; v++) {
-                        if (!(half ? has1 : has0) || ch0 + u >= n1 || (ch0 + u) * 32 + v * 16 + q * E >= P.N) continue;
-                        float y[E];
-                        load_units<E>(reinterpret_cast<const OT *>(my_rows + buffer + u * S::ROW_CHUNK + (half * V + v) * 512), y);
+            for (int v = 0; v < V; v++) {
+                if (!(half ? has1 : has0) || ch >= n1 || ch * 32 + v * 16 + q * E >= P.N) continue;
+                float y[E];
+                load_units<E>(reinterpret_cast<const OT *>(my_rows + buffer + (half * V + v) * 512), y);
 #pragma unroll
-                        for (int e = 0; e < E; e += 2) {
-                            y[e] += o[v * (E / 2) + e / 2][2 * half];
-                            y[e + 1] += o[v * (E / 2) + e / 2][2 * half + 1];
-                        }
-                        store_units<E>((half ? o1 : o0) + u * 32 + v * 16, y);
-                    }
+                for (int e = 0; e < E; e += 2) {
+                    y[e] += o[v * (E / 2) + e / 2][2 * half];
+                    y[e + 1] += o[v * (E / 2) + e / 2][2 * half + 1];
+                }
+                store_units<E>((half ? o1 : o0) + v * 16, y);
             }
         o0 += 128; o1 += 128;
         done_with(st);
     }
-    copy_bare_rows<THREADS>(P, share_id, base, out);
-    if (T == 16) cluster.sync();   // no CTA leaves while another reads its shares
+    copy_bare_rows<FEW_THREADS>(P, share_id, base, out);
+    cluster.sync();   // no CTA leaves while another reads its shares
 }
 
 // ---------------------------------------------------------------- many rows of an adapter: tcgen05
@@ -569,7 +583,7 @@ __global__ void __launch_bounds__(AdapterStage<XT, OT, T, RT>::THREADS, AdapterS
 //   h[128, r]     = X[128, K] A^T   stages of 64 of K: the rows' and A's pieces of 128 bytes, 128-byte swizzle
 //   out[128, 128] = H B^T + base    chunks of 128 columns, h as two bf16 pieces (16 bits of it; three for an
 //                                 f32 result, all of it), each its own product
-// with the cluster's exchange of h between them as above.  All threads copy (asynchronously, STAGES - 1 stages ahead), one
+// with the cluster's exchange of h between them as above.  All threads copy (asynchronously, LEAD stages ahead), one
 // issues the products, and a chunk's sums are read, added to base and stored while the next chunk's product runs.  The
 // columns of B lie permuted in shared memory so that a lane reads eight consecutive ones of a row.
 constexpr int TC_M = 128, TC_THREADS = 256;
@@ -620,7 +634,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_adapters_tc(AdapterArgs P, co
     pdl_wait();
     pdl_launch_dependents();
     const int share_id = id_of_share(P, 0);
-    find_tile<TC_M, TC_THREADS>(P, slot, rows, tile_id, tile_rows, tile_first);
+    if (P.order) find_tile<TC_M, TC_THREADS>(P, slot, rows, tile_id, tile_rows, tile_first);
+    else find_tile_by_ids<TC_M, TC_THREADS>(P, slot, rows, tile_id, tile_rows, tile_first, reinterpret_cast<int *>(smem));
     if (tile_rows == 0) {
         copy_bare_rows<TC_THREADS>(P, share_id, base, out);
         return;
@@ -909,10 +924,12 @@ static int64_t tiles_of(const AdapterArgs &P, int T) { return min((int64_t)P.n, 
 template <typename XT, typename OT, int RT>
 static cudaError_t launch_adapters_as(const AdapterArgs &P, const XT *x, const OT *base, OT *out, cudaStream_t s)
 {
-    using S = AdapterStage<XT, OT, 16, RT>;
-    const int64_t room = 148 * (int64_t)max(1, min(2 * S::MIN_CTAS, (int)(227 * 1024 / (S::SMEM + 6144))));
-    const int ctas = cluster_size(P.order ? tiles_of(P, 16) : min(P.n, P.L), room, 8.0, (P.K + P.N) / 128.0);   // in stages
-    return launch_clusters(k_adapters<XT, OT, 16, RT>, P.order ? P.n / 16 + P.L : P.n, ctas, S::THREADS, S::SMEM, P, x, base, out, s);
+    using S = AdapterStage<XT, OT, RT>;
+    static_assert(S::STAGES * S::BYTES >= (ADAPTER_MAX + 1) * 4, "room for the offsets");
+    const bool slots_by_id = P.order || P.n > ADAPTER_ROWS_LEADER;   // else every row is a slot
+    const int64_t room = 148 * (int64_t)max(1, min(8, (int)(227 * 1024 / (S::SMEM + 6144))));
+    const int ctas = cluster_size(slots_by_id ? tiles_of(P, FEW_M) : min(P.n, P.L), room, 8.0, (P.K + P.N) / 128.0);   // in stages
+    return launch_clusters(k_adapters<XT, OT, RT>, slots_by_id ? P.n / FEW_M + P.L : P.n, ctas, FEW_THREADS, S::SMEM, P, x, base, out, s);
 }
 
 template <typename OT, int RT>
@@ -925,7 +942,7 @@ static cudaError_t launch_adapters_tc(const AdapterArgs &P, const __nv_bfloat16 
 cudaError_t launch_adapters(const void *base, int out_dtype, const void *x, int x_dtype, const AdapterArgs &P, void *out, cudaStream_t s)
 {
     // tiles of 128 rows where an adapter has enough of them and the rows are the tensor cores' own type; else of 16
-    const bool wide = P.order && P.n / P.L >= TC_MIN_ROWS && x_dtype == PMOE_BF16;
+    const bool wide = P.n > ADAPTER_ROWS_LEADER && P.n / P.L >= TC_MIN_ROWS && x_dtype == PMOE_BF16;
     return with_type(out_dtype, [&](auto *op) {
         using OT = std::remove_pointer_t<decltype(op)>;
         const OT *bb = (const OT *)base;
@@ -956,7 +973,8 @@ extern "C" int pmoe_adapters_add(int device, const void *base, const void *x, in
                                  const void *a, const void *b, const float *scales, const int *ids, const int *order, const int *offsets,
                                  void *out, int out_dtype, void *stream)
 {
-    if (n < 0 || n > (1 << 30) || n_adapters <= 0 || n_adapters > 4096) return fail(PMOE_ERR_INVALID_ARG, "bad n / n_adapters (1 to 4096)");
+    if (n < 0 || n > (1 << 30) || n_adapters <= 0 || n_adapters > ADAPTER_MAX)
+        return fail(PMOE_ERR_INVALID_ARG, "bad n / n_adapters (1 to %d)", ADAPTER_MAX);
     if (K <= 0 || K % 8 || N <= 0 || N % 8 || K > (1 << 20) || N > (1 << 20))
         return fail(PMOE_ERR_UNSUPPORTED_SHAPE, "K and N must be multiples of 8 up to 2^20 (got %d, %d)", K, N);
     if (rank <= 0 || rank % 8 || rank > ADAPTER_MAX_RANK)

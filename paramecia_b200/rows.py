@@ -261,10 +261,8 @@ def add_rms_norm_q8(resid: torch.Tensor, delta: Optional[torch.Tensor], weight: 
     return new_resid, q, scales, values
 
 
-# Rows up to which pmoe_adapters_add groups the ids itself (it could up to 1024): every row then asks for a cluster of CTAs, most
-# of which find that another row leads their tile.  Rank 16 / 64 of 2048 x 2048: 8.2 / 14 us with 128 rows against 11 / 14 us
-# with the sort, 25 / 48 against 14 / 17 us with 512.
-_ADAPTER_ROWS_UNSORTED = 128
+# rows up to which pmoe_adapters_add groups the ids itself
+_ADAPTER_ROWS_UNSORTED = 1024
 
 
 def adapters_add(base: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, ids: torch.Tensor,
@@ -275,8 +273,8 @@ def adapters_add(base: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.
 
     base [n, N] and x [n, K] f32 or bf16; a [L, r, K] and b [L, N, r] bf16, r a multiple of 8 up to 128 (pad a smaller one with
     zeros), K and N multiples of 8; ids [n] int32, a row whose id is outside [0, L) keeps base; scales [L] f32 (None: ones).
-    ``order`` = sort_by_expert(ids, L), worth keeping when several projections share the ids; made here from 129 rows on
-    when it is not given.  ``out``: the tensor to fill (base itself for in place).  An operator for inference."""
+    ``order`` = sort_by_expert(ids, L), worth keeping when several projections share the ids; made here from 1025
+    rows on when it is not given.  ``out``: the tensor to fill (base itself for in place).  An operator for inference."""
     device = _on_gpu("x", x)
     xd, od = _typed("x", x, device), _typed("base", base, device)
     for name, t in (("a", a), ("b", b)):
