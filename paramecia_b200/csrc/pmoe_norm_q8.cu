@@ -25,22 +25,26 @@ __device__ inline float max_abs(float m, float v)
 
 // How a group becomes 8 bits.  With u = r * weight and top = max |u| over the group, v = u / m and
 //   scale = max |v| / 127 = top * (1 / m) / 127,   v / scale = u * (127 / top):
-// the quotient needs neither m nor the rounded scale, which saves two products an element, lets both statistics be
-// reduced at once, and takes three roundings where dividing v by its scale takes five (each moves values over a border
-// of the 8-bit numbers).
+// the quotient needs neither m nor the rounded scale, which saves two products an element and lets both statistics be
+// reduced at once.  For int8 it is taken in f32 (u, top, 127 / top: three roundings, where dividing v by its scale takes five).
+// The 8-bit floats are what a consumer multiplies as they are, so there q is the rounding of the exact quotient: every
+// value is rounded twice, from a quotient that is certainly too small and one that is certainly too large, and where the
+// two differ, as for one value in 10^5, the group is done again in 64 bits from the row as it was stored.
+constexpr float BELOW = 1.f - 0x1.6p-22f, ABOVE = 1.f + 0x1.6p-22f;   // five roundings of 2^-24 and a little
+
 struct GroupScale {
-    float scale, inverse, top;
-    bool plain;    // the product with `inverse` is the quotient, and in the type's range up to what the rounding takes back
+    float scale, top;
+    bool plain;    // scale is a number above 0, and `most / top` does not overflow
     template <bool E4M3> __device__ static GroupScale of(float top, float inv_m)
     {
         GroupScale g;
         g.scale = __fdiv_rn(top * inv_m, E4M3 ? 448.f : 127.f);
         g.top = top;
         g.plain = top >= 0x1p-100f && g.scale > 0.f && g.scale < INFINITY;
-        g.inverse = __fdiv_rn(E4M3 ? 448.f : 127.f, top);
         return g;
     }
-    // v / scale for the other groups: 0 where the scale is 0, infinite or NaN, else without the inverse, which may overflow
+    template <bool E4M3> __device__ float inverse() const { return __fdiv_rn(E4M3 ? 448.f : 127.f, top); }
+    // u * (127 / top) for the other groups: 0 where the scale is 0, infinite or NaN
     template <bool E4M3> __device__ float ratio(float u) const
     {
         return scale > 0.f && scale < INFINITY ? __fdiv_rn(u, top) * (E4M3 ? 448.f : 127.f) : 0.f;
@@ -50,35 +54,46 @@ struct GroupScale {
 // 1 / sqrt(mean + eps); of 0 it is infinite and of an infinity 0, so that u * inv_m is u / m there too
 __device__ inline float inverse_rms(float ss, int H, float eps) { return __frcp_rn(sqrtf(ss / (float)H + eps)); }
 
-// Ratios to 8 bits (the bytes of `packed`, in order) and, with HELD, back to what they stand for in units of the scale.
-template <bool E4M3, bool HELD, int N> __device__ inline void to_8bit(float (&r)[N], uint32_t *packed)
+// N numbers u[i] * f to 8 bits, the bytes of `packed` in order.  N is 1 or a multiple of 4.
+template <bool E4M3, int N> __device__ inline void to_8bit(const float (&u)[N], float f, uint32_t *packed)
 {
     if constexpr (E4M3) {
 #pragma unroll
         for (int i = 0; i < N; i += 2) {
-            const __nv_fp8x2_storage_t b = __nv_cvt_float2_to_fp8x2(make_float2(r[i], i + 1 < N ? r[i + 1] : 0.f), __NV_SATFINITE, __NV_E4M3);
-            if (HELD) {
-                const float2 f = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(b, __NV_E4M3)));
-                r[i] = f.x;
-                if (i + 1 < N) r[i + 1] = f.y;
-            }
-            if (i % 4 == 0) packed[i / 4] = b;
+            const __nv_fp8x2_storage_t b = __nv_cvt_float2_to_fp8x2(make_float2(u[i] * f, i + 1 < N ? u[i + 1] * f : 0.f), __NV_SATFINITE, __NV_E4M3);
+            if (i % 4 == 0) packed[i / 4] = N == 1 ? b & 0xff : b;
             else packed[i / 4] |= (uint32_t)b << 16;
         }
     } else {
-        // 1.5 * 2^23 + r rounds r to the nearest integer, ties to even, and its low byte is that integer's
-        constexpr float MAGIC = 12582912.f;
+        // 1.5 * 2^23 + x rounds x to the nearest integer, ties to even, and its low byte is that integer's
         uint32_t t[N];
 #pragma unroll
-        for (int i = 0; i < N; i++) {
-            const float f = r[i] + MAGIC;
-            t[i] = __float_as_uint(f);
-            if (HELD) r[i] = f - MAGIC;
-        }
+        for (int i = 0; i < N; i++) t[i] = __float_as_uint(fmaf(u[i], f, 12582912.f));
         if constexpr (N == 1) packed[0] = t[0] & 0xff;
         else
 #pragma unroll
             for (int i = 0; i < N; i += 4) packed[i / 4] = __byte_perm(__byte_perm(t[i], t[i + 1], 0x0040), __byte_perm(t[i + 2], t[i + 3], 0x0040), 0x5410);
+    }
+}
+
+// the exact quotient of d by the group's largest magnitude, as an 8-bit float
+__device__ inline uint32_t to_e4m3_exact(double d, double top)
+{
+    return (uint32_t)__nv_cvt_float_to_fp8((float)(d * 448.0 / top), __NV_SATFINITE, __NV_E4M3);
+}
+
+// What four bytes stand for in units of the scale
+template <bool E4M3> __device__ inline void held4(uint32_t packed, float *y)
+{
+    if constexpr (E4M3) {
+        const float2 a = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)packed, __NV_E4M3)));
+        const float2 b = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(packed >> 16), __NV_E4M3)));
+        y[0] = a.x; y[1] = a.y; y[2] = b.x; y[3] = b.y;
+    } else {
+        // byte + 128 as the low byte of 2^23
+        const uint32_t t = packed ^ 0x80808080u;
+#pragma unroll
+        for (int i = 0; i < 4; i++) y[i] = __uint_as_float(__byte_perm(t, 0x4b000000u, 0x7650 | i)) - 8388736.f;
     }
 }
 
@@ -105,10 +120,12 @@ __device__ inline void add_and_store(float (&v)[8], const float (&d)[8], __nv_bf
 // bf16 + bf16 -> bf16, e4m3), so memory bounds it and the row must stay on the chip between its two statistics: here in
 // registers, eight consecutive elements a thread and pass, a row never longer than threads * PASSES * 8.  A group is 4, 8, 16
 // or 32 neighbouring threads of a pass (its maximum by shuffles) or the whole row (shuffles and a shared array).  The second
-// limit is the issue rate: with two quotients an element 16384 rows of 2048 took 126 us.  Now 46 us, 0.79 of the
-// measured copy rate (sixteen elements a thread and half the threads: 50 us).
-template <typename RT, typename DT, typename VT, bool E4M3, int PASSES>
-__global__ void __launch_bounds__(1024) k_norm_q8(const RT *resid_in, const DT *__restrict__ delta, const float *__restrict__ weight, int H,
+// limit is the issue rate: with two quotients an element 16384 rows of 2048 took 126 us.  Now 51 us, 0.72 of the
+// measured copy rate.
+// THREADS: the most a launch has.  With one pass the registers are held to what fills an SM (2048 threads): the part in 64 bits wants
+// twice as many, and with them 16384 rows took 60 us for 51.
+template <typename RT, typename DT, typename VT, bool E4M3, int PASSES, int THREADS>
+__global__ void __launch_bounds__(THREADS, PASSES == 1 ? 2048 / THREADS : 1) k_norm_q8(const RT *resid_in, const DT *__restrict__ delta, const float *__restrict__ weight, int H,
                                                   float eps, int group, RT *resid_out, uint8_t *__restrict__ q,
                                                   float *__restrict__ scales, VT *__restrict__ values)
 {
@@ -184,29 +201,108 @@ __global__ void __launch_bounds__(1024) k_norm_q8(const RT *resid_in, const DT *
         if (G == 1) row_top = max_abs(row_top, __shfl_xor_sync(0xffffffffu, row_top, s));
     }
     const float inv_m = inverse_rms(ss, H, eps);
+    bool border[PASSES];
 #pragma unroll
     for (int p = 0; p < PASSES; p++) {
         const int h = (p * blockDim.x + tid) * 8;
+        border[p] = false;
         if (h >= H) continue;
         const GroupScale gs = GroupScale::of<E4M3>(G == 1 ? row_top : top[p], inv_m);
         if (G == 1 ? h == 0 : (h & (group - 1)) == 0) row_scales[G == 1 ? 0 : h >> log2_group] = gs.scale;
+        uint32_t packed[2];
         if (gs.plain) {
-#pragma unroll
-            for (int i = 0; i < 8; i++) v[p][i] *= gs.inverse;
+            const float inverse = gs.inverse<E4M3>();
+            to_8bit<E4M3>(v[p], E4M3 ? inverse * BELOW : inverse, packed);
+            if constexpr (E4M3) {
+                uint32_t above[2];
+                to_8bit<E4M3>(v[p], inverse * ABOVE, above);
+                border[p] = packed[0] != above[0] || packed[1] != above[1];
+            }
         } else {
 #pragma unroll
             for (int i = 0; i < 8; i++) v[p][i] = gs.ratio<E4M3>(v[p][i]);
-        }
-        uint32_t packed[2];
-        if (values) {
-            to_8bit<E4M3, true>(v[p], packed);
-#pragma unroll
-            for (int i = 0; i < 8; i++) v[p][i] *= gs.scale;   // NaN where the scale is not finite: 0 * inf
-            store_units<8>(values + base + h, v[p]);
-        } else {
-            to_8bit<E4M3, false>(v[p], packed);
+            to_8bit<E4M3>(v[p], 1.f, packed);
         }
         *reinterpret_cast<uint2 *>(q + base + h) = make_uint2(packed[0], packed[1]);
+        if (values) {
+            float y[8];
+            held4<E4M3>(packed[0], y);
+            held4<E4M3>(packed[1], y + 4);
+#pragma unroll
+            for (int i = 0; i < 8; i++) y[i] *= gs.scale;   // NaN where the scale is not finite: 0 * inf
+            store_units<8>(values + base + h, y);
+        }
+    }
+    if constexpr (E4M3) {
+        bool any = false;
+#pragma unroll
+        for (int p = 0; p < PASSES; p++) any |= border[p];
+        if (G == 1 ? !__syncthreads_or(any) : !__any_sync(0xffffffffu, any)) return;
+        __shared__ double red_exact[32];
+        double d[8], t = 0;
+        // the exact products of a pass; the stored residual is what was normalised
+        auto products = [&](int p) {
+            const int h = (p * blockDim.x + tid) * 8;
+#pragma unroll
+            for (int i = 0; i < 8; i++) d[i] = 0;
+            if (h < H) {
+                float r[8], w[8], a[8];
+                load_units<8>((resid_out ? resid_out : resid_in) + base + h, r);
+                if (weight) load_units<8>(weight + h, w);
+                if (delta && !resid_out) {
+                    load_units<8>(delta + base + h, a);
+                    add_and_store(r, a, (RT *)nullptr);
+                }
+#pragma unroll
+                for (int i = 0; i < 8; i++) d[i] = weight ? (double)r[i] * (double)w[i] : (double)r[i];
+            }
+            double most = 0;
+#pragma unroll
+            for (int i = 0; i < 8; i++) most = fmax(most, fabs(d[i]));
+            return most;
+        };
+        auto store = [&](int p) {
+            const int h = (p * blockDim.x + tid) * 8;
+            const GroupScale gs = GroupScale::of<E4M3>((float)t, inv_m);   // rounding keeps the order: t's rounding is `top`
+            if (h >= H || !gs.plain) return;
+            uint32_t packed[2] = {0u, 0u};
+#pragma unroll
+            for (int i = 0; i < 8; i++) packed[i / 4] |= to_e4m3_exact(d[i], t) << (8 * (i & 3));
+            *reinterpret_cast<uint2 *>(q + base + h) = make_uint2(packed[0], packed[1]);
+            if (values) {
+                float y[8];
+                held4<E4M3>(packed[0], y);
+                held4<E4M3>(packed[1], y + 4);
+#pragma unroll
+                for (int i = 0; i < 8; i++) y[i] *= gs.scale;
+                store_units<8>(values + base + h, y);
+            }
+        };
+        if (G > 1) {
+#pragma unroll 1
+            for (int p = 0; p < PASSES; p++) {
+                t = products(p);
+#pragma unroll
+                for (int s = 1; s < 32; s <<= 1)
+                    if (s * 8 < group) t = fmax(t, __shfl_xor_sync(0xffffffffu, t, s));
+                store(p);
+            }
+        } else {
+#pragma unroll 1
+            for (int p = 0; p < PASSES; p++) t = fmax(t, products(p));
+#pragma unroll
+            for (int s = 16; s >= 1; s >>= 1) t = fmax(t, __shfl_xor_sync(0xffffffffu, t, s));
+            if (lane == 0) red_exact[warp] = t;
+            __syncthreads();
+            t = lane < warps ? red_exact[lane] : 0.0;
+#pragma unroll
+            for (int s = 16; s >= 1; s >>= 1) t = fmax(t, __shfl_xor_sync(0xffffffffu, t, s));
+#pragma unroll 1
+            for (int p = 0; p < PASSES; p++) {
+                if (PASSES > 1) products(p);
+                store(p);
+            }
+        }
     }
 }
 
@@ -272,6 +368,7 @@ __global__ void __launch_bounds__(1024) k_norm_q8_any(const RT *resid_in, const 
         if (G == 1) row_top = max_abs(row_top, __shfl_xor_sync(0xffffffffu, row_top, s));
     }
     const float inv_m = inverse_rms(ss, H, eps);
+    bool border = false;
 #pragma unroll
     for (int p = 0; p < PASSES; p++) {
         const int h0 = (p * warps + warp) * 256 + lane;
@@ -286,6 +383,7 @@ __global__ void __launch_bounds__(1024) k_norm_q8_any(const RT *resid_in, const 
 #pragma unroll
                     for (int i = 0; i < 8; i += 2 * s) top[i] = max_abs(top[i], top[i + s]);
         GroupScale gs = GroupScale::of<E4M3>(row_top, inv_m);
+        float inverse = gs.inverse<E4M3>();
         if (G == 1 && h0 == 0) row_scales[0] = gs.scale;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
@@ -294,14 +392,70 @@ __global__ void __launch_bounds__(1024) k_norm_q8_any(const RT *resid_in, const 
 #pragma unroll
                 for (int s = 16; s >= 1; s >>= 1) top[i] = max_abs(top[i], __shfl_xor_sync(0xffffffffu, top[i], s));
                 gs = GroupScale::of<E4M3>(top[i], inv_m);
+                inverse = gs.inverse<E4M3>();
                 if (lane == 0 && h < H) row_scales[h >> log2_group] = gs.scale;
             }
             if (h >= H) continue;
-            float r[1] = {gs.plain ? v[p][i] * gs.inverse : gs.ratio<E4M3>(v[p][i])};
-            uint32_t b;
-            to_8bit<E4M3, true>(r, &b);
+            const float x[1] = {gs.plain ? v[p][i] : gs.ratio<E4M3>(v[p][i])};
+            uint32_t low;
+            to_8bit<E4M3>(x, !gs.plain ? 1.f : E4M3 ? inverse * BELOW : inverse, &low);
+            if constexpr (E4M3) {
+                uint32_t high;
+                to_8bit<E4M3>(x, gs.plain ? inverse * ABOVE : 1.f, &high);
+                border |= low != high;
+            }
+            q[h] = (uint8_t)low;
+            if (values) {
+                float y[4];
+                held4<E4M3>(low, y);
+                store_from_float(values, h, y[0] * gs.scale);
+            }
+        }
+    }
+    if constexpr (E4M3) {
+        if (G == 1 ? !__syncthreads_or(border) : !__any_sync(0xffffffffu, border)) return;
+        __shared__ double red_exact[32];
+        auto product = [&](int h) {   // exact; the stored residual is what was normalised
+            if (h >= H) return 0.0;
+            RT r;
+            store_from_float(&r, 0, resid_out ? load_as_float(resid_out, h) : load_as_float(resid_in, h) + (delta ? load_as_float(delta, h) : 0.f));
+            return (double)load_as_float(&r, 0) * (weight ? (double)weight[h] : 1.0);
+        };
+        auto store = [&](int h, double t) {
+            const GroupScale gs = GroupScale::of<E4M3>((float)t, inv_m);
+            if (h >= H || !gs.plain) return;
+            const uint32_t b = to_e4m3_exact(product(h), t);
             q[h] = (uint8_t)b;
-            if (values) store_from_float(values, h, r[0] * gs.scale);
+            if (values) {
+                float y[4];
+                held4<E4M3>(b, y);
+                store_from_float(values, h, y[0] * gs.scale);
+            }
+        };
+        if (G > 1) {
+            for (int p = 0; p < PASSES; p++)
+                for (int i0 = 0; i0 < 256; i0 += group) {
+                    const int h0 = (p * warps + warp) * 256 + i0 + lane;
+                    double t = 0;
+                    for (int k = 0; k < group; k += 32) t = fmax(t, fabs(product(h0 + k)));
+#pragma unroll
+                    for (int s = 16; s >= 1; s >>= 1) t = fmax(t, __shfl_xor_sync(0xffffffffu, t, s));
+                    for (int k = 0; k < group; k += 32) store(h0 + k, t);
+                }
+        } else {
+            // over the elements that this thread wrote: no other thread touches their bytes
+            double t = 0;
+            for (int p = 0; p < PASSES; p++)
+                for (int i = 0; i < 256; i += 32) t = fmax(t, fabs(product((p * warps + warp) * 256 + i + lane)));
+#pragma unroll
+            for (int s = 16; s >= 1; s >>= 1) t = fmax(t, __shfl_xor_sync(0xffffffffu, t, s));
+            if (lane == 0) red_exact[warp] = t;
+            __syncthreads();
+            t = lane < warps ? red_exact[lane] : 0.0;
+#pragma unroll
+            for (int s = 16; s >= 1; s >>= 1) t = fmax(t, __shfl_xor_sync(0xffffffffu, t, s));
+            for (int p = 0; p < PASSES; p++)
+                for (int i = 0; i < 256; i += 32) store((p * warps + warp) * 256 + i + lane, t);
         }
     }
 }
@@ -327,8 +481,9 @@ cudaError_t launch_norm_q8(const void *resid_in, int resid_dtype, const void *de
                 };
                 const bool f8 = q_dtype == PMOE_F8_E4M3;
                 if (wide)
-                    return passes == 1 ? go(f8 ? k_norm_q8<RT, DT, VT, true, 1> : k_norm_q8<RT, DT, VT, false, 1>, threads)
-                                       : go(f8 ? k_norm_q8<RT, DT, VT, true, 2> : k_norm_q8<RT, DT, VT, false, 2>, threads);
+                    return threads <= 256 ? go(f8 ? k_norm_q8<RT, DT, VT, true, 1, 256> : k_norm_q8<RT, DT, VT, false, 1, 256>, threads)
+                           : passes == 1  ? go(f8 ? k_norm_q8<RT, DT, VT, true, 1, 1024> : k_norm_q8<RT, DT, VT, false, 1, 1024>, threads)
+                                          : go(f8 ? k_norm_q8<RT, DT, VT, true, 2, 1024> : k_norm_q8<RT, DT, VT, false, 2, 1024>, threads);
                 return go(f8 ? k_norm_q8_any<RT, DT, VT, true> : k_norm_q8_any<RT, DT, VT, false>, min(1024, (H + 255) / 256 * 32));
             });
         });

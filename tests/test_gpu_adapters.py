@@ -63,7 +63,7 @@ def check(base, x, a, b, ids, scales, got):
 SHAPES = [(1, 2048, 2048, 16, 8, "one"), (1, 64, 64, 8, 1, "none"), (2, 2048, 512, 64, 3, "mixed"), (17, 1000, 504, 24, 5, "mixed"),
           (64, 2048, 4096, 32, 48, "mixed"), (100, 512, 2048, 128, 2, "one"), (333, 264, 520, 40, 300, "mixed"), (5, 8, 8, 8, 2, "mixed"),
           (1024, 512, 512, 16, 7, "runs"), (1025, 512, 520, 16, 7, "mixed"), (3001, 512, 1024, 64, 4, "runs"), (2000, 256, 256, 8, 4000, "mixed"),
-          (5000, 128, 264, 112, 3, "one"), (1500, 520, 64, 56, 9, "none"), (129, 4096, 72, 120, 1, "one")]
+          (5000, 128, 264, 112, 3, "one"), (2000, 264, 136, 32, 5, "mixed"), (700, 8, 8, 8, 1, "one"), (1030, 72, 1000, 16, 8, "runs"), (130, 1024, 1024, 64, 1, "mixed"), (1500, 520, 64, 56, 9, "none"), (129, 4096, 72, 120, 1, "one")]
 
 
 @pytest.mark.parametrize("xt, bt", [(f32, f32), (bf16, bf16), (f32, bf16), (bf16, f32)])
@@ -103,6 +103,26 @@ def test_other_rows_are_not_touched_by_a_bad_one():
     same = (ids != 3) & (torch.arange(40, device=DEV) != 7) & (torch.arange(40, device=DEV) != 9)
     assert torch.equal(got[same], want[same])
     assert torch.isnan(got[7]).all() and torch.isnan(got[ids == 3]).all() and not torch.isfinite(got[9]).any()
+
+
+@pytest.mark.parametrize("n, L, xt", [(90, 5, f32), (500, 3, bf16), (500, 200, bf16), (1024, 2, f32), (3000, 4, bf16)])
+def test_with_and_without_the_order_and_twice(n, L, xt):
+    """Grouped by the sort, by the kernel itself, and once more on another stream: the same rows meet in the same tiles, so the
+    bits are equal wherever the tiles are."""
+    base, x, a, b, ids, scales = make(n, 512, 264, 48, L, xt, f32, n + L)
+    order = pm.sort_by_expert(ids, L)
+    first = pm.adapters_add(base, x, a, b, ids, scales=scales, order=order)
+    again = pm.adapters_add(base, x, a, b, ids, scales=scales, order=order)
+    assert torch.equal(first, again)
+    check(base, x, a, b, ids, scales, first)
+    check(base, x, a, b, ids, scales, pm.adapters_add(base, x, a, b, ids, scales=scales))
+    side = torch.cuda.Stream(DEV)
+    side.wait_stream(torch.cuda.current_stream(DEV))
+    with torch.cuda.stream(side):
+        other = pm.adapters_add(base, x, a, b, ids, scales=scales, order=order)
+    side.synchronize()
+    assert torch.equal(first, other)
+    pm.rows_status(DEV)
 
 
 def test_no_rows_and_long_rows():

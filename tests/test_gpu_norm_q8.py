@@ -55,6 +55,24 @@ def check(resid, delta, weight, group, q_dtype, values_dtype, eps=1e-6):
         assert torch.equal(values, (q.float() * per.float()).to(values_dtype))
 
 
+@pytest.mark.parametrize("group", [0, 32, 128])
+@pytest.mark.parametrize("n, H, rt", [(400, 2048, f32), (300, 1003, bf16), (50, 9000, f32), (64, 12288, bf16), (333, 520, bf16)])
+def test_8_bit_floats_are_the_rounding_of_the_exact_quotient(n, H, rt, group):
+    """Products of two f32 numbers are exact in 64 bits, and one more product and quotient are off by 2^-52: no value of
+    these rows lies as near to a border of e4m3, so every byte has to be equal."""
+    resid, delta, weight = make(n, H, rt, bf16, H)
+    weight[:7] = 1.0
+    resid[1] = torch.arange(H, device=DEV).to(rt) % 31 - 15          # with delta 0: exact ties among the quotients
+    delta[1] = 0
+    for w in (weight, None):
+        new, q, scales, _ = pm.add_rms_norm_q8(resid, delta, w, 1e-6, group=group, q_dtype=torch.float8_e4m3fn)
+        d = new.double() * (1.0 if w is None else w.double())
+        g = group or H
+        pad = torch.nn.functional.pad(d, (0, -H % g)).view(n, -1, g)
+        want = (pad * 448 / pad.abs().amax(2, keepdim=True).clamp(min=1e-300)).view(n, -1)[:, :H]
+        assert torch.equal(q.float(), want.float().to(torch.float8_e4m3fn).float())
+
+
 def make(n, H, rt, dt, seed):
     g = torch.Generator(device=DEV)
     g.manual_seed(seed)

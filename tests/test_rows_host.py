@@ -98,5 +98,7 @@ def test_host_tensors_are_refused():
         with pytest.raises(pm.PmoeError) as e:
             f()
         assert e.value.code == -9
+    with pytest.raises(pm.PmoeError):
+        pm.rows_status("cpu")
     with pytest.raises(ValueError):
         pm.sort_by_expert([1, 2], 4)
