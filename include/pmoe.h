@@ -357,8 +357,8 @@ int pmoe_combine_rows_grad(int device, const void *grad_out, int grad_dtype, con
 /*
  * Low-rank adapters of many requests beside one projection (the low-rank update of QMatMul, models/with_tracing.rs:103-337,
  * which the reference holds once and merges): out[t] = base[t] + scales[i] * B_i (A_i x[t]), i = ids[t]; a row whose id is
- * outside [0, n_adapters) gets base[t].  x [n, K] and base, out [n, N] F32 or BF16 (base and out alike; out may be base);
- * a [n_adapters, rank, K] and b [n_adapters, N, rank] BF16; scales [n_adapters] f32 or NULL (all ones); ids [n] int32.
+ * outside [0, n_adapters) gets base[t].  x [n, K] and base, out [n, N] F32 or BF16 (base and out alike; out may be base, and
+ * must not overlap x); a [n_adapters, rank, K] and b [n_adapters, N, rank] BF16; scales [n_adapters] f32 or NULL (all ones); ids [n] int32.
  * order and offsets: pmoe_sort_pairs of ids (top_k 1, expert_base 0, E = n_adapters), which a host computes once for all
  * projections of a batch, or both NULL for n <= 1024.  K and N multiples of 8, rank a multiple of 8 up to 128, all
  * pointers 16-byte aligned.  Products are exact bf16 products summed in f32; f32 rows lose nothing.

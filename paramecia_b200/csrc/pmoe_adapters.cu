@@ -260,8 +260,8 @@ __device__ inline void find_tile_by_ids(const AdapterArgs &P, int slot, int *row
 // A CTA of four warps walks its share of K and then its share of N in stages of four chunks of 32, a chunk a warp: a stage
 // holds what the matrix instructions of a chunk need, as the lanes need it (sixteen bytes per lane, lanes side by side, so no
 // access meets a bank twice), and a warp reads what its own lanes fetched.  The copies are asynchronous and STAGES stages are on
-// their way, the first ones of N while the shares of h are still being added: one decoding row of 2048 x 2048 takes 5.2 us, 64
-// rows with 36 adapters of rank 32 (2048 to 4096) 11 us, which is the chain id -> rows -> h -> exchange -> columns.
+// their way, the first ones of N while the shares of h are still being added: one decoding row of 2048 x 2048 takes 5 us, 64
+// rows with 36 adapters of rank 32 (2048 to 4096) 9.7 us, which is the chain id -> rows -> h -> exchange -> columns.
 // RT: groups of eight ranks that the accumulators are sized for.
 constexpr int FEW_M = 16, FEW_THREADS = 128;
 

@@ -13,7 +13,8 @@ per-expert adapters, a training step); ``MoeBlock`` does all of it inside its ke
     ...                                             # back through the experts: grad_rows -> grad_xs
     grad_x = dispatch_rows_grad(grad_xs, order)
 
-Nothing here waits for the GPU or reads a count back: sizes depend on the shapes alone.
+Nothing here waits for the GPU or reads a count back: sizes depend on the shapes alone.  These are plain functions on device
+memory, as everything in this package is: autograd does not record them, and the gradients are the ones above.
 """
 from __future__ import annotations
 
@@ -68,6 +69,16 @@ def _ids(what: str, t: torch.Tensor) -> torch.Tensor:
     if t.dtype == torch.int64:
         return t.clamp(-1, 2 ** 31 - 1).to(torch.int32)
     raise PmoeError(-2, f"{what} must be int32 or int64, got {t.dtype}")
+
+
+def _apart(what: str, out: torch.Tensor, t: Optional[torch.Tensor], same: bool = False) -> None:
+    """Refuses an `out` that lies over an input whose elements other rows still need; `same`: it may be the input itself."""
+    if t is None:
+        return
+    a, b = out.data_ptr(), t.data_ptr()
+    if a < b + t.numel() * t.element_size() and b < a + out.numel() * out.element_size():
+        if not (same and a == b and out.dtype == t.dtype):
+            raise ValueError(f"out must not overlap {what}")
 
 
 class ExpertOrder:
@@ -142,6 +153,7 @@ def dispatch_rows(x: torch.Tensor, order: ExpertOrder, out: Optional[torch.Tenso
         out = torch.empty(*rows, dtype=x.dtype, device=device)
     else:
         _check_buffer("out", out, rows, x.dtype, device)
+        _apart("x", out, x)
     if x.shape[1] == 0:
         return out
     check(lib().pmoe_dispatch_rows(device.index, x.data_ptr(), x.shape[1] * x.element_size(), order.n, order.top_k, order._place,
@@ -184,6 +196,8 @@ def combine_rows(rows: torch.Tensor, order: ExpertOrder, weights: Optional[torch
         od = _out_type("out_dtype", out.dtype)
     else:
         _check_buffer("out", out, shape, tuple(_TYPES), device)
+        _apart("rows", out, rows)
+        _apart("extra", out, e, same=True)
         od = _TYPES[out.dtype]
     check(lib().pmoe_combine_rows(device.index, rows.data_ptr(), rd, rows.shape[0], order.n, order.top_k, rows.shape[1], order._place,
                                   None if w is None else w.data_ptr(), None if e is None else e.data_ptr(),
@@ -313,6 +327,8 @@ def adapters_add(base: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.
         if out.data_ptr() % 16:
             raise ValueError("out must be 16-byte aligned")
         base = _aligned(base)
+        _apart("x", out, x)
+        _apart("base", out, base, same=True)
     check(lib().pmoe_adapters_add(device.index, base.data_ptr(), x.data_ptr(), xd, n, K, N, r, L, a.data_ptr(), b.data_ptr(),
                                   None if s is None else s.data_ptr(), ids.data_ptr(), None if order is None else order._order,
                                   None if order is None else order._offsets, out.data_ptr(), od, _stream(device.index)))

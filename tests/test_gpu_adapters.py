@@ -157,6 +157,7 @@ def test_refusals():
               lambda: pm.adapters_add(base, x, a, b[:2], ids), lambda: pm.adapters_add(base, x, a[0], b, ids),
               lambda: pm.adapters_add(base, x, a, b, ids[:2]), lambda: pm.adapters_add(base, x, a, b, ids.cpu()),
               lambda: pm.adapters_add(base, x, a, b, ids, scales=scales[:2]), lambda: pm.adapters_add(base, x, a, b, ids, order=order),
+              lambda: pm.adapters_add(base, x, a, b, ids, out=x), lambda: pm.adapters_add(base[:3], x[:3], a, b, ids[:3], out=base[1:]),
               lambda: pm.adapters_add(base, x, a, b, ids, out=base.bfloat16()), lambda: pm.adapters_add(base, x, a, b, ids, out=x[:2])):
         with pytest.raises(ValueError):
             f()

@@ -272,6 +272,8 @@ def test_refusals():
            lambda: pm.dispatch_rows(x, o, out=rows[:7]), lambda: pm.dispatch_rows(x, o, out=rows.bfloat16()),
            lambda: pm.combine_rows(x, o), lambda: pm.combine_rows(rows, o, w[:3]), lambda: pm.combine_rows(rows, o, w.cpu()),
            lambda: pm.combine_rows(rows, o, extra=rows), lambda: pm.combine_rows(rows, o, out=rows),
+           lambda: pm.dispatch_rows(rows[:4], o, out=rows), lambda: pm.combine_rows(rows, o, out=rows[2:6]),
+           lambda: pm.combine_rows(torch.ones_like(rows), o, extra=rows[:4], out=rows[1:5]),
            lambda: pm.combine_rows_grad(rows, rows, o), lambda: pm.combine_rows_grad(x, x, o),
            lambda: pm.sort_by_expert(w.int().view(2, 2, 2), 4), lambda: pm.sort_by_expert(w.int(), 4, expert_base=-1),
            lambda: pm.sort_by_expert(torch.zeros((4, 0), dtype=torch.int32, device=DEV), 4)]
