@@ -10,6 +10,7 @@
 // K for its share of h = A x, the shares are added through distributed shared memory, and each CTA then takes a part of the N
 // output columns.  h never goes to memory, and a single token still uses eight SMs.  Two kernels of that form: tiles of
 // sixteen rows on the warp-level matrix instructions (k_adapters), and of 128 rows on tcgen05 (k_adapters_tc).
+#include <atomic>
 #include <cooperative_groups.h>
 
 #include "pmoe_internal.h"
@@ -881,12 +882,18 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_adapters_tc(AdapterArgs P, co
 
 // slots clusters of `ctas` CTAs
 template <typename Kern, typename XT, typename OT>
-static cudaError_t launch_clusters(Kern kern, int slots, int ctas, int threads, size_t smem, const AdapterArgs &P, const XT *x, const OT *base, OT *out,
+static cudaError_t launch_clusters(Kern kern, std::atomic<uint64_t> &asked, int slots, int ctas, int threads, size_t smem, const AdapterArgs &P, const XT *x, const OT *base, OT *out,
                                    cudaStream_t s)
 {
-    if (smem > 40 * 1024) {   // with the static arrays, more than a launch may have without asking
-        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (smem > 40 * 1024) {   // with the static arrays, more than a launch may have without asking: once for each device
+        int device = 0;
+        cudaError_t e = cudaGetDevice(&device);
         if (e != cudaSuccess) return e;
+        if (device > 63 || !(asked.load(std::memory_order_relaxed) >> device & 1)) {
+            e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+            if (e != cudaSuccess) return e;
+            if (device <= 63) asked.fetch_or(1ull << device, std::memory_order_relaxed);
+        }
     }
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)slots * ctas);
@@ -929,14 +936,16 @@ static cudaError_t launch_adapters_as(const AdapterArgs &P, const XT *x, const O
     const bool slots_by_id = P.order || P.n > ADAPTER_ROWS_LEADER;   // else every row is a slot
     const int64_t room = 148 * (int64_t)max(1, min(8, (int)(227 * 1024 / (S::SMEM + 6144))));
     const int ctas = cluster_size(slots_by_id ? tiles_of(P, FEW_M) : min(P.n, P.L), room, 8.0, (P.K + P.N) / 128.0);   // in stages
-    return launch_clusters(k_adapters<XT, OT, RT>, slots_by_id ? P.n / FEW_M + P.L : P.n, ctas, FEW_THREADS, S::SMEM, P, x, base, out, s);
+    static std::atomic<uint64_t> asked{0};
+    return launch_clusters(k_adapters<XT, OT, RT>, asked, slots_by_id ? P.n / FEW_M + P.L : P.n, ctas, FEW_THREADS, S::SMEM, P, x, base, out, s);
 }
 
 template <typename OT, int RT>
 static cudaError_t launch_adapters_tc(const AdapterArgs &P, const __nv_bfloat16 *x, const OT *base, OT *out, cudaStream_t s)
 {
     const int ctas = cluster_size(tiles_of(P, TC_M), 148, 8.0, P.K / 64 * 0.35 + P.N / 128 * 0.9);   // in microseconds
-    return launch_clusters(k_adapters_tc<OT, RT>, P.n / TC_M + P.L, ctas, TC_THREADS, TcTile<OT, RT>::SMEM, P, x, base, out, s);
+    static std::atomic<uint64_t> asked{0};
+    return launch_clusters(k_adapters_tc<OT, RT>, asked, P.n / TC_M + P.L, ctas, TC_THREADS, TcTile<OT, RT>::SMEM, P, x, base, out, s);
 }
 
 cudaError_t launch_adapters(const void *base, int out_dtype, const void *x, int x_dtype, const AdapterArgs &P, void *out, cudaStream_t s)

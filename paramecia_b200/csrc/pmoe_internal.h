@@ -28,7 +28,8 @@ struct DeviceGuard {
     explicit DeviceGuard(int device)
     {
         if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
-        ok = cudaSetDevice(device) == cudaSuccess;
+        ok = prev == device || cudaSetDevice(device) == cudaSuccess;
+        if (prev == device) prev = -1;   // nothing to restore
     }
     ~DeviceGuard()
     {

@@ -162,7 +162,7 @@ def dispatch_rows(x: torch.Tensor, order: ExpertOrder, out: Optional[torch.Tenso
 
 
 def _pair_weights(weights: torch.Tensor, order: ExpertOrder, device) -> torch.Tensor:
-    if not isinstance(weights, torch.Tensor) or weights.device != device or weights.numel() != order.n * order.top_k:
+    if not isinstance(weights, torch.Tensor) or weights.device != device or tuple(weights.shape) != (order.n, order.top_k):
         raise ValueError(f"weights must be [{order.n}, {order.top_k}] on {device}")
     return _f32(weights)
 

@@ -270,7 +270,7 @@ def test_refusals():
     w = torch.zeros((4, 2), device=DEV)
     bad = [lambda: pm.dispatch_rows(x[:3], o), lambda: pm.dispatch_rows(x[0], o), lambda: pm.dispatch_rows(x, "order"),
            lambda: pm.dispatch_rows(x, o, out=rows[:7]), lambda: pm.dispatch_rows(x, o, out=rows.bfloat16()),
-           lambda: pm.combine_rows(x, o), lambda: pm.combine_rows(rows, o, w[:3]), lambda: pm.combine_rows(rows, o, w.cpu()),
+           lambda: pm.combine_rows(x, o), lambda: pm.combine_rows(rows, o, w[:3]), lambda: pm.combine_rows(rows, o, w.t()), lambda: pm.combine_rows_grad(x, rows, o, w.reshape(-1)), lambda: pm.combine_rows(rows, o, w.cpu()),
            lambda: pm.combine_rows(rows, o, extra=rows), lambda: pm.combine_rows(rows, o, out=rows),
            lambda: pm.dispatch_rows(rows[:4], o, out=rows), lambda: pm.combine_rows(rows, o, out=rows[2:6]),
            lambda: pm.combine_rows(torch.ones_like(rows), o, extra=rows[:4], out=rows[1:5]),
