@@ -36,7 +36,7 @@ _stream = torch._C._cuda_getCurrentRawStream
 
 
 def _f32(t: torch.Tensor) -> torch.Tensor:
-    return t.contiguous() if t.dtype == torch.float32 else t.to(torch.float32).contiguous()
+    return t.contiguous() if t.dtype is torch.float32 else t.to(torch.float32).contiguous()
 
 
 def _on_gpu(what: str, t: torch.Tensor) -> torch.device:
@@ -117,19 +117,20 @@ def sort_by_expert(indices: torch.Tensor, num_experts: int, expert_base: int = 0
     expert_base <= id < expert_base + num_experts (an expert-parallel rank's slice); all others, negative ones among
     them, are skipped.  The result depends on the ids alone, not on timing."""
     device = _on_gpu("indices", indices)
-    if indices.dim() not in (1, 2):
+    shape = indices.shape
+    if len(shape) not in (1, 2):
         raise ValueError("indices must be [n, top_k] or [n]")
     if not 1 <= int(num_experts) <= _MAX_EXPERTS:
         raise PmoeError(-3, f"1 to {_MAX_EXPERTS} experts are served, got {num_experts}")
     if expert_base < 0:
         raise ValueError("expert_base must not be negative")
-    n, top_k = indices.shape[0], indices.shape[1] if indices.dim() == 2 else 1
+    n, top_k = shape[0], shape[1] if len(shape) == 2 else 1
     if top_k == 0:
         raise ValueError("indices must have at least one slot")
     idx = _ids("indices", indices)
     o = ExpertOrder(n, top_k, int(num_experts), device)
-    check(lib().pmoe_sort_pairs(device.index, idx.data_ptr(), n, top_k, int(expert_base), o.num_experts, o._order, o._place, o._offsets,
-                                _stream(device.index)))
+    i = device.index
+    check(lib().pmoe_sort_pairs(i, idx.data_ptr(), n, top_k, int(expert_base), o.num_experts, o._order, o._place, o._offsets, _stream(i)))
     return o
 
 
@@ -145,32 +146,35 @@ def dispatch_rows(x: torch.Tensor, order: ExpertOrder, out: Optional[torch.Tenso
     8-bit rows, their scales).  The rows behind the last kept pair are zero.  ``out``: the tensor to fill."""
     device = _on_gpu("x", x)
     _ordered(order, device)
-    if x.dim() != 2 or x.shape[0] != order.n:
-        raise ValueError(f"x must be [{order.n}, H], got {tuple(x.shape)}")
-    x = x.contiguous()
-    rows = (order.n * order.top_k, x.shape[1])
+    shape, n, top_k = x.shape, order.n, order.top_k
+    if len(shape) != 2 or shape[0] != n:
+        raise ValueError(f"x must be [{n}, H], got {tuple(shape)}")
+    x, H = x.contiguous(), shape[1]
     if out is None:
-        out = torch.empty(*rows, dtype=x.dtype, device=device)
+        out = torch.empty(n * top_k, H, dtype=x.dtype, device=device)
     else:
-        _check_buffer("out", out, rows, x.dtype, device)
+        _check_buffer("out", out, (n * top_k, H), x.dtype, device)
         _apart("x", out, x)
-    if x.shape[1] == 0:
+    if H == 0:
         return out
-    check(lib().pmoe_dispatch_rows(device.index, x.data_ptr(), x.shape[1] * x.element_size(), order.n, order.top_k, order._place,
-                                   order._offsets, order.num_experts, out.data_ptr(), _stream(device.index)))
+    i = device.index
+    check(lib().pmoe_dispatch_rows(i, x.data_ptr(), H * x.element_size(), n, top_k, order._place, order._offsets, order.num_experts,
+                                   out.data_ptr(), _stream(i)))
     return out
 
 
 def _pair_weights(weights: torch.Tensor, order: ExpertOrder, device) -> torch.Tensor:
-    if not isinstance(weights, torch.Tensor) or weights.device != device or tuple(weights.shape) != (order.n, order.top_k):
+    if not isinstance(weights, torch.Tensor) or weights.device != device or weights.shape != (order.n, order.top_k):
         raise ValueError(f"weights must be [{order.n}, {order.top_k}] on {device}")
     return _f32(weights)
 
 
-def _pair_rows(what: str, rows: torch.Tensor, order: ExpertOrder) -> torch.Tensor:
-    if rows.dim() != 2 or rows.shape[0] != order.n * order.top_k or rows.shape[1] == 0:
-        raise ValueError(f"{what} must be [{order.n * order.top_k}, H], got {tuple(rows.shape)}")
-    return rows.contiguous()
+def _pair_rows(what: str, rows: torch.Tensor, order: ExpertOrder) -> Tuple[torch.Tensor, int, int]:
+    """The rows contiguous, their number and their length."""
+    shape = rows.shape
+    if len(shape) != 2 or shape[0] != order.n * order.top_k or shape[1] == 0:
+        raise ValueError(f"{what} must be [{order.n * order.top_k}, H], got {tuple(shape)}")
+    return rows.contiguous(), shape[0], shape[1]
 
 
 def combine_rows(rows: torch.Tensor, order: ExpertOrder, weights: Optional[torch.Tensor] = None,
@@ -182,26 +186,26 @@ def combine_rows(rows: torch.Tensor, order: ExpertOrder, weights: Optional[torch
     device = _on_gpu("rows", rows)
     _ordered(order, device)
     rd = _typed("rows", rows, device)
-    rows = _pair_rows("rows", rows, order)
-    shape = (order.n, rows.shape[1])
+    rows, pairs, H = _pair_rows("rows", rows, order)
+    n = order.n
     w = None if weights is None else _pair_weights(weights, order, device)
-    e = None
+    e, ed = None, 0
     if extra is not None:
-        _typed("extra", extra, device)
-        if tuple(extra.shape) != shape:
-            raise ValueError(f"extra must be {shape}, got {tuple(extra.shape)}")
+        ed = _typed("extra", extra, device)
+        if extra.shape != (n, H):
+            raise ValueError(f"extra must be {(n, H)}, got {tuple(extra.shape)}")
         e = extra.contiguous()
     if out is None:
-        out = torch.empty(*shape, dtype=out_dtype or rows.dtype, device=device)
-        od = _out_type("out_dtype", out.dtype)
+        od = rd if out_dtype is None else _out_type("out_dtype", out_dtype)
+        out = torch.empty(n, H, dtype=out_dtype or rows.dtype, device=device)
     else:
-        _check_buffer("out", out, shape, tuple(_TYPES), device)
+        _check_buffer("out", out, (n, H), tuple(_TYPES), device)
         _apart("rows", out, rows)
         _apart("extra", out, e, same=True)
         od = _TYPES[out.dtype]
-    check(lib().pmoe_combine_rows(device.index, rows.data_ptr(), rd, rows.shape[0], order.n, order.top_k, rows.shape[1], order._place,
-                                  None if w is None else w.data_ptr(), None if e is None else e.data_ptr(),
-                                  0 if e is None else _TYPES[e.dtype], out.data_ptr(), od, _stream(device.index)))
+    i = device.index
+    check(lib().pmoe_combine_rows(i, rows.data_ptr(), rd, pairs, n, order.top_k, H, order._place, None if w is None else w.data_ptr(),
+                                  None if e is None else e.data_ptr(), ed, out.data_ptr(), od, _stream(i)))
     return out
 
 
@@ -218,16 +222,17 @@ def combine_rows_grad(grad_out: torch.Tensor, rows: torch.Tensor, order: ExpertO
     device = _on_gpu("grad_out", grad_out)
     _ordered(order, device)
     gd, rd = _typed("grad_out", grad_out, device), _typed("rows", rows, device)
-    rows = _pair_rows("rows", rows, order)
-    if tuple(grad_out.shape) != (order.n, rows.shape[1]):
-        raise ValueError(f"grad_out must be {(order.n, rows.shape[1])}, got {tuple(grad_out.shape)}")
+    rows, pairs, H = _pair_rows("rows", rows, order)
+    n, top_k = order.n, order.top_k
+    if grad_out.shape != (n, H):
+        raise ValueError(f"grad_out must be {(n, H)}, got {tuple(grad_out.shape)}")
     g = grad_out.contiguous()
     w = None if weights is None else _pair_weights(weights, order, device)
     grad_rows = torch.empty_like(rows)
-    grad_w = torch.empty(order.n, order.top_k, dtype=torch.float32, device=device)
-    check(lib().pmoe_combine_rows_grad(device.index, g.data_ptr(), gd, rows.data_ptr(), rd, order.n, order.top_k, rows.shape[1],
-                                       order._place, order._offsets, order.num_experts, None if w is None else w.data_ptr(),
-                                       grad_rows.data_ptr(), grad_w.data_ptr(), _stream(device.index)))
+    grad_w = torch.empty(n, top_k, dtype=torch.float32, device=device)
+    i = device.index
+    check(lib().pmoe_combine_rows_grad(i, g.data_ptr(), gd, rows.data_ptr(), rd, n, top_k, H, order._place, order._offsets, order.num_experts,
+                                       None if w is None else w.data_ptr(), grad_rows.data_ptr(), grad_w.data_ptr(), _stream(i)))
     return grad_rows, grad_w
 
 
@@ -241,20 +246,21 @@ def add_rms_norm_q8(resid: torch.Tensor, delta: Optional[torch.Tensor], weight: 
     when not asked for).  q and scales go to the experts through ``dispatch_rows``.  Rounding has no gradient: this is an
     operator for inference."""
     device = _on_gpu("resid", resid)
-    if resid.dim() != 2:
+    shape = resid.shape
+    if len(shape) != 2:
         raise ValueError("resid must be [n, H]")
-    n, H = resid.shape
+    n, H = shape
     rd = _typed("resid", resid, device)
     r = resid.contiguous()
     d = dd = None
     if delta is not None:
         dd = _typed("delta", delta, device)
-        if delta.shape != resid.shape:
+        if delta.shape != shape:
             raise ValueError(f"delta must be {(n, H)}, got {tuple(delta.shape)}")
         d = delta.contiguous()
     w = None
     if weight is not None:
-        if not isinstance(weight, torch.Tensor) or weight.device != device or tuple(weight.shape) != (H,):
+        if not isinstance(weight, torch.Tensor) or weight.device != device or weight.shape != (H,):
             raise ValueError(f"weight must be [{H}] on {device}")
         w = _f32(weight)
     if q_dtype not in _Q_TYPES:
@@ -268,10 +274,10 @@ def add_rms_norm_q8(resid: torch.Tensor, delta: Optional[torch.Tensor], weight: 
     q = torch.empty_like(r, dtype=q_dtype)
     scales = torch.empty(n, (H + group - 1) // group if group else 1, dtype=torch.float32, device=device)
     values = None if values_dtype is None else torch.empty_like(r, dtype=values_dtype)
-    check(lib().pmoe_add_rms_norm_q8(device.index, r.data_ptr(), rd, None if d is None else d.data_ptr(), dd or 0,
-                                     None if w is None else w.data_ptr(), n, H, float(eps), group, new_resid.data_ptr(), _Q_TYPES[q_dtype],
-                                     q.data_ptr(), scales.data_ptr(), None if values is None else values.data_ptr(), vd,
-                                     _stream(device.index)))
+    i = device.index
+    check(lib().pmoe_add_rms_norm_q8(i, r.data_ptr(), rd, None if d is None else d.data_ptr(), dd or 0, None if w is None else w.data_ptr(), n, H,
+                                     float(eps), group, new_resid.data_ptr(), _Q_TYPES[q_dtype], q.data_ptr(), scales.data_ptr(),
+                                     None if values is None else values.data_ptr(), vd, _stream(i)))
     return new_resid, q, scales, values
 
 
@@ -297,12 +303,12 @@ def adapters_add(base: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.
         if t.dtype != torch.bfloat16:
             raise PmoeError(-2, f"{name} must be bfloat16, got {t.dtype}")
     L, r, K = a.shape
-    N = b.shape[1]
-    if L == 0 or tuple(b.shape) != (L, N, r):
+    Lb, N, rb = b.shape
+    if L == 0 or Lb != L or rb != r:
         raise ValueError(f"a must be [L, r, K] and b [L, N, r], got {tuple(a.shape)} and {tuple(b.shape)}")
-    if x.dim() != 2 or x.shape[1] != K or tuple(base.shape) != (x.shape[0], N):
+    n = x.shape[0] if x.dim() == 2 else -1
+    if n < 0 or x.shape[1] != K or base.shape != (n, N):
         raise ValueError(f"x must be [n, {K}] and base [n, {N}], got {tuple(x.shape)} and {tuple(base.shape)}")
-    n = x.shape[0]
     if not isinstance(ids, torch.Tensor) or ids.device != device or ids.numel() != n:
         raise ValueError(f"ids must be [{n}] on {device}")
     if L > _MAX_EXPERTS:
@@ -312,7 +318,8 @@ def adapters_add(base: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.
         if not isinstance(scales, torch.Tensor) or scales.device != device or scales.numel() != L:
             raise ValueError(f"scales must be [{L}] on {device}")
         s = _f32(scales)
-    x, a, b, ids = _aligned(x), _aligned(a), _aligned(b), _ids("ids", ids.reshape(-1))
+    (x, xp), (a, ap), (b, bp), (base, basep) = _aligned(x), _aligned(a), _aligned(b), _aligned(base)
+    ids = _ids("ids", ids if ids.dim() == 1 else ids.reshape(-1))
     if order is not None:
         _ordered(order, device)
         if (order.n, order.top_k, order.num_experts) != (n, 1, L):
@@ -320,25 +327,28 @@ def adapters_add(base: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.
     elif n > _ADAPTER_ROWS_UNSORTED:
         order = sort_by_expert(ids, L)
     if out is None:
-        base = _aligned(base)
         out = torch.empty_like(base)
     else:
         _check_buffer("out", out, (n, N), base.dtype, device)
         if out.data_ptr() % 16:
             raise ValueError("out must be 16-byte aligned")
-        base = _aligned(base)
         _apart("x", out, x)
         _apart("base", out, base, same=True)
-    check(lib().pmoe_adapters_add(device.index, base.data_ptr(), x.data_ptr(), xd, n, K, N, r, L, a.data_ptr(), b.data_ptr(),
-                                  None if s is None else s.data_ptr(), ids.data_ptr(), None if order is None else order._order,
-                                  None if order is None else order._offsets, out.data_ptr(), od, _stream(device.index)))
+    i = device.index
+    check(lib().pmoe_adapters_add(i, basep, xp, xd, n, K, N, r, L, ap, bp, None if s is None else s.data_ptr(), ids.data_ptr(),
+                                  None if order is None else order._order, None if order is None else order._offsets, out.data_ptr(), od,
+                                  _stream(i)))
     return out
 
 
-def _aligned(t: torch.Tensor) -> torch.Tensor:
-    """Contiguous, from a 16-byte boundary on (a view may begin anywhere)."""
+def _aligned(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
+    """The tensor contiguous and from a 16-byte boundary on (a view may begin anywhere), and its address."""
     t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+    p = t.data_ptr()
+    if p % 16:
+        t = t.clone()
+        p = t.data_ptr()
+    return t, p
 
 
 def rows_status(device="cuda") -> None:
