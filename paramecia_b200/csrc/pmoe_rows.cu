@@ -261,7 +261,8 @@ struct RowThreads {
 
 // Rows are moved as bytes, so any element type goes: a unit is read once and written to the token's places.  The rows behind
 // the last kept pair are zeroed by the same CTAs.
-template <typename V>
+// M: units a thread takes at once, `step` apart; four where a unit is small, so that a place is read once for all of them.
+template <typename V, int M>
 __global__ void __launch_bounds__(256) k_dispatch_rows(const V *__restrict__ x, int units, int n, int top_k, const int *__restrict__ place,
                                                        const int *__restrict__ offsets, int E, V *__restrict__ out, RowThreads rt)
 {
@@ -271,12 +272,18 @@ __global__ void __launch_bounds__(256) k_dispatch_rows(const V *__restrict__ x, 
     int t, first, step;
     rt.mine(t, first, step);
     if (t < n)
-        for (int u = first; u < units; u += step) {
-            const V v = x[(size_t)t * units + u];
+        for (int u = first; u < units; u += step * M) {
+            V v[M];
+#pragma unroll
+            for (int m = 0; m < M; m++) v[m] = u + m * step < units ? x[(size_t)t * units + u + m * step] : V{};
 #pragma unroll 4
             for (int j = 0; j < top_k; j++) {
                 const int to = place[(size_t)t * top_k + j];
-                if ((unsigned)to < (unsigned)P) out[(size_t)to * units + u] = v;
+                if ((unsigned)to >= (unsigned)P) continue;
+                V *row = out + (size_t)to * units + u;
+#pragma unroll
+                for (int m = 0; m < M; m++)
+                    if (u + m * step < units) row[m * step] = v[m];
             }
         }
     for (int64_t r = (int64_t)max(0, offsets[E]) + blockIdx.x; r < P; r += gridDim.x)
@@ -289,16 +296,17 @@ cudaError_t launch_dispatch_rows(const void *x, size_t row_bytes, int n, int top
     const uintptr_t a = (uintptr_t)x | (uintptr_t)out | row_bytes;
     auto go = [&](auto v) {
         using V = decltype(v);
+        constexpr int M = sizeof(V) <= 4 ? 4 : 1;
         const int units = (int)(row_bytes / sizeof(V));
-        const RowThreads rt = RowThreads::of(units, n);
-        return launch_pdl(k_dispatch_rows<V>, dim3(rt.grid), dim3(256), 0, s, (const V *)x, units, n, top_k, place, offsets, E, (V *)out, rt);
+        const RowThreads rt = RowThreads::of((units + M - 1) / M, n);
+        return launch_pdl(k_dispatch_rows<V, M>, dim3(rt.grid), dim3(256), 0, s, (const V *)x, units, n, top_k, place, offsets, E, (V *)out, rt);
     };
     count_launch();
     return a % 16 == 0 ? go(uint4{}) : a % 8 == 0 ? go(uint2{}) : a % 4 == 0 ? go(0u) : a % 2 == 0 ? go((uint16_t)0) : go((uint8_t)0);
 }
 
 // out_t = extra_t + sum_j w_tj rows[place_tj], f32 in slot order.  Without weights it is the gradient of the dispatch.
-// Four rows are loaded before the first is added.  (extra may be out: a thread reads the elements it later writes.)
+// (extra may be out: a thread reads the elements it later writes.)
 template <int U, typename RT, typename ET, typename OT>
 __global__ void __launch_bounds__(256) k_combine_rows(const RT *__restrict__ rows, int H, int n, int top_k, int n_rows,
                                                       const int *__restrict__ place, const float *__restrict__ w, const ET *extra,
@@ -312,32 +320,44 @@ __global__ void __launch_bounds__(256) k_combine_rows(const RT *__restrict__ row
     if (t >= n) return;
     place += (size_t)t * top_k;
     if (w) w += (size_t)t * top_k;
-    for (int u = first; u < units; u += step) {
-        float acc[U] = {};
-        for (int j = 0; j < top_k && n_rows > 0; j += 4) {
-            float v[4][U], f[4];
-            bool there[4];
+    // M units at once, `step` apart (four where a unit is one or two elements: a place and a weight are read once for all), of
+    // BATCH rows, without a branch between the loads: the first row and the last unit stand in for what does not count.
+    constexpr int M = U <= 2 ? 4 : 1, BATCH = U <= 2 ? 2 : 4;
+    for (int u = first; u < units; u += step * M) {
+        float acc[M][U] = {};
+        int at[M];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                // four loads without a branch between them: the first row stands in for one that does not count
+        for (int m = 0; m < M; m++) at[m] = M == 1 ? u * U : min(u + m * step, units - 1) * U;
+        for (int j = 0; j < top_k && n_rows > 0; j += BATCH) {
+            float v[BATCH][M][U], f[BATCH];
+            bool there[BATCH];
+#pragma unroll
+            for (int i = 0; i < BATCH; i++) {
                 const int r = j + i < top_k ? place[j + i] : -1;
                 there[i] = (unsigned)r < (unsigned)n_rows;
                 f[i] = w && j + i < top_k ? w[j + i] : 1.f;
-                load_units<U>(rows + (size_t)(there[i] ? r : 0) * H + u * U, v[i]);
+#pragma unroll
+                for (int m = 0; m < M; m++) load_units<U>(rows + (size_t)(there[i] ? r : 0) * H + at[m], v[i][m]);
             }
 #pragma unroll
-            for (int i = 0; i < 4; i++)
+            for (int i = 0; i < BATCH; i++)
                 if (there[i])
 #pragma unroll
-                    for (int e = 0; e < U; e++) acc[e] = fmaf(f[i], v[i][e], acc[e]);
-        }
-        if (extra) {
-            float v[U];
-            load_units<U>(extra + (size_t)t * H + u * U, v);
+                    for (int m = 0; m < M; m++)
 #pragma unroll
-            for (int e = 0; e < U; e++) acc[e] += v[e];
+                        for (int e = 0; e < U; e++) acc[m][e] = fmaf(f[i], v[i][m][e], acc[m][e]);
         }
-        store_units<U>(out + (size_t)t * H + u * U, acc);
+#pragma unroll
+        for (int m = 0; m < M; m++) {
+            if (M > 1 && u + m * step >= units) break;
+            if (extra) {
+                float v[U];
+                load_units<U>(extra + (size_t)t * H + at[m], v);
+#pragma unroll
+                for (int e = 0; e < U; e++) acc[m][e] += v[e];
+            }
+            store_units<U>(out + (size_t)t * H + at[m], acc[m]);
+        }
     }
 }
 
@@ -367,7 +387,7 @@ cudaError_t launch_combine_rows(const void *rows, int rows_dtype, int n_rows, in
     count_launch();
     const int u = unit_elements(H, rows_dtype == PMOE_F32 || extra_dtype == PMOE_F32 || out_dtype == PMOE_F32,
                                 {{rows, rows_dtype}, {extra, extra_dtype}, {out, out_dtype}});
-    const RowThreads rt = RowThreads::of(H / u, n);
+    const RowThreads rt = RowThreads::of(u <= 2 ? (H / u + 3) / 4 : H / u, n);
     return with_type(rows_dtype, [&](auto *rp) {
         return with_type(extra_dtype, [&](auto *ep) {
             return with_type(out_dtype, [&](auto *op) {
