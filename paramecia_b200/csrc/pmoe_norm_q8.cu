@@ -76,10 +76,16 @@ template <bool E4M3, int N> __device__ inline void to_8bit(const float (&u)[N], 
     }
 }
 
-// the exact quotient of d by the group's largest magnitude, as an 8-bit float
+// The quotient of d by the group's largest magnitude, rounded once to an 8-bit float.  d and top are products of two f32 numbers:
+// 448 d is exact, and a quotient that is not a tie of e4m3 (five significant bits) is further from it than half a step of 64 bits,
+// so the 64-bit quotient lies on the same side of every tie as the exact one, or on it where that does.  On the way to f32 the last
+// bit says whether anything was cut off: rounding to nearest there would put a quotient beside a tie onto it.
 __device__ inline uint32_t to_e4m3_exact(double d, double top)
 {
-    return (uint32_t)__nv_cvt_float_to_fp8((float)(d * 448.0 / top), __NV_SATFINITE, __NV_E4M3);
+    const double quotient = d * 448.0 / top;
+    const float cut = __double2float_rz(quotient);
+    const float f = __uint_as_float(__float_as_uint(cut) | ((double)cut != quotient ? 1u : 0u));
+    return (uint32_t)__nv_cvt_float_to_fp8(f, __NV_SATFINITE, __NV_E4M3);
 }
 
 // What four bytes stand for in units of the scale
