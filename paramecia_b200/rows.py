@@ -67,7 +67,7 @@ def _ids(what: str, t: torch.Tensor) -> torch.Tensor:
     if t.dtype == torch.int32:
         return t.contiguous()
     if t.dtype == torch.int64:
-        return t.clamp(-1, 2 ** 31 - 1).to(torch.int32)
+        return t.clamp(-1, 2 ** 31 - 1).to(torch.int32).contiguous()   # both keep the strides of a transposed table
     raise PmoeError(-2, f"{what} must be int32 or int64, got {t.dtype}")
 
 
