@@ -10,7 +10,6 @@
 // K for its share of h = A x, the shares are added through distributed shared memory, and each CTA then takes a part of the N
 // output columns.  h never goes to memory, and a single token still uses eight SMs.  Two kernels of that form: tiles of
 // sixteen rows on the warp-level matrix instructions (k_adapters), and of 128 rows on tcgen05 (k_adapters_tc).
-#include <atomic>
 #include <cooperative_groups.h>
 
 #include "pmoe_internal.h"
@@ -885,15 +884,9 @@ template <typename Kern, typename XT, typename OT>
 static cudaError_t launch_clusters(Kern kern, std::atomic<uint64_t> &asked, int slots, int ctas, int threads, size_t smem, const AdapterArgs &P, const XT *x, const OT *base, OT *out,
                                    cudaStream_t s)
 {
-    if (smem > 40 * 1024) {   // with the static arrays, more than a launch may have without asking: once for each device
-        int device = 0;
-        cudaError_t e = cudaGetDevice(&device);
+    if (smem > 40 * 1024) {   // with the static arrays, more than a launch may have without asking
+        cudaError_t e = allow_smem((const void *)kern, smem, asked);
         if (e != cudaSuccess) return e;
-        if (device > 63 || !(asked.load(std::memory_order_relaxed) >> device & 1)) {
-            e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-            if (e != cudaSuccess) return e;
-            if (device <= 63) asked.fetch_or(1ull << device, std::memory_order_relaxed);
-        }
     }
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)slots * ctas);

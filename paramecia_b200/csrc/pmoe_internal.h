@@ -1,6 +1,7 @@
 // Host-side internals shared by the files that implement the C ABI: error reporting, the device guard and the
 // layer handle.
 #pragma once
+#include <atomic>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
@@ -36,6 +37,22 @@ struct DeviceGuard {
         if (prev >= 0) cudaSetDevice(prev);
     }
 };
+
+// Lets `kern` have up to `most` bytes of dynamic shared memory on the current device, once a device (`asked`, one for each kernel,
+// has a bit for each).  The limit belongs to the kernel, not to a launch: it must be the same in every call, or a thread
+// that lowers it makes another thread's launch fail.
+inline cudaError_t allow_smem(const void *kern, size_t most, std::atomic<uint64_t> &asked)
+{
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess) return e;
+    if (device > 63 || !(asked.load(std::memory_order_relaxed) >> device & 1)) {
+        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
+        if (e != cudaSuccess) return e;
+        if (device <= 63) asked.fetch_or(1ull << device, std::memory_order_relaxed);
+    }
+    return cudaSuccess;
+}
 
 }  // namespace pmoe
 

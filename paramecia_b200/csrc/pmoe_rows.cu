@@ -39,6 +39,7 @@ constexpr int SORT_THREADS = 1024;
 constexpr int SORT_CTAS = 8;
 constexpr int SORT_BATCH = 16;
 constexpr int SORT_ONE_CTA = 4096;   // pairs up to which one CTA sorts
+constexpr int SORT_SMEM = 200 * 1024;
 
 struct SortKeys {
     uint32_t v[SORT_BATCH];
@@ -203,16 +204,17 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_pairs(const uint32_t *__r
 
 cudaError_t launch_sort_pairs(const uint32_t *idx, int P, int base, int E, int *order, int *place, int *offsets, cudaStream_t s)
 {
-    // counts and masks of all warps within 200 KB; no more warps than there are steps of 32 pairs
-    const int most = min(32, (int)((200 * 1024 - 8 * E) / (8 * E)));
+    // counts and masks of all warps within SORT_SMEM; no more warps than there are steps of 32 pairs
+    const int most = min(32, (int)((SORT_SMEM - 8 * E) / (8 * E)));
     const bool one = P <= SORT_ONE_CTA;
     const int ctas = one ? 1 : SORT_CTAS;
     const int warps = min(most, max(1, (P + 31) / 32 / ctas));
     const int run = (int)((((int64_t)P + ctas * warps - 1) / (ctas * warps) + 31) / 32 * 32);
     const size_t smem = ((size_t)2 * warps + 2) * E * sizeof(int);
     auto *kern = one ? k_sort_pairs<1> : k_sort_pairs<SORT_CTAS>;
+    static std::atomic<uint64_t> asked[2] = {};
     if (smem > 40 * 1024) {
-        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        cudaError_t e = allow_smem((const void *)kern, SORT_SMEM, asked[one]);
         if (e != cudaSuccess) return e;
     }
     cudaLaunchConfig_t cfg{};

@@ -35,3 +35,30 @@ def test_transposed_ids(n, k, E, dtype):
     every_other[:, ::2] = slots_first.t()
     o = pm.sort_by_expert(every_other[:, ::2], E)
     assert np.array_equal(o.place.cpu().numpy(), plain_places(idx, E))
+
+
+def test_sorts_of_several_threads():
+    """Calls that need different amounts of shared memory, from threads that launch at the same time: none is refused, and
+    every one has its own result."""
+    shapes = [(4096, 512), (4096, 4096), (4096, 256), (20000, 512), (20000, 4096)]      # pairs, experts
+    rc, calls = {}, 4000
+    start = threading.Barrier(len(shapes))
+
+    def run(i):
+        P, E = shapes[i]
+        ids = torch.from_numpy(np.random.default_rng(i).integers(0, E, P).astype(np.int32)).to(DEV)
+        places, offsets = torch.empty(P, dtype=torch.int32, device=DEV), torch.empty(E + 1, dtype=torch.int32, device=DEV)
+        stream = torch.cuda.Stream(DEV)
+        torch.cuda.synchronize()
+        sort = pm.lib().pmoe_sort_pairs
+        start.wait()
+        bad = sum(sort(0, ids.data_ptr(), P, 1, 0, E, None, places.data_ptr(), offsets.data_ptr(), stream.cuda_stream) != 0 for _ in range(calls))
+        stream.synchronize()
+        rc[i] = bad, np.array_equal(places.cpu().numpy(), plain_places(ids.cpu().numpy(), E))
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(len(shapes))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert rc == {i: (0, True) for i in range(len(shapes))}
