@@ -86,12 +86,12 @@ class ExpertOrder:
 
     ``order`` int32 [n * top_k]: the pair at each row, -1 behind the last kept pair; ``place`` int32 [n, top_k]: the row of
     each pair, -1 for a pair that is not kept; ``offsets`` int32 [num_experts + 1]: the rows of expert e are
-    offsets[e] to offsets[e + 1]."""
+    offsets[e] to offsets[e + 1].  Expert e is the one whose id is expert_base + e."""
 
-    __slots__ = ("n", "top_k", "num_experts", "device", "_data", "_order", "_place", "_offsets")
+    __slots__ = ("n", "top_k", "num_experts", "expert_base", "device", "_data", "_order", "_place", "_offsets")
 
-    def __init__(self, n: int, top_k: int, num_experts: int, device):
-        self.n, self.top_k, self.num_experts, self.device = n, top_k, num_experts, device
+    def __init__(self, n: int, top_k: int, num_experts: int, device, expert_base: int = 0):
+        self.n, self.top_k, self.num_experts, self.device, self.expert_base = n, top_k, num_experts, device, expert_base
         pairs = n * top_k
         # one allocation for the three arrays; each begins on a 16-byte boundary
         step = (pairs + 3) // 4 * 4
@@ -128,9 +128,9 @@ def sort_by_expert(indices: torch.Tensor, num_experts: int, expert_base: int = 0
     if top_k == 0:
         raise ValueError("indices must have at least one slot")
     idx = _ids("indices", indices)
-    o = ExpertOrder(n, top_k, int(num_experts), device)
+    o = ExpertOrder(n, top_k, int(num_experts), device, int(expert_base))
     i = device.index
-    check(lib().pmoe_sort_pairs(i, idx.data_ptr(), n, top_k, int(expert_base), o.num_experts, o._order, o._place, o._offsets, _stream(i)))
+    check(lib().pmoe_sort_pairs(i, idx.data_ptr(), n, top_k, o.expert_base, o.num_experts, o._order, o._place, o._offsets, _stream(i)))
     return o
 
 
@@ -322,7 +322,7 @@ def adapters_add(base: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.
     ids = _ids("ids", ids if ids.dim() == 1 else ids.reshape(-1))
     if order is not None:
         _ordered(order, device)
-        if (order.n, order.top_k, order.num_experts) != (n, 1, L):
+        if (order.n, order.top_k, order.num_experts, order.expert_base) != (n, 1, L, 0):   # of a slice: other adapters, and rows in no tile
             raise ValueError(f"order must be sort_by_expert(ids, {L}) of these {n} ids")
     elif n > _ADAPTER_ROWS_UNSORTED:
         order = sort_by_expert(ids, L)

@@ -62,3 +62,18 @@ def test_sorts_of_several_threads():
     for t in threads:
         t.join()
     assert rc == {i: (0, True) for i in range(len(shapes))}
+
+
+@pytest.mark.parametrize("base", [1, 3, 8])
+def test_an_order_of_another_slice_is_refused(base):
+    """Rows below the slice's first id are in no tile of such an order and would be left unwritten."""
+    ids = torch.arange(20, dtype=torch.int32, device=DEV) % 8
+    x, rows = torch.ones((20, 16), device=DEV), torch.ones((20, 24), device=DEV)
+    a = torch.ones((8, 8, 16), dtype=torch.bfloat16, device=DEV)
+    b = torch.ones((8, 24, 8), dtype=torch.bfloat16, device=DEV)
+    o = pm.sort_by_expert(ids, 8, expert_base=base)
+    assert o.expert_base == base and pm.sort_by_expert(ids, 8).expert_base == 0
+    with pytest.raises(ValueError, match="order must be"):
+        pm.adapters_add(rows, x, a, b, ids, order=o)
+    got = pm.adapters_add(rows, x, a, b, ids, order=pm.sort_by_expert(ids, 8))
+    assert torch.equal(got, torch.full_like(got, 129.0))
