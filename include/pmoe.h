@@ -332,6 +332,9 @@ int pmoe_add_rms_norm_q8(int device, const void *resid_in, int resid_dtype, cons
  * pmoe_sort_pairs: offsets [E + 1] = number of kept pairs of the experts before e; place [n, top_k] = the pair's row in
  * expert order, -1 when it is skipped; order [n * top_k] = the pair at a row, -1 from row offsets[E] on.  Stable: pairs
  * of one expert stay in ascending order.  order or place may be NULL.  E <= 4096, n * top_k <= 2^30.
+ *
+ * In these entries and the two around them an output that lies over an input, or over another output, is refused
+ * (PMOE_ERR_INVALID_ARG) but where a description allows it.
  */
 int pmoe_sort_pairs(int device, const uint32_t *idx, int n, int top_k, int expert_base, int E, int *order, int *place, int *offsets,
                     void *stream);

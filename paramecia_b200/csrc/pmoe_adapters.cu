@@ -990,6 +990,10 @@ extern "C" int pmoe_adapters_add(int device, const void *base, const void *x, in
                     ADAPTER_ROWS_UNSORTED);
     if (!aligned16(base) || !aligned16(x) || !aligned16(a) || !aligned16(b) || !aligned16(out))
         return fail(PMOE_ERR_INVALID_ARG, "base, x, a, b and out must be 16-byte aligned");
+    const size_t ids_bytes = (size_t)n * sizeof(int), out_bytes = (size_t)n * N * block_bytes(out_dtype), L = n_adapters;
+    if (overlap({{out, out_bytes}}, {{base == out ? nullptr : base, out_bytes}, {x, (size_t)n * K * block_bytes(x_dtype)}, {a, L * rank * K * 2}, {b, L * N * rank * 2},
+                                     {scales, L * sizeof(float)}, {ids, ids_bytes}, {order, ids_bytes}, {offsets, (L + 1) * sizeof(int)}}))
+        return fail(PMOE_ERR_INVALID_ARG, "out must not overlap an input (it may be base)");
     DeviceGuard guard(device);
     if (!guard.ok) return fail(PMOE_ERR_NO_DEVICE, "cannot select device %d", device);
     const AdapterArgs args{n, K, N, rank, n_adapters, (const __nv_bfloat16 *)a, (const __nv_bfloat16 *)b, scales, ids, order, offsets};

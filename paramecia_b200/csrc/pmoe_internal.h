@@ -6,6 +6,7 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <initializer_list>
 #include <string>
 #include <vector>
 
@@ -52,6 +53,28 @@ inline cudaError_t allow_smem(const void *kern, size_t most, std::atomic<uint64_
         if (device <= 63) asked.fetch_or(1ull << device, std::memory_order_relaxed);
     }
     return cudaSuccess;
+}
+
+// Memory that a call reads or writes
+struct Span {
+    const void *at;
+    size_t bytes;
+    bool over(const Span &o) const
+    {
+        return at && o.at && (uintptr_t)at < (uintptr_t)o.at + o.bytes && (uintptr_t)o.at < (uintptr_t)at + bytes;
+    }
+};
+// Whether an output lies over one of the inputs or over another output.  Kernels read some inputs more than once and in several
+// CTAs, which must see the same each time.
+inline bool overlap(std::initializer_list<Span> outputs, std::initializer_list<Span> inputs)
+{
+    for (auto o = outputs.begin(); o != outputs.end(); o++) {
+        for (auto &i : inputs)
+            if (o->over(i)) return true;
+        for (auto p = o + 1; p != outputs.end(); p++)
+            if (o->over(*p)) return true;
+    }
+    return false;
 }
 
 }  // namespace pmoe

@@ -513,6 +513,12 @@ extern "C" int pmoe_add_rms_norm_q8(int device, const void *resid_in, int resid_
     if (!(eps >= 0.f)) return fail(PMOE_ERR_INVALID_ARG, "eps must not be negative");
     if (!n) return PMOE_OK;
     if (!resid_in || !q || !scales) return fail(PMOE_ERR_INVALID_ARG, "resid_in / q / scales is NULL");
+    const size_t values_n = (size_t)n * H, G = group ? ((size_t)H + group - 1) / group : 1;
+    const Span in{resid_in, values_n * block_bytes(resid_dtype)}, more{delta, values_n * block_bytes(delta_dtype)}, stored{resid_out, in.bytes};
+    if (overlap({{q, values_n}, {scales, n * G * sizeof(float)}, {values, values_n * block_bytes(values_dtype)}},
+                {in, more, stored, {weight, (size_t)H * sizeof(float)}}) ||
+        (resid_out != resid_in && stored.over(in)) || ((resid_out != delta || resid_dtype != delta_dtype) && stored.over(more)))
+        return fail(PMOE_ERR_INVALID_ARG, "the outputs must not overlap the inputs (resid_out may be resid_in) or one another");
     DeviceGuard guard(device);
     if (!guard.ok) return fail(PMOE_ERR_NO_DEVICE, "cannot select device %d", device);
     CU(launch_norm_q8(resid_in, resid_dtype, delta, delta ? delta_dtype : resid_dtype, weight, n, H, eps, group ? group : H, resid_out,

@@ -492,6 +492,9 @@ int pmoe_sort_pairs(int device, const uint32_t *idx, int n, int top_k, int exper
     if (rc) return rc;
     if (expert_base < 0) return fail(PMOE_ERR_INVALID_ARG, "expert_base must not be negative");
     if (!offsets || (n && !idx)) return fail(PMOE_ERR_INVALID_ARG, "idx / offsets is NULL");
+    const size_t pairs = (size_t)n * top_k * sizeof(int);
+    if (overlap({{order, pairs}, {place, pairs}, {offsets, ((size_t)E + 1) * sizeof(int)}}, {{idx, pairs}}))
+        return fail(PMOE_ERR_INVALID_ARG, "order, place and offsets must not overlap idx or one another");
     DeviceGuard guard(device);
     if (!guard.ok) return fail(PMOE_ERR_NO_DEVICE, "cannot select device %d", device);
     CU(launch_sort_pairs(idx, n * top_k, expert_base, E, order, place, offsets, (cudaStream_t)stream));
@@ -506,6 +509,9 @@ int pmoe_dispatch_rows(int device, const void *x, size_t row_bytes, int n, int t
     if (!row_bytes || row_bytes > (1u << 30)) return fail(PMOE_ERR_INVALID_ARG, "row_bytes must be 1 to 2^30");
     if (!n) return PMOE_OK;
     if (!x || !place || !offsets || !out) return fail(PMOE_ERR_INVALID_ARG, "x / place / offsets / out is NULL");
+    const size_t pairs = (size_t)n * top_k;
+    if (overlap({{out, pairs * row_bytes}}, {{x, (size_t)n * row_bytes}, {place, pairs * sizeof(int)}, {offsets, ((size_t)E + 1) * sizeof(int)}}))
+        return fail(PMOE_ERR_INVALID_ARG, "out must not overlap x, place or offsets");
     DeviceGuard guard(device);
     if (!guard.ok) return fail(PMOE_ERR_NO_DEVICE, "cannot select device %d", device);
     CU(launch_dispatch_rows(x, row_bytes, n, top_k, place, offsets, E, out, (cudaStream_t)stream));
@@ -522,6 +528,11 @@ int pmoe_combine_rows(int device, const void *rows, int rows_dtype, int n_rows, 
         return fail(PMOE_ERR_UNSUPPORTED_DTYPE, "rows / extra / out must be F32 or BF16");
     if (!n) return PMOE_OK;
     if ((n_rows && !rows) || !place || !out) return fail(PMOE_ERR_INVALID_ARG, "rows / place / out is NULL");
+    const size_t pairs = (size_t)n * top_k, out_bytes = (size_t)n * H * block_bytes(out_dtype);
+    const bool in_place = extra == out && extra_dtype == out_dtype;
+    if (overlap({{out, out_bytes}}, {{rows, (size_t)n_rows * H * block_bytes(rows_dtype)}, {place, pairs * sizeof(int)}, {w, pairs * sizeof(float)},
+                                     {in_place ? nullptr : extra, (size_t)n * H * block_bytes(extra_dtype)}}))
+        return fail(PMOE_ERR_INVALID_ARG, "out must not overlap rows, place or w, and extra only as a whole and in the same type");
     DeviceGuard guard(device);
     if (!guard.ok) return fail(PMOE_ERR_NO_DEVICE, "cannot select device %d", device);
     CU(launch_combine_rows(rows, rows_dtype, n_rows, n, top_k, H, place, w, extra, extra ? extra_dtype : out_dtype, out, out_dtype,
@@ -539,6 +550,11 @@ int pmoe_combine_rows_grad(int device, const void *grad_out, int grad_dtype, con
     if (!n) return PMOE_OK;
     if (!grad_rows && !grad_w) return fail(PMOE_ERR_INVALID_ARG, "neither grad_rows nor grad_w is asked for");
     if (!grad_out || !place || !offsets || (grad_w && !rows)) return fail(PMOE_ERR_INVALID_ARG, "grad_out / rows / place / offsets is NULL");
+    const size_t pairs = (size_t)n * top_k, rows_bytes = pairs * H * block_bytes(rows_dtype);
+    if (overlap({{grad_rows, rows_bytes}, {grad_w, pairs * sizeof(float)}},
+                {{grad_out, (size_t)n * H * block_bytes(grad_dtype)}, {rows, rows_bytes}, {place, pairs * sizeof(int)},
+                 {offsets, ((size_t)E + 1) * sizeof(int)}, {w, pairs * sizeof(float)}}))
+        return fail(PMOE_ERR_INVALID_ARG, "grad_rows and grad_w must not overlap an input or one another");
     DeviceGuard guard(device);
     if (!guard.ok) return fail(PMOE_ERR_NO_DEVICE, "cannot select device %d", device);
     CU(launch_combine_grad(grad_out, grad_dtype, rows, rows_dtype, n, top_k, H, place, offsets, E, w, grad_rows, grad_w,

@@ -155,6 +155,7 @@ def dispatch_rows(x: torch.Tensor, order: ExpertOrder, out: Optional[torch.Tenso
     else:
         _check_buffer("out", out, (n * top_k, H), x.dtype, device)
         _apart("x", out, x)
+        _apart("order", out, order._data)
     if H == 0:
         return out
     i = device.index
@@ -202,6 +203,8 @@ def combine_rows(rows: torch.Tensor, order: ExpertOrder, weights: Optional[torch
         _check_buffer("out", out, (n, H), tuple(_TYPES), device)
         _apart("rows", out, rows)
         _apart("extra", out, e, same=True)
+        _apart("weights", out, w)
+        _apart("order", out, order._data)
         od = _TYPES[out.dtype]
     i = device.index
     check(lib().pmoe_combine_rows(i, rows.data_ptr(), rd, pairs, n, order.top_k, H, order._place, None if w is None else w.data_ptr(),
@@ -332,8 +335,9 @@ def adapters_add(base: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.
         _check_buffer("out", out, (n, N), base.dtype, device)
         if out.data_ptr() % 16:
             raise ValueError("out must be 16-byte aligned")
-        _apart("x", out, x)
         _apart("base", out, base, same=True)
+        for name, t in (("x", x), ("a", a), ("b", b), ("ids", ids), ("scales", s), ("order", None if order is None else order._data)):
+            _apart(name, out, t)
     i = device.index
     check(lib().pmoe_adapters_add(i, basep, xp, xd, n, K, N, r, L, ap, bp, None if s is None else s.data_ptr(), ids.data_ptr(),
                                   None if order is None else order._order, None if order is None else order._offsets, out.data_ptr(), od,

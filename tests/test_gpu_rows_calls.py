@@ -77,3 +77,21 @@ def test_an_order_of_another_slice_is_refused(base):
         pm.adapters_add(rows, x, a, b, ids, order=o)
     got = pm.adapters_add(rows, x, a, b, ids, order=pm.sort_by_expert(ids, 8))
     assert torch.equal(got, torch.full_like(got, 129.0))
+
+
+def test_an_out_over_ids_weights_or_the_order_is_refused():
+    n, k, N = 64, 2, 64
+    pool = torch.zeros(4096, dtype=torch.int32, device=DEV)              # what the outputs lie in
+    out = pool.view(torch.float32).view(n, N)
+    ids = pool[:n * k].view(n, k)
+    o = pm.sort_by_expert(torch.zeros_like(ids), 4)
+    rows, x = torch.ones((n * k, N), device=DEV), torch.ones((n, N), device=DEV)
+    a, b = torch.zeros((4, 8, N), dtype=torch.bfloat16, device=DEV), torch.zeros((4, N, 8), dtype=torch.bfloat16, device=DEV)
+    first = pool[:n]
+    over_order = o._data[:(n * k) // 4 * 4].view(torch.float32).view(n * k, 1)
+    for f in (lambda: pm.combine_rows(rows, o, ids.view(torch.float32), out=out), lambda: pm.dispatch_rows(x[:, :1].contiguous(), o, out=over_order),
+              lambda: pm.adapters_add(x, x.clone(), a, b, first, out=out), lambda: pm.adapters_add(x, x.clone(), a, b, o.place[:, 0].contiguous(), scales=pool[:4].view(torch.float32), out=out),
+              lambda: pm.adapters_add(x, x.clone(), pool.view(torch.bfloat16)[:4 * 8 * N].view(4, 8, N), b, torch.zeros_like(first), out=out)):
+        with pytest.raises(ValueError, match="must not overlap"):
+            f()
+    assert not pool.any()
