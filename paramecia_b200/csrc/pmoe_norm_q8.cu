@@ -23,6 +23,9 @@ __device__ inline float max_abs(float m, float v)
     return r;
 }
 
+// the same in 64 bits
+__device__ inline double max_nan(double m, double v) { return v > m || v != v ? v : m; }
+
 // How a group becomes 8 bits.  With u = r * weight and top = max |u| over the group, v = u / m and
 //   scale = max |v| / 127 = top * (1 / m) / 127,   v / scale = u * (127 / top):
 // the quotient needs neither m nor the rounded scale, which saves two products an element and lets both statistics be
@@ -264,7 +267,7 @@ __global__ void __launch_bounds__(THREADS, PASSES == 1 ? 2048 / THREADS : 1) k_n
             }
             double most = 0;
 #pragma unroll
-            for (int i = 0; i < 8; i++) most = fmax(most, fabs(d[i]));
+            for (int i = 0; i < 8; i++) most = max_nan(most, fabs(d[i]));
             return most;
         };
         auto store = [&](int p) {
@@ -290,19 +293,19 @@ __global__ void __launch_bounds__(THREADS, PASSES == 1 ? 2048 / THREADS : 1) k_n
                 t = products(p);
 #pragma unroll
                 for (int s = 1; s < 32; s <<= 1)
-                    if (s * 8 < group) t = fmax(t, __shfl_xor_sync(0xffffffffu, t, s));
+                    if (s * 8 < group) t = max_nan(t, __shfl_xor_sync(0xffffffffu, t, s));
                 store(p);
             }
         } else {
 #pragma unroll 1
-            for (int p = 0; p < PASSES; p++) t = fmax(t, products(p));
+            for (int p = 0; p < PASSES; p++) t = max_nan(t, products(p));
 #pragma unroll
-            for (int s = 16; s >= 1; s >>= 1) t = fmax(t, __shfl_xor_sync(0xffffffffu, t, s));
+            for (int s = 16; s >= 1; s >>= 1) t = max_nan(t, __shfl_xor_sync(0xffffffffu, t, s));
             if (lane == 0) red_exact[warp] = t;
             __syncthreads();
             t = lane < warps ? red_exact[lane] : 0.0;
 #pragma unroll
-            for (int s = 16; s >= 1; s >>= 1) t = fmax(t, __shfl_xor_sync(0xffffffffu, t, s));
+            for (int s = 16; s >= 1; s >>= 1) t = max_nan(t, __shfl_xor_sync(0xffffffffu, t, s));
 #pragma unroll 1
             for (int p = 0; p < PASSES; p++) {
                 if (PASSES > 1) products(p);
@@ -443,23 +446,23 @@ __global__ void __launch_bounds__(1024) k_norm_q8_any(const RT *resid_in, const 
                 for (int i0 = 0; i0 < 256; i0 += group) {
                     const int h0 = (p * warps + warp) * 256 + i0 + lane;
                     double t = 0;
-                    for (int k = 0; k < group; k += 32) t = fmax(t, fabs(product(h0 + k)));
+                    for (int k = 0; k < group; k += 32) t = max_nan(t, fabs(product(h0 + k)));
 #pragma unroll
-                    for (int s = 16; s >= 1; s >>= 1) t = fmax(t, __shfl_xor_sync(0xffffffffu, t, s));
+                    for (int s = 16; s >= 1; s >>= 1) t = max_nan(t, __shfl_xor_sync(0xffffffffu, t, s));
                     for (int k = 0; k < group; k += 32) store(h0 + k, t);
                 }
         } else {
             // over the elements that this thread wrote: no other thread touches their bytes
             double t = 0;
             for (int p = 0; p < PASSES; p++)
-                for (int i = 0; i < 256; i += 32) t = fmax(t, fabs(product((p * warps + warp) * 256 + i + lane)));
+                for (int i = 0; i < 256; i += 32) t = max_nan(t, fabs(product((p * warps + warp) * 256 + i + lane)));
 #pragma unroll
-            for (int s = 16; s >= 1; s >>= 1) t = fmax(t, __shfl_xor_sync(0xffffffffu, t, s));
+            for (int s = 16; s >= 1; s >>= 1) t = max_nan(t, __shfl_xor_sync(0xffffffffu, t, s));
             if (lane == 0) red_exact[warp] = t;
             __syncthreads();
             t = lane < warps ? red_exact[lane] : 0.0;
 #pragma unroll
-            for (int s = 16; s >= 1; s >>= 1) t = fmax(t, __shfl_xor_sync(0xffffffffu, t, s));
+            for (int s = 16; s >= 1; s >>= 1) t = max_nan(t, __shfl_xor_sync(0xffffffffu, t, s));
             for (int p = 0; p < PASSES; p++)
                 for (int i = 0; i < 256; i += 32) store((p * warps + warp) * 256 + i + lane, t);
         }

@@ -55,3 +55,20 @@ def test_quotients_beside_a_tie(H, group):
         top = int(np.abs(row).max())
         want = {int(d): nearest(Fraction(448 * abs(int(d)), top)) for d in set(row.tolist())}
         assert [np.sign(d) * want[int(d)] for d in row] == out.tolist()
+
+
+@pytest.mark.parametrize("q_dtype", [torch.int8, torch.float8_e4m3fn])
+@pytest.mark.parametrize("H, group", [(512, 32), (505, 64), (9000, 128)])
+def test_a_nan_weight_stays_in_its_group(H, group, q_dtype):
+    """The other groups' quotients are full of ties, which the 64-bit part rounds once more; the group without a scale is zeros."""
+    resid = (torch.arange(2 * H, device=DEV) % 33 - 16).float().view(2, H)        # 28 |d| of 448: 84, 168 and 336 are ties
+    resid[:, ::32] = 16.0
+    weight = torch.ones(H, device=DEV)
+    _, q, scales, values = pm.add_rms_norm_q8(resid, None, weight, 1e-6, group=group, q_dtype=q_dtype, values_dtype=torch.float32)
+    weight[group + 3] = float("nan")
+    _, q2, scales2, values2 = pm.add_rms_norm_q8(resid, None, weight, 1e-6, group=group, q_dtype=q_dtype, values_dtype=torch.float32)
+    inside = torch.zeros(H, dtype=torch.bool, device=DEV)
+    inside[group:2 * group] = True
+    assert torch.isnan(scales2[:, 1]).all() and torch.isnan(values2[:, inside]).all() and (q2[:, inside].float() == 0).all()
+    scales2[:, 1] = scales[:, 1]
+    assert torch.equal(scales, scales2) and torch.equal(q.float()[:, ~inside], q2.float()[:, ~inside]) and torch.equal(values[:, ~inside], values2[:, ~inside])
