@@ -331,7 +331,7 @@ int pmoe_add_rms_norm_q8(int device, const void *resid_in, int resid_dtype, cons
  *
  * pmoe_sort_pairs: offsets [E + 1] = number of kept pairs of the experts before e; place [n, top_k] = the pair's row in
  * expert order, -1 when it is skipped; order [n * top_k] = the pair at a row, -1 from row offsets[E] on.  Stable: pairs
- * of one expert stay in ascending order.  order or place may be NULL.  E <= 4096, n * top_k <= 2^30.
+ * of one expert stay in ascending order.  order or place may be NULL.  E <= 4096, n * top_k <= 2^30, expert_base + E < 2^31.
  *
  * In these entries and the two around them an output that lies over an input, or over another output, is refused
  * (PMOE_ERR_INVALID_ARG) but where a description allows it.
@@ -339,14 +339,14 @@ int pmoe_add_rms_norm_q8(int device, const void *resid_in, int resid_dtype, cons
 int pmoe_sort_pairs(int device, const uint32_t *idx, int n, int top_k, int expert_base, int E, int *order, int *place, int *offsets,
                     void *stream);
 
-/* out[place[p]] = x[p / top_k] for every kept pair, rows of row_bytes bytes of any type; the rows from offsets[E] on are
+/* out[place[p]] = x[p / top_k] for every kept pair, rows of row_bytes (up to 2^30) bytes of any type; the rows from offsets[E] on are
  * zeroed.  x [n, row_bytes], out [n * top_k, row_bytes], which must not overlap. */
 int pmoe_dispatch_rows(int device, const void *x, size_t row_bytes, int n, int top_k, const int *place, const int *offsets, int E,
                        void *out, void *stream);
 
 /* out[t] = sum_j w[t, j] * rows[place[t, j]] (+ extra[t]), f32 sums in slot order, rounded once; pairs whose place is
  * outside [0, n_rows) contribute nothing and their rows are not read.  w NULL = all ones, which is the gradient of
- * pmoe_dispatch_rows.  rows [n_rows, H], extra [n, H] (NULL = none), out [n, H], each F32 or BF16; extra may be out when
+ * pmoe_dispatch_rows.  rows [n_rows, H], extra [n, H] (NULL = none), out [n, H], each F32 or BF16, H <= 2^30; extra may be out when
  * their types are equal (MoeBlock::forward_with_stats adds the shared expert there, qwen3_next.rs:1932-1937). */
 int pmoe_combine_rows(int device, const void *rows, int rows_dtype, int n_rows, int n, int top_k, int H, const int *place,
                       const float *w, const void *extra, int extra_dtype, void *out, int out_dtype, void *stream);

@@ -8,6 +8,7 @@
 //   order[place_p] = p  (-1 from offsets[E] on).
 // The order is stable, so all of it is a function of idx alone (the block's grouping leaves the order inside an expert
 // to its atomics).
+#include <climits>
 #include <cooperative_groups.h>
 #include <initializer_list>
 #include <utility>
@@ -472,6 +473,8 @@ cudaError_t launch_combine_grad(const void *grad_out, int grad_dtype, const void
     });
 }
 
+constexpr int MAX_ROW = 1 << 30;   // a thread's place in a row and its step to the next one add up in 32 bits
+
 static int check_pairs(int n, int top_k, int E)
 {
     if (n < 0 || top_k <= 0 || (int64_t)n * top_k > (1 << 30)) return fail(PMOE_ERR_INVALID_ARG, "n >= 0, top_k >= 1 and n * top_k <= 2^30 are served");
@@ -490,7 +493,7 @@ int pmoe_sort_pairs(int device, const uint32_t *idx, int n, int top_k, int exper
 {
     int rc = check_pairs(n, top_k, E);
     if (rc) return rc;
-    if (expert_base < 0) return fail(PMOE_ERR_INVALID_ARG, "expert_base must not be negative");
+    if (expert_base < 0 || expert_base > INT_MAX - E) return fail(PMOE_ERR_INVALID_ARG, "expert_base must be 0 to 2^31 - 1 - E");
     if (!offsets || (n && !idx)) return fail(PMOE_ERR_INVALID_ARG, "idx / offsets is NULL");
     const size_t pairs = (size_t)n * top_k * sizeof(int);
     if (overlap({{order, pairs}, {place, pairs}, {offsets, ((size_t)E + 1) * sizeof(int)}}, {{idx, pairs}}))
@@ -506,7 +509,7 @@ int pmoe_dispatch_rows(int device, const void *x, size_t row_bytes, int n, int t
 {
     int rc = check_pairs(n, top_k, E);
     if (rc) return rc;
-    if (!row_bytes || row_bytes > (1u << 30)) return fail(PMOE_ERR_INVALID_ARG, "row_bytes must be 1 to 2^30");
+    if (!row_bytes || row_bytes > MAX_ROW) return fail(PMOE_ERR_INVALID_ARG, "row_bytes must be 1 to 2^30");
     if (!n) return PMOE_OK;
     if (!x || !place || !offsets || !out) return fail(PMOE_ERR_INVALID_ARG, "x / place / offsets / out is NULL");
     const size_t pairs = (size_t)n * top_k;
@@ -523,7 +526,7 @@ int pmoe_combine_rows(int device, const void *rows, int rows_dtype, int n_rows, 
 {
     int rc = check_pairs(n, top_k, 1);
     if (rc) return rc;
-    if (H <= 0 || n_rows < 0) return fail(PMOE_ERR_INVALID_ARG, "bad H / n_rows");
+    if (H <= 0 || H > MAX_ROW || n_rows < 0) return fail(PMOE_ERR_INVALID_ARG, "H must be 1 to 2^30 and n_rows not negative");
     if (!f32_or_bf16(rows_dtype) || !f32_or_bf16(out_dtype) || (extra && !f32_or_bf16(extra_dtype)))
         return fail(PMOE_ERR_UNSUPPORTED_DTYPE, "rows / extra / out must be F32 or BF16");
     if (!n) return PMOE_OK;
@@ -545,7 +548,7 @@ int pmoe_combine_rows_grad(int device, const void *grad_out, int grad_dtype, con
 {
     int rc = check_pairs(n, top_k, E);
     if (rc) return rc;
-    if (H <= 0) return fail(PMOE_ERR_INVALID_ARG, "bad H");
+    if (H <= 0 || H > MAX_ROW) return fail(PMOE_ERR_INVALID_ARG, "H must be 1 to 2^30");
     if (!f32_or_bf16(grad_dtype) || !f32_or_bf16(rows_dtype)) return fail(PMOE_ERR_UNSUPPORTED_DTYPE, "grad_out / rows must be F32 or BF16");
     if (!n) return PMOE_OK;
     if (!grad_rows && !grad_w) return fail(PMOE_ERR_INVALID_ARG, "neither grad_rows nor grad_w is asked for");

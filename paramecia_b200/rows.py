@@ -28,6 +28,8 @@ from .moe import _check_buffer
 _TYPES = {torch.float32: F32, torch.bfloat16: BF16}
 _Q_TYPES = {torch.int8: I8, torch.float8_e4m3fn: F8_E4M3}
 _MAX_EXPERTS = 4096
+_MAX_PAIRS = _MAX_ROW = 2 ** 30
+_MAX_INT = 2 ** 31 - 1
 
 
 # The current stream's handle by device index: what torch.cuda.current_stream(device).cuda_stream gives, without making the
@@ -37,6 +39,12 @@ _stream = torch._C._cuda_getCurrentRawStream
 
 def _f32(t: torch.Tensor) -> torch.Tensor:
     return t.contiguous() if t.dtype is torch.float32 else t.to(torch.float32).contiguous()
+
+
+def _at_most(limit: int, *sizes: int) -> None:
+    """Sizes go to the C entries as 32-bit numbers, which must not wrap on the way."""
+    if max(sizes) > limit:
+        raise PmoeError(-1, f"sizes up to {limit} are served here, got {max(sizes)}")
 
 
 def _on_gpu(what: str, t: torch.Tensor) -> torch.device:
@@ -122,11 +130,12 @@ def sort_by_expert(indices: torch.Tensor, num_experts: int, expert_base: int = 0
         raise ValueError("indices must be [n, top_k] or [n]")
     if not 1 <= int(num_experts) <= _MAX_EXPERTS:
         raise PmoeError(-3, f"1 to {_MAX_EXPERTS} experts are served, got {num_experts}")
-    if expert_base < 0:
-        raise ValueError("expert_base must not be negative")
+    if not 0 <= expert_base < 2 ** 31 - num_experts:
+        raise ValueError(f"expert_base must be 0 to 2^31 - 1 - num_experts, got {expert_base}")
     n, top_k = shape[0], shape[1] if len(shape) == 2 else 1
     if top_k == 0:
         raise ValueError("indices must have at least one slot")
+    _at_most(_MAX_PAIRS, n * top_k)
     idx = _ids("indices", indices)
     o = ExpertOrder(n, top_k, int(num_experts), device, int(expert_base))
     i = device.index
@@ -175,6 +184,7 @@ def _pair_rows(what: str, rows: torch.Tensor, order: ExpertOrder) -> Tuple[torch
     shape = rows.shape
     if len(shape) != 2 or shape[0] != order.n * order.top_k or shape[1] == 0:
         raise ValueError(f"{what} must be [{order.n * order.top_k}, H], got {tuple(shape)}")
+    _at_most(_MAX_ROW, shape[1])
     return rows.contiguous(), shape[0], shape[1]
 
 
@@ -253,6 +263,7 @@ def add_rms_norm_q8(resid: torch.Tensor, delta: Optional[torch.Tensor], weight: 
     if len(shape) != 2:
         raise ValueError("resid must be [n, H]")
     n, H = shape
+    _at_most(_MAX_INT, n, H)
     rd = _typed("resid", resid, device)
     r = resid.contiguous()
     d = dd = None
@@ -312,6 +323,7 @@ def adapters_add(base: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.
     n = x.shape[0] if x.dim() == 2 else -1
     if n < 0 or x.shape[1] != K or base.shape != (n, N):
         raise ValueError(f"x must be [n, {K}] and base [n, {N}], got {tuple(x.shape)} and {tuple(base.shape)}")
+    _at_most(_MAX_INT, n, K, N, r)
     if not isinstance(ids, torch.Tensor) or ids.device != device or ids.numel() != n:
         raise ValueError(f"ids must be [{n}] on {device}")
     if L > _MAX_EXPERTS:

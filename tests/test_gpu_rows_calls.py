@@ -95,3 +95,24 @@ def test_an_out_over_ids_weights_or_the_order_is_refused():
         with pytest.raises(ValueError, match="must not overlap"):
             f()
     assert not pool.any()
+
+
+def test_sizes_that_no_int_holds_are_refused():
+    """Views of one element with such shapes: a size that wraps must not reach the C entries as another one."""
+    one, ids = torch.ones(1, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV)
+    half = one.bfloat16()
+    o = pm.sort_by_expert(ids, 4)
+    big = 2 ** 32 + 8
+    for f in (lambda: pm.combine_rows(one.expand(1, big), o), lambda: pm.combine_rows_grad(one.expand(1, big), one.expand(1, big), o),
+              lambda: pm.sort_by_expert(ids.expand(big), 4), lambda: pm.sort_by_expert(ids.expand(2 ** 28, 5), 4),
+              lambda: pm.add_rms_norm_q8(one.expand(1, big), None, None, 1e-6), lambda: pm.add_rms_norm_q8(one.expand(big, 8), None, None, 1e-6),
+              lambda: pm.adapters_add(one.expand(1, 8), one.expand(1, big), half.expand(1, 8, big), half.expand(1, 8, 8), ids),
+              lambda: pm.adapters_add(one.expand(big, 8), one.expand(big, 8), half.expand(1, 8, 8), half.expand(1, 8, 8), ids.expand(big))):
+        with pytest.raises(pm.PmoeError) as e:
+            f()
+        assert e.value.code == -1
+    for base in (2 ** 32, 2 ** 31 - 4):
+        with pytest.raises(ValueError):
+            pm.sort_by_expert(ids, 4, expert_base=base)
+    assert pm.sort_by_expert(ids - 2 ** 31, 4, expert_base=2 ** 31 - 5).place.tolist() == [[-1]]
+    assert pm.sort_by_expert(ids.long() + 2 ** 40, 4, expert_base=2 ** 31 - 5).place.tolist() == [[-1]]

@@ -55,3 +55,12 @@ def test_ids_are_dense(dtype):
     for t in (table, table.t(), table[:, ::2], table.t()[1:]):
         got = rows._ids("ids", t)
         assert got.dtype == torch.int32 and got.is_contiguous() and got.tolist() == t.tolist()
+
+
+def test_sizes_beyond_the_kernels_numbers_are_refused():
+    """Columns are counted in 32 bits, a stride of the grid beyond them; ids behind the last 32-bit number are none."""
+    for H in ((1 << 31) - 1, (1 << 30) + 1):
+        assert pm.lib().pmoe_combine_rows(0, ROWS, pm.BF16, 1, 1, 1, H, PLACE, None, None, 0, OUT, pm.BF16, None) == INVALID
+        assert pm.lib().pmoe_combine_rows_grad(0, X, pm.BF16, ROWS, pm.BF16, 1, 1, H, PLACE, OFFSETS, 4, None, OUT, OUT2, None) == INVALID
+    for base in ((1 << 31) - 1, (1 << 31) - 16):
+        assert pm.lib().pmoe_sort_pairs(0, IDX, 1, 1, base, 16, ORDER, PLACE, OFFSETS, None) == INVALID
