@@ -36,9 +36,12 @@ __device__ inline void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// A pair of f32 values as PIECES pairs of bf16 whose sum is the value: three hold all 24 bits of it (8 + 8 + 8, each
-// remainder is exact), two hold 16.
-template <int PIECES> __device__ inline void split_pair(float lo, float hi, uint32_t (&w)[PIECES])
+// A pair of f32 values as three pairs of bf16 whose sum is the value: they hold all 24 bits of it (8 + 8 + 8, each remainder
+// is exact).  So do f32 rows and h, whatever the result's type: two pieces of h were off by 2^-17 of what the adapter adds, which
+// is more than a bf16 result's own rounding where its terms or base cancel.
+constexpr int PIECES = 3;
+
+__device__ inline void split_pair(float lo, float hi, uint32_t (&w)[PIECES])
 {
 #pragma unroll
     for (int p = 0; p < PIECES; p++) {
@@ -52,7 +55,7 @@ template <int PIECES> __device__ inline void split_pair(float lo, float hi, uint
 // second sixteen bytes lie one unit of the warp further).
 template <typename XT> struct XFrag;
 template <> struct XFrag<__nv_bfloat16> {
-    static constexpr int PIECES = 1;
+    static constexpr int WORDS = 1;
     static __device__ void words(const uint4 *p, uint32_t (&w)[4][1])
     {
         const uint4 v = p[0];
@@ -60,14 +63,14 @@ template <> struct XFrag<__nv_bfloat16> {
     }
 };
 template <> struct XFrag<float> {
-    static constexpr int PIECES = 3;
-    static __device__ void words(const uint4 *p, uint32_t (&w)[4][3])
+    static constexpr int WORDS = PIECES;
+    static __device__ void words(const uint4 *p, uint32_t (&w)[4][PIECES])
     {
         const float4 v0 = reinterpret_cast<const float4 *>(p)[0], v1 = reinterpret_cast<const float4 *>(p)[32];
-        split_pair<3>(v0.x, v0.y, w[0]);
-        split_pair<3>(v0.z, v0.w, w[1]);
-        split_pair<3>(v1.x, v1.y, w[2]);
-        split_pair<3>(v1.z, v1.w, w[3]);
+        split_pair(v0.x, v0.y, w[0]);
+        split_pair(v0.z, v0.w, w[1]);
+        split_pair(v1.x, v1.y, w[2]);
+        split_pair(v1.z, v1.w, w[3]);
     }
 };
 
@@ -286,7 +289,6 @@ __global__ void __launch_bounds__(FEW_THREADS, RT == 16 ? 1 : 4) k_adapters(Adap
     __shared__ int rows[FEW_M];
     __shared__ int tile_id, tile_rows, tile_first;
     __shared__ int all_ids[ADAPTER_ROWS_LEADER];
-    constexpr int HP = sizeof(OT) == 4 ? 3 : 2;   // pieces of h: an f32 result keeps all of it, a bf16 result 16 bits
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3;
     cg::cluster_group cluster = cg::this_cluster();
     const int ctas = (int)cluster.num_blocks(), c = (int)cluster.block_rank(), slot = blockIdx.x / ctas;
@@ -438,7 +440,7 @@ __global__ void __launch_bounds__(FEW_THREADS, RT == 16 ? 1 : 4) k_adapters(Adap
     float acc[RT][4] = {};
     for (int st = 0; st < kstages; st++) {
         landed();
-        constexpr int V = sizeof(XT) / 2, PC = XFrag<XT>::PIECES;
+        constexpr int V = sizeof(XT) / 2, PC = XFrag<XT>::WORDS;
         const uint4 *rv = reinterpret_cast<const uint4 *>(my_rows + buffer);
         const uint4 *av = reinterpret_cast<const uint4 *>(my_weights + buffer) + lane;
         uint32_t w0[4][PC], w1[4][PC];
@@ -505,19 +507,19 @@ __global__ void __launch_bounds__(FEW_THREADS, RT == 16 ? 1 : 4) k_adapters(Adap
     // 4 (i / 2) + 2 j + i % 2 of the first or second half, four consecutive ones of each).  Ranks: a lane takes four
     // (RT = 2) or eight consecutive ones, which are one or two steps of the matrix instruction.
     constexpr int KS = RT / 2;
-    uint32_t hf[KS][HP][4];
+    uint32_t hf[KS][PIECES][4];
 #pragma unroll
     for (int s = 0; s < KS; s++) {
         const int k = RT == 2 ? q * 4 : s / 2 * 32 + q * 8 + s % 2 * 4;
         const float4 v0 = *reinterpret_cast<const float4 *>(h + g * HS + k);
         const float4 v1 = *reinterpret_cast<const float4 *>(h + (g + 8) * HS + k);
-        uint32_t w[4][HP];
-        split_pair<HP>(v0.x, v0.y, w[0]);
-        split_pair<HP>(v1.x, v1.y, w[1]);
-        split_pair<HP>(v0.z, v0.w, w[2]);
-        split_pair<HP>(v1.z, v1.w, w[3]);
+        uint32_t w[4][PIECES];
+        split_pair(v0.x, v0.y, w[0]);
+        split_pair(v1.x, v1.y, w[1]);
+        split_pair(v0.z, v0.w, w[2]);
+        split_pair(v1.z, v1.w, w[3]);
 #pragma unroll
-        for (int p = 0; p < HP; p++)
+        for (int p = 0; p < PIECES; p++)
 #pragma unroll
             for (int i = 0; i < 4; i++) hf[s][p][i] = w[i][p];
     }
@@ -533,7 +535,7 @@ __global__ void __launch_bounds__(FEW_THREADS, RT == 16 ? 1 : 4) k_adapters(Adap
 #pragma unroll
             for (int j = 0; j < 4; j++) v[j] = reinterpret_cast<const uint2 *>(wv)[j * 32 + lane];
 #pragma unroll
-            for (int p = 0; p < HP; p++)
+            for (int p = 0; p < PIECES; p++)
 #pragma unroll
                 for (int j = 0; j < 4; j++) mma_bf16(o[j], hf[0][p][0], hf[0][p][1], hf[0][p][2], hf[0][p][3], v[j].x, v[j].y);
         } else {
@@ -543,7 +545,7 @@ __global__ void __launch_bounds__(FEW_THREADS, RT == 16 ? 1 : 4) k_adapters(Adap
 #pragma unroll
                 for (int j = 0; j < 4; j++) v[j] = reinterpret_cast<const uint4 *>(wv)[(j * (RT / 4) + s) * 32 + lane];
 #pragma unroll
-                for (int p = 0; p < HP; p++) {
+                for (int p = 0; p < PIECES; p++) {
 #pragma unroll
                     for (int j = 0; j < 4; j++)
                         mma_bf16(o[j], hf[2 * s][p][0], hf[2 * s][p][1], hf[2 * s][p][2], hf[2 * s][p][3], v[j].x, v[j].y);
@@ -581,8 +583,7 @@ __global__ void __launch_bounds__(FEW_THREADS, RT == 16 ? 1 : 4) k_adapters(Adap
 // 42 us for this part).  Here a tile of 128 rows of one adapter is the M of tcgen05.mma, read from shared memory and summed in
 // tensor memory:
 //   h[128, r]     = X[128, K] A^T   stages of 64 of K: the rows' and A's pieces of 128 bytes, 128-byte swizzle
-//   out[128, 128] = H B^T + base    chunks of 128 columns, h as two bf16 pieces (16 bits of it; three for an
-//                                 f32 result, all of it), each its own product
+//   out[128, 128] = H B^T + base    chunks of 128 columns, each of h's three bf16 pieces its own product
 // with the cluster's exchange of h between them as above.  All threads copy (asynchronously, LEAD stages ahead), one
 // issues the products, and a chunk's sums are read, added to base and stored while the next chunk's product runs.  The
 // columns of B lie permuted in shared memory so that a lane reads eight consecutive ones of a row.
@@ -596,8 +597,7 @@ template <typename OT, int RT> struct TcTile {
     static constexpr int X_BYTES = TC_M * 128, A_BYTES = R * 128, B_BYTES = KB * 128 * 128;
     static constexpr int STAGE = X_BYTES + A_BYTES > B_BYTES ? X_BYTES + A_BYTES : B_BYTES;
     static constexpr int PS = R + 4;                                  // floats between two rows of this CTA's share of h
-    static constexpr int HP = sizeof(OT) == 4 ? 3 : 2;                // pieces of h
-    static constexpr int PART = TC_M * PS * 4, H_BYTES = HP * KB * TC_M * 128;
+    static constexpr int PART = TC_M * PS * 4, H_BYTES = PIECES * KB * TC_M * 128;
     static constexpr bool OVERLAY = RT == 16;                         // the share lies over the stages, which wait for the exchange
     static constexpr int ROOM = 218 * 1024 - H_BYTES - (OVERLAY ? 0 : PART);
     static constexpr int STAGES = ROOM / STAGE > 6 ? 6 : ROOM / STAGE;
@@ -629,7 +629,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_adapters_tc(AdapterArgs P, co
     cg::cluster_group cluster = cg::this_cluster();
     const int ctas = (int)cluster.num_blocks(), c = (int)cluster.block_rank(), slot = blockIdx.x / ctas;
     uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);   // the swizzle counts from 1024-byte boundaries
-    uint8_t *hs = smem + S::STAGES * S::STAGE;                                      // [HP][KB][128 rows of 128 bytes]
+    uint8_t *hs = smem + S::STAGES * S::STAGE;                                      // [PIECES][KB][128 rows of 128 bytes]
     float *part = reinterpret_cast<float *>(S::OVERLAY ? smem : hs + S::H_BYTES);   // [128][PS]
     pdl_wait();
     pdl_launch_dependents();
@@ -750,17 +750,17 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_adapters_tc(AdapterArgs P, co
         for (int i = c * TC_THREADS + tid; i < TC_M * RT; i += CTAS * TC_THREADS) {   // eight ranks of a row
             const int row = i / RT, k8 = i % RT;
             const float4 u = sum_of_cluster<CTAS>(cluster, part + row * S::PS + k8 * 8), v = sum_of_cluster<CTAS>(cluster, part + row * S::PS + k8 * 8 + 4);
-            uint32_t w[4][S::HP];
-            split_pair<S::HP>(u.x * scale, u.y * scale, w[0]);
-            split_pair<S::HP>(u.z * scale, u.w * scale, w[1]);
-            split_pair<S::HP>(v.x * scale, v.y * scale, w[2]);
-            split_pair<S::HP>(v.z * scale, v.w * scale, w[3]);
+            uint32_t w[4][PIECES];
+            split_pair(u.x * scale, u.y * scale, w[0]);
+            split_pair(u.z * scale, u.w * scale, w[1]);
+            split_pair(v.x * scale, v.y * scale, w[2]);
+            split_pair(v.z * scale, v.w * scale, w[3]);
             uint8_t *at = hs + k8 / 8 * (TC_M * 128) + row * 128 + ((k8 % 8 ^ row % 8) << 4);
 #pragma unroll
             for (int o = 0; o < CTAS; o++) {
                 uint8_t *there = cluster.map_shared_rank(at, o);
 #pragma unroll
-                for (int p = 0; p < S::HP; p++)
+                for (int p = 0; p < PIECES; p++)
                     *reinterpret_cast<uint4 *>(there + p * S::KB * TC_M * 128) = make_uint4(w[0][p], w[1][p], w[2][p], w[3][p]);
             }
         }
@@ -842,7 +842,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_adapters_tc(AdapterArgs P, co
             tc_fence_after();
             const uint8_t *buffer = smem + ((kst + st) % S::STAGES) * S::STAGE;
 #pragma unroll
-            for (int p = 0; p < S::HP; p++)
+            for (int p = 0; p < PIECES; p++)
 #pragma unroll
                 for (int kb = 0; kb < S::KB; kb++) {
                     const uint64_t da = smem_desc_sw128(hs + (p * S::KB + kb) * TC_M * 128), db = smem_desc_sw128(buffer + kb * 16384);
