@@ -37,7 +37,8 @@ __device__ inline void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_
 }
 
 // A pair of f32 values as three pairs of bf16 whose sum is the value: they hold all 24 bits of it (8 + 8 + 8, each remainder
-// is exact).  So do f32 rows and h, whatever the result's type: two pieces of h were off by 2^-17 of what the adapter adds, which
+// is exact: the upper half of the bits left is cut off, which makes no infinity of a large number).  An infinity has no remainder; a
+// NaN's is one, also where its upper half is an infinity's.  So do f32 rows and h, whatever the result's type: two pieces of h were off by 2^-17 of what the adapter adds, which
 // is more than a bf16 result's own rounding where its terms or base cancel.
 constexpr int PIECES = 3;
 
@@ -45,9 +46,11 @@ __device__ inline void split_pair(float lo, float hi, uint32_t (&w)[PIECES])
 {
 #pragma unroll
     for (int p = 0; p < PIECES; p++) {
-        w[p] = pack_bf16(lo, hi);
-        lo -= __uint_as_float(w[p] << 16);
-        hi -= __uint_as_float(w[p] & 0xffff0000u);
+        const uint32_t l = __float_as_uint(lo), h = __float_as_uint(hi);
+        w[p] = __byte_perm(l, h, 0x7632);
+        const float rest_l = lo - __uint_as_float(l & 0xffff0000u), rest_h = hi - __uint_as_float(h & 0xffff0000u);
+        lo = p == 0 && fabsf(lo) == INFINITY ? 0.f : rest_l;
+        hi = p == 0 && fabsf(hi) == INFINITY ? 0.f : rest_h;
     }
 }
 
@@ -497,7 +500,8 @@ __global__ void __launch_bounds__(FEW_THREADS, RT == 16 ? 1 : 4) k_adapters(Adap
         for (int i = tid; i < FEW_M * per_row; i += FEW_THREADS) {
             const int at = i / per_row * HS + i % per_row * 4;
             const float4 s = sum_of_cluster<CTAS>(cluster, part + at);
-            *reinterpret_cast<float4 *>(h + at) = make_float4(s.x * scale, s.y * scale, s.z * scale, s.w * scale);
+            const bool rank = i % per_row * 4 < P.r;   // ranks behind r are zeros, also where x is infinite
+            *reinterpret_cast<float4 *>(h + at) = rank ? make_float4(s.x * scale, s.y * scale, s.z * scale, s.w * scale) : make_float4(0.f, 0.f, 0.f, 0.f);
         }
     });
     __syncthreads();
@@ -751,10 +755,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_adapters_tc(AdapterArgs P, co
             const int row = i / RT, k8 = i % RT;
             const float4 u = sum_of_cluster<CTAS>(cluster, part + row * S::PS + k8 * 8), v = sum_of_cluster<CTAS>(cluster, part + row * S::PS + k8 * 8 + 4);
             uint32_t w[4][PIECES];
-            split_pair(u.x * scale, u.y * scale, w[0]);
-            split_pair(u.z * scale, u.w * scale, w[1]);
-            split_pair(v.x * scale, v.y * scale, w[2]);
-            split_pair(v.z * scale, v.w * scale, w[3]);
+            const bool rank = k8 * 8 < P.r;   // ranks behind r are zeros, also where x is infinite
+            split_pair(rank ? u.x * scale : 0.f, rank ? u.y * scale : 0.f, w[0]);
+            split_pair(rank ? u.z * scale : 0.f, rank ? u.w * scale : 0.f, w[1]);
+            split_pair(rank ? v.x * scale : 0.f, rank ? v.y * scale : 0.f, w[2]);
+            split_pair(rank ? v.z * scale : 0.f, rank ? v.w * scale : 0.f, w[3]);
             uint8_t *at = hs + k8 / 8 * (TC_M * 128) + row * 128 + ((k8 % 8 ^ row % 8) << 4);
 #pragma unroll
             for (int o = 0; o < CTAS; o++) {

@@ -1,4 +1,5 @@
-"""Low-rank adapters at values where the bits of h and the special values matter.  Everything is chosen so that f32 sums are exact."""
+"""Low-rank adapters at values where the bits of h and the special values matter.  Values are chosen so that f32 sums are exact, but for
+one sum whose bound stands beside it."""
 import pytest
 import torch
 
@@ -30,3 +31,38 @@ def test_h_keeps_the_bits_of_f32(n, r, xt, bt):
     b[0, :, 0], b[0, :, 1] = 1.0, -1.0
     got = pm.adapters_add(torch.zeros((n, N), dtype=bt, device=DEV), x.to(xt), a, b, torch.zeros(n, dtype=torch.int32, device=DEV))
     assert torch.equal(got, torch.full_like(got, 2.0 ** -18))
+
+
+@pytest.mark.parametrize("xt, bt", TYPES)
+@pytest.mark.parametrize("r", [8, 16, 24, 64, 128])
+@pytest.mark.parametrize("n", ROWS)
+def test_infinities_stay_infinities(n, r, xt, bt):
+    """With A and B positive an infinity of x, or of a sum that overflows, is one of the same sign in its row, whatever lies behind
+    the rank and behind K; the largest numbers stay numbers, and a NaN is one, be it in the lowest bits."""
+    K, N, inf = 72, 40, float("inf")
+    most = torch.finfo(xt).max
+    a = torch.full((1, r, K), 2.0 ** -8, dtype=bf16, device=DEV)
+    b = torch.full((1, N, r), 2.0 ** -9, dtype=bf16, device=DEV)
+    x = torch.zeros((n, K), dtype=xt, device=DEV)
+    at = [0, n // 3, n // 2, n - 1]
+    for first, value, want in ((0, inf, inf), (1, -inf, -inf), (2, most, None), (3, float("nan"), float("nan"))):
+        x.zero_()
+        x[at[first], 5] = value
+        if value != value and xt == f32:
+            x.view(torch.int32)[at[first], 5] = 0x7f800001
+        got = pm.adapters_add(torch.zeros((n, N), dtype=bt, device=DEV), x, a, b, torch.zeros(n, dtype=torch.int32, device=DEV))
+        row = got[at[first]].clone()
+        got[at[first]] = 0
+        assert (got == 0).all()
+        if want is None:
+            # h is exact; the second product adds r equal terms in three pieces.  Three such terms of 24 bits need 26, so partial sums
+            # are not exact: the matrix unit aligns the seventeen addends of a step of sixteen ranks and cuts each at 2^-23 of the sum
+            # at most, in 3 * ceil(r / 16) steps.  Then one rounding to the result's type.
+            exact = most * 2.0 ** -17 * r
+            assert ((row.double() - exact).abs() <= (3 * -(-r // 16) * 17 * 2.0 ** -23 + torch.finfo(bt).eps / 2) * exact).all()
+        else:
+            assert torch.equal(row.float().nan_to_num(7.0, 8.0, 9.0), torch.full_like(row.float(), want).nan_to_num(7.0, 8.0, 9.0))
+    x.zero_()
+    x[0, :2] = most     # both h and the result overflow
+    got = pm.adapters_add(torch.zeros((n, N), dtype=bt, device=DEV), x, a * 2.0 ** 9, b * 2.0 ** 9, torch.zeros(n, dtype=torch.int32, device=DEV))
+    assert (got[0] == inf).all() and (got[1:] == 0).all()
