@@ -370,9 +370,10 @@ int pmoe_adapters_add(int device, const void *base, const void *x, int x_dtype, 
                       const void *a, const void *b, const float *scales, const int *ids, const int *order, const int *offsets, void *out,
                       int out_dtype, void *stream);
 
-/* Synchronises the stream and reports the device-side status word of pmoe_adapters_add (PMOE_OK, or PMOE_ERR_TIMEOUT when a
- * bounded wait inside a kernel ran out and its output is not to be used), clearing it: pmoe_layer_status for the operators
- * that have no handle. */
+/* Synchronises the stream and reports whether a bounded wait inside pmoe_adapters_add ran out (PMOE_ERR_TIMEOUT, else PMOE_OK)
+ * on this device since the last call with this stream, or since the library was loaded: pmoe_layer_status for the operators that
+ * have no handle.  The kernels only count, so the call does not say whose wait it was: every output of the device since then, of
+ * any stream, is suspect, and every stream that asks hears of it, once. */
 int pmoe_rows_status(int device, void *stream);
 
 /*

@@ -13,6 +13,7 @@
 #include <cooperative_groups.h>
 
 #include "pmoe_internal.h"
+#include "pmoe_status.h"
 #include "pmoe_tcgen05.cuh"
 #include "pmoe_vec.cuh"
 
@@ -594,7 +595,12 @@ __global__ void __launch_bounds__(FEW_THREADS, RT == 16 ? 1 : 4) k_adapters(Adap
 constexpr int TC_M = 128, TC_THREADS = 256;
 constexpr int TC_MIN_ROWS = 96;   // rows an adapter has on average
 
-__device__ DevStatus g_rows_status;   // a wait that ran out (pmoe_rows_status)
+// Waits that ran out, of all streams since the library was loaded (pmoe_rows_status), and where the last one was
+struct Failures {
+    unsigned count;
+    int detail;
+};
+__device__ Failures g_failures;
 
 template <typename OT, int RT> struct TcTile {
     static constexpr int R = RT * 8, KB = (R + 63) / 64;              // ranks, blocks of 64 of them
@@ -659,7 +665,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_adapters_tc(AdapterArgs P, co
     auto product_done = [&](int use) {
         if (ok && !mbar_wait_spin(&bars[use % S::STAGES], (use / S::STAGES) & 1)) {
             ok = false;
-            set_status(&g_rows_status, PMOE_ERR_TIMEOUT, 40, use);
+            atomicExch(&g_failures.detail, use);
+            atomicAdd(&g_failures.count, 1u);
         }
     };
 
@@ -1011,13 +1018,14 @@ extern "C" int pmoe_rows_status(int device, void *stream)
     DeviceGuard guard(device);
     if (!guard.ok) return fail(PMOE_ERR_NO_DEVICE, "cannot select device %d", device);
     cudaStream_t s = (cudaStream_t)stream;
-    DevStatus st{}, zero{};
-    CU(cudaMemcpyFromSymbolAsync(&st, g_rows_status, sizeof st, 0, cudaMemcpyDeviceToHost, s));
+    Failures f{};
+    CU(cudaMemcpyFromSymbolAsync(&f, g_failures, sizeof f, 0, cudaMemcpyDeviceToHost, s));
     CU(cudaStreamSynchronize(s));
-    if (st.code) {
-        CU(cudaMemcpyToSymbolAsync(g_rows_status, &zero, sizeof zero, 0, cudaMemcpyHostToDevice, s));
-        CU(cudaStreamSynchronize(s));
-        return fail(st.code, "device status %d raised by kernel tag %d (detail %d)", st.code, st.where, st.detail);
+    static FailureCounts counts;
+    bool news = f.count != 0;
+    try {
+        news = counts.news(device, stream, f.count);
+    } catch (...) {   // no memory for a stream's entry: an old failure is reported once more
     }
-    return PMOE_OK;
+    return news ? fail(PMOE_ERR_TIMEOUT, "a wait inside pmoe_adapters_add ran out (%u so far, the last at stage %d)", f.count, f.detail) : PMOE_OK;
 }

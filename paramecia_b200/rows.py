@@ -368,8 +368,9 @@ def _aligned(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
 
 
 def rows_status(device="cuda") -> None:
-    """Synchronises the current stream of `device` and raises PmoeError if a bounded wait inside ``adapters_add`` ran out
-    (its output is then not to be used): ``MoeBlock.status`` for the operators that have no handle."""
+    """Synchronises the current stream of `device` and raises PmoeError if a bounded wait inside ``adapters_add`` ran out on it, on
+    any stream, since this stream's last call (since the library was loaded, if it has made none): outputs from then on are not to
+    be used.  Every stream that asks hears of it once.  ``MoeBlock.status`` for the operators that have no handle."""
     d = torch.device(device)
     if d.type != "cuda":
         raise PmoeError(-9, "rows_status needs a CUDA device; libpmoe has no CPU path")
