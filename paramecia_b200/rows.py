@@ -37,8 +37,20 @@ _MAX_INT = 2 ** 31 - 1
 _stream = torch._C._cuda_getCurrentRawStream
 
 
+def _dense(t: torch.Tensor) -> torch.Tensor:
+    """The tensor contiguous, and its values in memory as they are (torch may mark a view as negative instead)."""
+    t = t.contiguous()
+    return t.resolve_neg() if t.is_neg() else t
+
+
 def _f32(t: torch.Tensor) -> torch.Tensor:
-    return t.contiguous() if t.dtype is torch.float32 else t.to(torch.float32).contiguous()
+    return _dense(t if t.dtype is torch.float32 else t.to(torch.float32))
+
+
+def _check_out(out: torch.Tensor, shape, dtype, device) -> None:
+    _check_buffer("out", out, shape, dtype, device)
+    if out.is_neg() or out.is_conj():
+        raise ValueError("out must not be a conjugate or negated view")
 
 
 def _at_most(limit: int, *sizes: int) -> None:
@@ -158,11 +170,11 @@ def dispatch_rows(x: torch.Tensor, order: ExpertOrder, out: Optional[torch.Tenso
     shape, n, top_k = x.shape, order.n, order.top_k
     if len(shape) != 2 or shape[0] != n:
         raise ValueError(f"x must be [{n}, H], got {tuple(shape)}")
-    x, H = x.contiguous(), shape[1]
+    x, H = _dense(x.resolve_conj()), shape[1]
     if out is None:
         out = torch.empty(n * top_k, H, dtype=x.dtype, device=device)
     else:
-        _check_buffer("out", out, (n * top_k, H), x.dtype, device)
+        _check_out(out, (n * top_k, H), x.dtype, device)
         _apart("x", out, x)
         _apart("order", out, order._data)
     if H == 0:
@@ -185,7 +197,7 @@ def _pair_rows(what: str, rows: torch.Tensor, order: ExpertOrder) -> Tuple[torch
     if len(shape) != 2 or shape[0] != order.n * order.top_k or shape[1] == 0:
         raise ValueError(f"{what} must be [{order.n * order.top_k}, H], got {tuple(shape)}")
     _at_most(_MAX_ROW, shape[1])
-    return rows.contiguous(), shape[0], shape[1]
+    return _dense(rows), shape[0], shape[1]
 
 
 def combine_rows(rows: torch.Tensor, order: ExpertOrder, weights: Optional[torch.Tensor] = None,
@@ -205,12 +217,12 @@ def combine_rows(rows: torch.Tensor, order: ExpertOrder, weights: Optional[torch
         ed = _typed("extra", extra, device)
         if extra.shape != (n, H):
             raise ValueError(f"extra must be {(n, H)}, got {tuple(extra.shape)}")
-        e = extra.contiguous()
+        e = _dense(extra)
     if out is None:
         od = rd if out_dtype is None else _out_type("out_dtype", out_dtype)
         out = torch.empty(n, H, dtype=out_dtype or rows.dtype, device=device)
     else:
-        _check_buffer("out", out, (n, H), tuple(_TYPES), device)
+        _check_out(out, (n, H), tuple(_TYPES), device)
         _apart("rows", out, rows)
         _apart("extra", out, e, same=True)
         _apart("weights", out, w)
@@ -239,7 +251,7 @@ def combine_rows_grad(grad_out: torch.Tensor, rows: torch.Tensor, order: ExpertO
     n, top_k = order.n, order.top_k
     if grad_out.shape != (n, H):
         raise ValueError(f"grad_out must be {(n, H)}, got {tuple(grad_out.shape)}")
-    g = grad_out.contiguous()
+    g = _dense(grad_out)
     w = None if weights is None else _pair_weights(weights, order, device)
     grad_rows = torch.empty_like(rows)
     grad_w = torch.empty(n, top_k, dtype=torch.float32, device=device)
@@ -265,13 +277,13 @@ def add_rms_norm_q8(resid: torch.Tensor, delta: Optional[torch.Tensor], weight: 
     n, H = shape
     _at_most(_MAX_INT, n, H)
     rd = _typed("resid", resid, device)
-    r = resid.contiguous()
+    r = _dense(resid)
     d = dd = None
     if delta is not None:
         dd = _typed("delta", delta, device)
         if delta.shape != shape:
             raise ValueError(f"delta must be {(n, H)}, got {tuple(delta.shape)}")
-        d = delta.contiguous()
+        d = _dense(delta)
     w = None
     if weight is not None:
         if not isinstance(weight, torch.Tensor) or weight.device != device or weight.shape != (H,):
@@ -333,6 +345,8 @@ def adapters_add(base: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.
         if not isinstance(scales, torch.Tensor) or scales.device != device or scales.numel() != L:
             raise ValueError(f"scales must be [{L}] on {device}")
         s = _f32(scales)
+    if x.is_neg() or base.is_neg():
+        x, base = x.resolve_neg(), base.resolve_neg()
     (x, xp), (a, ap), (b, bp), (base, basep) = _aligned(x), _aligned(a), _aligned(b), _aligned(base)
     ids = _ids("ids", ids if ids.dim() == 1 else ids.reshape(-1))
     if order is not None:
@@ -344,7 +358,7 @@ def adapters_add(base: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.
     if out is None:
         out = torch.empty_like(base)
     else:
-        _check_buffer("out", out, (n, N), base.dtype, device)
+        _check_out(out, (n, N), base.dtype, device)
         if out.data_ptr() % 16:
             raise ValueError("out must be 16-byte aligned")
         _apart("base", out, base, same=True)

@@ -116,3 +116,32 @@ def test_sizes_that_no_int_holds_are_refused():
             pm.sort_by_expert(ids, 4, expert_base=base)
     assert pm.sort_by_expert(ids - 2 ** 31, 4, expert_base=2 ** 31 - 5).place.tolist() == [[-1]]
     assert pm.sort_by_expert(ids.long() + 2 ** 40, 4, expert_base=2 ** 31 - 5).place.tolist() == [[-1]]
+
+
+def test_views_that_negate_or_conjugate():
+    """torch keeps a conjugate, and the imaginary part of one, as a view with a mark: the memory holds the other sign."""
+    z = torch.complex(*torch.randn((2, 30, 64), device=DEV).unbind(0))
+    ids = torch.arange(60, dtype=torch.int32, device=DEV).view(30, 2) % 7
+    o = pm.sort_by_expert(ids, 7)
+    pair = o.order.long()
+    assert z.conj().is_conj() and z.conj().imag.is_neg()
+    assert torch.equal(pm.dispatch_rows(z.conj(), o), z.conj().resolve_conj()[pair // 2])
+    neg = z.conj().imag                       # strided, negative
+    flat = torch._neg_view(neg.contiguous())  # dense, negative
+    for v in (neg, flat):
+        plain = v.clone().resolve_neg()
+        assert v.is_neg() and not plain.is_neg()
+        assert torch.equal(pm.dispatch_rows(v, o), plain[pair // 2])
+        rows, want = pm.dispatch_rows(plain, o), pm.dispatch_rows(plain, o)
+        neg_rows = torch._neg_view(-rows)
+        w = torch._neg_view(-torch.rand((30, 2), device=DEV))
+        assert torch.equal(pm.combine_rows(neg_rows, o, w, extra=v), pm.combine_rows(want, o, w.clone().resolve_neg(), extra=plain))
+        for a, b in zip(pm.combine_rows_grad(v, neg_rows, o, w), pm.combine_rows_grad(plain, want, o, w.clone().resolve_neg())):
+            assert torch.equal(a, b)
+        for a, b in zip(pm.add_rms_norm_q8(v, v, v[0], 1e-6)[:3], pm.add_rms_norm_q8(plain, plain, plain[0], 1e-6)[:3]):
+            assert torch.equal(a, b)
+        a, b = (torch.randn(s, device=DEV).bfloat16() for s in ((7, 8, 64), (7, 64, 8)))
+        first = ids[:, 0].contiguous()
+        assert torch.equal(pm.adapters_add(v, v, a, b, first), pm.adapters_add(plain, plain, a, b, first))
+    with pytest.raises(ValueError):
+        pm.combine_rows(want, o, out=torch._neg_view(torch.zeros((30, 64), device=DEV)))
