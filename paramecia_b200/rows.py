@@ -37,10 +37,11 @@ _MAX_INT = 2 ** 31 - 1
 _stream = torch._C._cuda_getCurrentRawStream
 
 
-def _dense(t: torch.Tensor) -> torch.Tensor:
-    """The tensor contiguous, and its values in memory as they are (torch may mark a view as negative instead)."""
+def _dense(t: torch.Tensor, dtype: int = F32) -> torch.Tensor:
+    """The tensor contiguous, and its values in memory as they are: torch may mark a view as negative instead, one of f32 (half of a
+    complex number) but not of bf16."""
     t = t.contiguous()
-    return t.resolve_neg() if t.is_neg() else t
+    return t.resolve_neg() if dtype == F32 and t.is_neg() else t
 
 
 def _f32(t: torch.Tensor) -> torch.Tensor:
@@ -53,10 +54,9 @@ def _check_out(out: torch.Tensor, shape, dtype, device) -> None:
         raise ValueError("out must not be a conjugate or negated view")
 
 
-def _at_most(limit: int, *sizes: int) -> None:
+def _too_large(limit: int, *sizes: int) -> PmoeError:
     """Sizes go to the C entries as 32-bit numbers, which must not wrap on the way."""
-    if max(sizes) > limit:
-        raise PmoeError(-1, f"sizes up to {limit} are served here, got {max(sizes)}")
+    return PmoeError(-1, f"sizes up to {limit} are served here, got {max(sizes)}")
 
 
 def _on_gpu(what: str, t: torch.Tensor) -> torch.device:
@@ -147,7 +147,8 @@ def sort_by_expert(indices: torch.Tensor, num_experts: int, expert_base: int = 0
     n, top_k = shape[0], shape[1] if len(shape) == 2 else 1
     if top_k == 0:
         raise ValueError("indices must have at least one slot")
-    _at_most(_MAX_PAIRS, n * top_k)
+    if n * top_k > _MAX_PAIRS:
+        raise _too_large(_MAX_PAIRS, n * top_k)
     idx = _ids("indices", indices)
     o = ExpertOrder(n, top_k, int(num_experts), device, int(expert_base))
     i = device.index
@@ -170,7 +171,9 @@ def dispatch_rows(x: torch.Tensor, order: ExpertOrder, out: Optional[torch.Tenso
     shape, n, top_k = x.shape, order.n, order.top_k
     if len(shape) != 2 or shape[0] != n:
         raise ValueError(f"x must be [{n}, H], got {tuple(shape)}")
-    x, H = _dense(x.resolve_conj()), shape[1]
+    if x.is_conj():
+        x = x.resolve_conj()
+    x, H = _dense(x), shape[1]
     if out is None:
         out = torch.empty(n * top_k, H, dtype=x.dtype, device=device)
     else:
@@ -191,13 +194,14 @@ def _pair_weights(weights: torch.Tensor, order: ExpertOrder, device) -> torch.Te
     return _f32(weights)
 
 
-def _pair_rows(what: str, rows: torch.Tensor, order: ExpertOrder) -> Tuple[torch.Tensor, int, int]:
+def _pair_rows(what: str, rows: torch.Tensor, dtype: int, order: ExpertOrder) -> Tuple[torch.Tensor, int, int]:
     """The rows contiguous, their number and their length."""
     shape = rows.shape
     if len(shape) != 2 or shape[0] != order.n * order.top_k or shape[1] == 0:
         raise ValueError(f"{what} must be [{order.n * order.top_k}, H], got {tuple(shape)}")
-    _at_most(_MAX_ROW, shape[1])
-    return _dense(rows), shape[0], shape[1]
+    if shape[1] > _MAX_ROW:
+        raise _too_large(_MAX_ROW, shape[1])
+    return _dense(rows, dtype), shape[0], shape[1]
 
 
 def combine_rows(rows: torch.Tensor, order: ExpertOrder, weights: Optional[torch.Tensor] = None,
@@ -209,7 +213,7 @@ def combine_rows(rows: torch.Tensor, order: ExpertOrder, weights: Optional[torch
     device = _on_gpu("rows", rows)
     _ordered(order, device)
     rd = _typed("rows", rows, device)
-    rows, pairs, H = _pair_rows("rows", rows, order)
+    rows, pairs, H = _pair_rows("rows", rows, rd, order)
     n = order.n
     w = None if weights is None else _pair_weights(weights, order, device)
     e, ed = None, 0
@@ -217,7 +221,7 @@ def combine_rows(rows: torch.Tensor, order: ExpertOrder, weights: Optional[torch
         ed = _typed("extra", extra, device)
         if extra.shape != (n, H):
             raise ValueError(f"extra must be {(n, H)}, got {tuple(extra.shape)}")
-        e = _dense(extra)
+        e = _dense(extra, ed)
     if out is None:
         od = rd if out_dtype is None else _out_type("out_dtype", out_dtype)
         out = torch.empty(n, H, dtype=out_dtype or rows.dtype, device=device)
@@ -247,11 +251,11 @@ def combine_rows_grad(grad_out: torch.Tensor, rows: torch.Tensor, order: ExpertO
     device = _on_gpu("grad_out", grad_out)
     _ordered(order, device)
     gd, rd = _typed("grad_out", grad_out, device), _typed("rows", rows, device)
-    rows, pairs, H = _pair_rows("rows", rows, order)
+    rows, pairs, H = _pair_rows("rows", rows, rd, order)
     n, top_k = order.n, order.top_k
     if grad_out.shape != (n, H):
         raise ValueError(f"grad_out must be {(n, H)}, got {tuple(grad_out.shape)}")
-    g = _dense(grad_out)
+    g = _dense(grad_out, gd)
     w = None if weights is None else _pair_weights(weights, order, device)
     grad_rows = torch.empty_like(rows)
     grad_w = torch.empty(n, top_k, dtype=torch.float32, device=device)
@@ -275,15 +279,16 @@ def add_rms_norm_q8(resid: torch.Tensor, delta: Optional[torch.Tensor], weight: 
     if len(shape) != 2:
         raise ValueError("resid must be [n, H]")
     n, H = shape
-    _at_most(_MAX_INT, n, H)
+    if n > _MAX_INT or H > _MAX_INT:
+        raise _too_large(_MAX_INT, n, H)
     rd = _typed("resid", resid, device)
-    r = _dense(resid)
+    r = _dense(resid, rd)
     d = dd = None
     if delta is not None:
         dd = _typed("delta", delta, device)
         if delta.shape != shape:
             raise ValueError(f"delta must be {(n, H)}, got {tuple(delta.shape)}")
-        d = _dense(delta)
+        d = _dense(delta, dd)
     w = None
     if weight is not None:
         if not isinstance(weight, torch.Tensor) or weight.device != device or weight.shape != (H,):
@@ -335,7 +340,8 @@ def adapters_add(base: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.
     n = x.shape[0] if x.dim() == 2 else -1
     if n < 0 or x.shape[1] != K or base.shape != (n, N):
         raise ValueError(f"x must be [n, {K}] and base [n, {N}], got {tuple(x.shape)} and {tuple(base.shape)}")
-    _at_most(_MAX_INT, n, K, N, r)
+    if n > _MAX_INT or K > _MAX_INT or N > _MAX_INT or r > _MAX_INT:
+        raise _too_large(_MAX_INT, n, K, N, r)
     if not isinstance(ids, torch.Tensor) or ids.device != device or ids.numel() != n:
         raise ValueError(f"ids must be [{n}] on {device}")
     if L > _MAX_EXPERTS:
@@ -345,9 +351,7 @@ def adapters_add(base: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.
         if not isinstance(scales, torch.Tensor) or scales.device != device or scales.numel() != L:
             raise ValueError(f"scales must be [{L}] on {device}")
         s = _f32(scales)
-    if x.is_neg() or base.is_neg():
-        x, base = x.resolve_neg(), base.resolve_neg()
-    (x, xp), (a, ap), (b, bp), (base, basep) = _aligned(x), _aligned(a), _aligned(b), _aligned(base)
+    (x, xp), (a, ap), (b, bp), (base, basep) = _aligned(x, xd), _aligned(a, BF16), _aligned(b, BF16), _aligned(base, od)
     ids = _ids("ids", ids if ids.dim() == 1 else ids.reshape(-1))
     if order is not None:
         _ordered(order, device)
@@ -371,9 +375,9 @@ def adapters_add(base: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.
     return out
 
 
-def _aligned(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
+def _aligned(t: torch.Tensor, dtype: int) -> Tuple[torch.Tensor, int]:
     """The tensor contiguous and from a 16-byte boundary on (a view may begin anywhere), and its address."""
-    t = t.contiguous()
+    t = _dense(t, dtype)
     p = t.data_ptr()
     if p % 16:
         t = t.clone()
