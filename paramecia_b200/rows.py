@@ -227,6 +227,8 @@ def combine_rows(rows: torch.Tensor, order: ExpertOrder, weights: Optional[torch
         out = torch.empty(n, H, dtype=out_dtype or rows.dtype, device=device)
     else:
         _check_out(out, (n, H), tuple(_TYPES), device)
+        if out_dtype is not None and _out_type("out_dtype", out_dtype) != _TYPES[out.dtype]:
+            raise ValueError(f"out is {out.dtype}, out_dtype {out_dtype}")
         _apart("rows", out, rows)
         _apart("extra", out, e, same=True)
         _apart("weights", out, w)

@@ -145,3 +145,13 @@ def test_views_that_negate_or_conjugate():
         assert torch.equal(pm.adapters_add(v, v, a, b, first), pm.adapters_add(plain, plain, a, b, first))
     with pytest.raises(ValueError):
         pm.combine_rows(want, o, out=torch._neg_view(torch.zeros((30, 64), device=DEV)))
+
+
+def test_an_out_of_another_type_than_out_dtype_is_refused():
+    o = pm.sort_by_expert(torch.zeros((4, 2), dtype=torch.int32, device=DEV), 3)
+    rows, out = torch.ones((8, 16), device=DEV), torch.zeros((4, 16), dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(ValueError, match="out_dtype"):
+        pm.combine_rows(rows, o, out_dtype=torch.float32, out=out)
+    with pytest.raises(pm.PmoeError):
+        pm.combine_rows(rows, o, out_dtype=torch.float16, out=out)
+    assert pm.combine_rows(rows, o, out_dtype=torch.bfloat16, out=out) is out and (out == 2).all()
