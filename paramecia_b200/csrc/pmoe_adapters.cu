@@ -762,18 +762,18 @@ __global__ void __launch_bounds__(TC_THREADS, 1) k_adapters_tc(AdapterArgs P, co
             const int row = i / RT, k8 = i % RT;
             const float4 u = sum_of_cluster<CTAS>(cluster, part + row * S::PS + k8 * 8), v = sum_of_cluster<CTAS>(cluster, part + row * S::PS + k8 * 8 + 4);
             uint32_t w[4][PIECES];
-            const bool rank = k8 * 8 < P.r;   // ranks behind r are zeros, also where x is infinite
-            split_pair(rank ? u.x * scale : 0.f, rank ? u.y * scale : 0.f, w[0]);
-            split_pair(rank ? u.z * scale : 0.f, rank ? u.w * scale : 0.f, w[1]);
-            split_pair(rank ? v.x * scale : 0.f, rank ? v.y * scale : 0.f, w[2]);
-            split_pair(rank ? v.z * scale : 0.f, rank ? v.w * scale : 0.f, w[3]);
+            const uint32_t rank = k8 * 8 < P.r ? ~0u : 0u;   // ranks behind r are zeros, also where x is infinite
+            split_pair(u.x * scale, u.y * scale, w[0]);
+            split_pair(u.z * scale, u.w * scale, w[1]);
+            split_pair(v.x * scale, v.y * scale, w[2]);
+            split_pair(v.z * scale, v.w * scale, w[3]);
             uint8_t *at = hs + k8 / 8 * (TC_M * 128) + row * 128 + ((k8 % 8 ^ row % 8) << 4);
 #pragma unroll
             for (int o = 0; o < CTAS; o++) {
                 uint8_t *there = cluster.map_shared_rank(at, o);
 #pragma unroll
                 for (int p = 0; p < PIECES; p++)
-                    *reinterpret_cast<uint4 *>(there + p * S::KB * TC_M * 128) = make_uint4(w[0][p], w[1][p], w[2][p], w[3][p]);
+                    *reinterpret_cast<uint4 *>(there + p * S::KB * TC_M * 128) = make_uint4(w[0][p] & rank, w[1][p] & rank, w[2][p] & rank, w[3][p] & rank);
             }
         }
     });
