@@ -364,7 +364,8 @@ int pmoe_combine_rows_grad(int device, const void *grad_out, int grad_dtype, con
  * must not overlap x); a [n_adapters, rank, K] and b [n_adapters, N, rank] BF16; scales [n_adapters] f32 or NULL (all ones); ids [n] int32.
  * order and offsets: pmoe_sort_pairs of ids (top_k 1, expert_base 0, E = n_adapters), which a host computes once for all
  * projections of a batch, or both NULL for n <= 1024.  K and N multiples of 8, rank a multiple of 8 up to 128, all
- * pointers 16-byte aligned.  Products are exact bf16 products summed in f32; f32 rows lose nothing.
+ * pointers 16-byte aligned.  Products are exact bf16 products summed in f32: f32 rows and A x keep all their bits as three bf16
+ * pieces.  The sums are the matrix instructions', which cut where f32 arithmetic rounds (about 3e-7 of an f32 result).
  */
 int pmoe_adapters_add(int device, const void *base, const void *x, int x_dtype, int n, int K, int N, int rank, int n_adapters,
                       const void *a, const void *b, const float *scales, const int *ids, const int *order, const int *offsets, void *out,

@@ -202,8 +202,8 @@ __device__ inline void find_tile(const AdapterArgs &P, int slot, int *rows, int 
 }
 
 // From the ids alone: every CTA counts them, then looks for the rows of its own tile.  A sort in front is a launch of its own,
-// 4 us for few rows (1000 rows, 4 adapters of rank 64: 16.3 us without it, 20.7 us with it), but it reads the ids once where
-// here every CTA does: 8192 rows take 56 us without and 47 us with it.
+// 4 us for few rows (1000 rows, 4 adapters of rank 64: 16.7 us without it, 20.9 us with it; 1024 rows, 16 adapters: 18.6 and 17.6), but it
+// reads the ids once where here every CTA does: 8192 rows took 56 us without and 47 us with it.
 // offsets: L + 1 words of shared memory
 template <int T, int THREADS>
 __device__ inline void find_tile_by_ids(const AdapterArgs &P, int slot, int *rows, int &tile_id, int &tile_rows, int &tile_first, int *offsets)
@@ -268,7 +268,7 @@ __device__ inline void find_tile_by_ids(const AdapterArgs &P, int slot, int *row
 // holds what the matrix instructions of a chunk need, as the lanes need it (sixteen bytes per lane, lanes side by side, so no
 // access meets a bank twice), and a warp reads what its own lanes fetched.  The copies are asynchronous and STAGES stages are on
 // their way, the first ones of N while the shares of h are still being added: one decoding row of 2048 x 2048 takes 5 us, 64
-// rows with 36 adapters of rank 32 (2048 to 4096) 9.7 us, which is the chain id -> rows -> h -> exchange -> columns.
+// rows with 36 adapters of rank 32 (2048 to 4096) 10.1 us, which is the chain id -> rows -> h -> exchange -> columns.
 // RT: groups of eight ranks that the accumulators are sized for.
 constexpr int FEW_M = 16, FEW_THREADS = 128;
 
@@ -593,7 +593,14 @@ __global__ void __launch_bounds__(FEW_THREADS, RT == 16 ? 1 : 4) k_adapters(Adap
 // issues the products, and a chunk's sums are read, added to base and stored while the next chunk's product runs.  The
 // columns of B lie permuted in shared memory so that a lane reads eight consecutive ones of a row.
 constexpr int TC_M = 128, TC_THREADS = 256;
-constexpr int TC_MIN_ROWS = 96;   // rows an adapter has on average
+// Rows an adapter has on average from which these tiles are taken.  K = N = 2048, bf16, us of 16-row and 128-row tiles, 16 adapters in sorted order:
+//   rows an adapter    64          96          128         192         512
+//   rank 16         8.5 / 29    15 / 29     10 / 18     19 / 20     31 / 31
+//   rank 64         13 / 28     24 / 29     19 / 20     37 / 21     58 / 34
+//   rank 128        21 / 36     38 / 38     31 / 26     60 / 27    118 / 42
+// The crossing lies between 96 and 192 for ranks of 64 and more and at 512 for rank 16; with four adapters or one, whose tiles of 128 do not
+// fill the card, 16-row tiles stay ahead to 512 rows (four of rank 64: 19 / 29).  96 is the lower end of that range.
+constexpr int TC_MIN_ROWS = 96;
 
 // Waits that ran out, of all streams since the library was loaded (pmoe_rows_status), and where the last one was
 struct Failures {
@@ -919,7 +926,13 @@ static cudaError_t launch_clusters(Kern kern, std::atomic<uint64_t> &asked, int 
 
 // The cluster's size: more CTAs share a tile's K and N (`shared` of work), each with the same work around it (finding the
 // tile, the exchange of h: `around`).  Taken is the size with the shortest sum over the waves that the grid makes: eight where
-// the rows are few, one or two where the tiles alone fill the card's `room`.
+// the rows are few, one or two where the tiles alone fill the card's `room`.  Measured, us with clusters of 1, 2, 4, 8 CTAs (* is taken):
+//   16-row tiles: 1 row 12.2 8.2 6.1 5.1*; 64 rows of 48 ids 18.6 11.7 11.9 11.6*; 128 rows of as many ids, rank 64 19.7 19.2 25.1* 41.7;
+//     1024 f32 rows of 4 ids 29.9 20.5 18.5* 32.1; 4096 f32 rows of 12 ids 28.0* 29.1 32.1 41.7; 8192 rows of 100 ids 80.6* 86.3 108 189
+//   128-row tiles: 1024 rows of 4 ids 46.9 28.4 19.2 16.8*; 2048 rows of 4 ids 46.8 27.5 18.4 28.5*; 8192 rows of 12 ids 50.2 33.1* 59.1 84.1;
+//     16384 rows of 12 ids, rank 16 49.8* 58.1 78.4 155
+// The sum takes `room` for as many SMs as the card has.  Clusters of eight with a CTA an SM fill it less than that, and slots without a tile are not
+// counted, which costs 10 us in the case of 2048 rows and 6 in that of 128.
 static int cluster_size(int64_t tiles, int64_t room, double around, double shared)
 {
     int ctas = AD_MAX_CTAS;

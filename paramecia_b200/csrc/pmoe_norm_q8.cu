@@ -29,9 +29,9 @@ __device__ inline double max_nan(double m, double v) { return v > m || v != v ? 
 // How a group becomes 8 bits.  With u = r * weight and top = max |u| over the group, v = u / m and
 //   scale = max |v| / 127 = top * (1 / m) / 127,   v / scale = u * (127 / top):
 // the quotient needs neither m nor the rounded scale, which saves two products an element and lets both statistics be
-// reduced at once.  For int8 it is taken in f32 (u, top, 127 / top: three roundings, where dividing v by its scale takes five).
-// The 8-bit floats are what a consumer multiplies as they are, so there q is the rounding of the exact quotient: every
-// value is rounded twice, from a quotient that is certainly too small and one that is certainly too large, and where the
+// reduced at once.  For int8 it is taken in f32 (u, top, 127 / top: three roundings, where dividing v by its scale takes five): a
+// value within 2^-15 of the middle between two steps may become either (of 24 million values none was another than the exact
+// quotient's).  An e4m3 q is the rounding of the exact quotient: every value is rounded twice, from a quotient that is certainly too small and one that is certainly too large, and where the
 // two differ, as for one value in 10^5, the group is done again in 64 bits from the row as it was stored.
 constexpr float BELOW = 1.f - 0x1.6p-22f, ABOVE = 1.f + 0x1.6p-22f;   // five roundings of 2^-24 and a little
 
@@ -125,14 +125,15 @@ __device__ inline void add_and_store(float (&v)[8], const float (&d)[8], __nv_bf
     if (to) *reinterpret_cast<uint4 *>(to) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// One CTA per row.  The operator reads and writes each element once (13 bytes for f32 + f32 -> f32, int8, f32 values; 7 for
-// bf16 + bf16 -> bf16, e4m3), so memory bounds it and the row must stay on the chip between its two statistics: here in
+// One CTA per row.  The operator reads and writes each element once (17 bytes for f32 + f32 -> f32, int8, f32 values, 13 without
+// values; 7 for bf16 + bf16 -> bf16, e4m3), so memory bounds it and the row must stay on the chip between its two statistics: here in
 // registers, eight consecutive elements a thread and pass, a row never longer than threads * PASSES * 8.  A group is 4, 8, 16
 // or 32 neighbouring threads of a pass (its maximum by shuffles) or the whole row (shuffles and a shared array).  The second
-// limit is the issue rate: with two quotients an element 16384 rows of 2048 took 126 us.  Now 51 us, 0.72 of the
-// measured copy rate.
+// limit is the issue rate: with two quotients an element 16384 rows of 2048 bf16 took 126 us to e4m3.  Now 51 us, 0.72 of the
+// measured copy rate, with 44 instructions an element in 85 % of the issue slots; to int8 45 us, 0.81 of it, and from f32 rows 67 to 71 us, 0.95 and more.
+// Where many quotients are ties (bf16 rows without weights) the 64-bit part runs for most rows: 87 us by groups of 128, 97 us by rows.
 // THREADS: the most a launch has.  With one pass the registers are held to what fills an SM (2048 threads): the part in 64 bits wants
-// twice as many, and with them 16384 rows took 60 us for 51.
+// twice as many.  It is compiled in with 192 to 240 bytes of spills a thread for e4m3; with the registers 16384 rows took 60 us for 51.
 template <typename RT, typename DT, typename VT, bool E4M3, int PASSES, int THREADS>
 __global__ void __launch_bounds__(THREADS, PASSES == 1 ? 2048 / THREADS : 1) k_norm_q8(const RT *resid_in, const DT *__restrict__ delta, const float *__restrict__ weight, int H,
                                                   float eps, int group, RT *resid_out, uint8_t *__restrict__ q,
@@ -317,7 +318,8 @@ __global__ void __launch_bounds__(THREADS, PASSES == 1 ? 2048 / THREADS : 1) k_n
 
 // Rows that no vector load fits (H not a multiple of 8, or an address off its boundary).  A warp has 256 consecutive
 // elements a pass, lane l those at l, l + 32, ...: its loads are whole lines whatever the address, and a group of 32 to
-// 256 values is one to eight registers of a warp.
+// 256 values is one to eight registers of a warp.  16384 rows of 2047, us: f32 to int8 95 by rows and 113 by groups of 128; bf16 to int8 121 and
+// 141, to e4m3 158 and 178, and 266 and 356 where most rows hold ties: an element a load, a store and a conversion.
 template <typename RT, typename DT, typename VT, bool E4M3>
 __global__ void __launch_bounds__(1024) k_norm_q8_any(const RT *resid_in, const DT *__restrict__ delta, const float *__restrict__ weight,
                                                       int H, float eps, int group, RT *resid_out, uint8_t *__restrict__ q,

@@ -28,13 +28,15 @@ namespace cg = cooperative_groups;
 //   2. the CTAs' totals are exchanged through distributed shared memory; scans over (e, CTA, w): cnt[w][e] becomes the
 //      place of that warp's first pair of e among this CTA's pairs, shift[e] what leads from there to the place among all
 //   3. the runs once more: place = cnt[w][e] + rank inside the step + shift[e]
-// The pairs are few bytes (4 to read, 8 to write): what counts is latency and the work of the eight SMs.
+// The pairs are few bytes (4 to read, 8 to write): what counts is latency up to some 40960 pairs, and beyond the work of the eight SMs,
+// about 4 us for each further 40960; from 131073 pairs on a run has more steps than a lane keeps, and its keys are read twice.
 // - A lane loads its keys of sixteen steps at once and keeps them, with their ranks, from 1. to 3. where the run is no longer.
 // - The lanes of a step with the same expert meet in a mask in shared memory, one word per warp and expert (__match_any_sync
 //   and ballots over the bits of the expert's number took 2000 and 1300 cycles a step with 32 warps an SM).
 // - The pairs are written to `order` from shared memory, where 3. leaves them in this CTA's order: neighbours of an
 //   expert then leave in one sector instead of one each.
-// 40960 pairs of 512 experts: 17 us with __match_any_sync, 12.6 us with ballots and direct writes, now 10.7 us (81920: 30, 19, 14.6 us).
+// 40960 pairs of 512 experts: 17 us with __match_any_sync, 12.6 us with ballots and direct writes, now 10.6 us (81920: 30, 19, 14.5 us).
+// 163840: 29 us; 40960 of 128 experts: 9.9 us.  1024 threads leave 64 registers each: the cluster's form spills 64 bytes a thread, the other 20.
 constexpr int SORT_MAX_E = 4096;
 constexpr int SORT_THREADS = 1024;
 constexpr int SORT_CTAS = 8;

@@ -14,7 +14,8 @@ per-expert adapters, a training step); ``MoeBlock`` does all of it inside its ke
     grad_x = dispatch_rows_grad(grad_xs, order)
 
 Nothing here waits for the GPU or reads a count back: sizes depend on the shapes alone.  These are plain functions on device
-memory, as everything in this package is: autograd does not record them, and the gradients are the ones above.
+memory, as everything in this package is: autograd does not record them, and the gradients are the ones above.  Inputs that
+require a gradient are taken (experts of torch's between the two ends give such rows); the results are detached.
 """
 from __future__ import annotations
 
