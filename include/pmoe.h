@@ -316,8 +316,9 @@ int pmoe_add_rms_norm(int device, const float *resid_in, const float *delta, con
  *   a group of zeros has scale 0 and zeros.  values (NULL = not wanted) = q * scale in F32 or BF16.
  * resid_in, resid_out [n, H] F32 or BF16; delta [n, H] F32 or BF16; q [n, H] bytes; scales [n, ceil(H / group)] f32.
  * group is 32, 64, 128, 256 or 0 for the whole row (the last group of a row may be short); H <= 16384.  A group that
- * holds an infinity or a NaN has a scale that is not finite, and zeros.  Sums and the norm are f32; an E4M3 q is the rounding
- * of the exact quotient (r * weight) / (max |r * weight| / 448), an I8 q that of the quotient in f32.
+ * holds an infinity or a NaN, or whose r * weight overflows f32, has a scale that is not finite, and zeros.  Sums and the norm
+ * are f32; an E4M3 q is the rounding of the exact quotient (r * weight) / (max |r * weight| / 448), an I8 q that of the
+ * quotient in f32.
  */
 int pmoe_add_rms_norm_q8(int device, const void *resid_in, int resid_dtype, const void *delta, int delta_dtype, const float *weight,
                          int n, int H, float eps, int group, void *resid_out, int q_dtype, void *q, float *scales, void *values,
